@@ -198,6 +198,113 @@ int   slate_hip_attention_ragged(float* out, const float* q, const float* Kpool,
                                  int T, int n_q_heads, int n_kv_heads, int head_dim,
                                  int64_t head_stride, int max_pos);
 
+/* Rotary positions beyond rope_rows: pairs in halves or interleaved, part of
+ * a head, frequencies rescaled for contexts longer than the trained one, any
+ * position.  Pair i < rot_dim/2 turns by pos * w_i and is multiplied by
+ * `magnitude`; the elements past rot_dim are copied.  w_i starts as
+ * theta_base^(-2i/rot_dim) and `scaling` changes it:
+ *   0  not at all;
+ *   1  w_i / factor (every position is divided);
+ *   2  by how often the pair turns in the trained context, t = orig_ctx * w_i
+ *      / 2 pi: t <= low gives w_i / factor, t >= high keeps w_i, in between
+ *      the two are mixed linearly in t;
+ *   3  (YaRN) by the pair's index: the pairs that turn `high` and `low` times
+ *      are x(t) = rot_dim * ln(orig_ctx / (2 pi t)) / (2 ln theta_base); up
+ *      to a = max(0, floor x(high)) w_i is kept, from b = min(rot_dim - 1,
+ *      ceil x(low)) on it is w_i / factor, in between mixed linearly in i.
+ * Angles are formed and reduced to one turn in 64 bits, so far positions are
+ * as exact as near ones; the rotation is in f32. */
+typedef struct slate_hip_rope {
+    int    layout;      /* 0: pairs (i, i + rot_dim/2) as rope_rows, 1: pairs (2i, 2i + 1) */
+    int    rot_dim;     /* even, 2 .. min(head_dim, 512) */
+    int    scaling;     /* 0 .. 3, above */
+    int    orig_ctx;    /* scaling 2 and 3: positions of the trained context, >= 1 */
+    double theta_base;  /* > 0 (scaling 3: > 1) */
+    double factor;      /* scaling 1 .. 3: > 0 */
+    double low, high;   /* scaling 2 and 3: turns, 0 < low < high */
+    double magnitude;   /* 0: the default, 0.1 ln(factor) + 1 for scaling 3 (1 where factor <= 1), else 1 */
+} slate_hip_rope_t;
+/* y[row, head, :] = the rotated x[row, head, :]; rows are ld floats apart in
+ * both (ld >= n_heads * head_dim).  pos is device int32[n_rows], any value: a
+ * negative position turns backwards (the transpose of the rotation, which is
+ * also its gradient; `magnitude` multiplies either way).  y is x (in place)
+ * or does not overlap it. */
+int   slate_hip_rope_scaled(float* y, const float* x, const int32_t* pos, int n_rows, int n_heads, int head_dim,
+                            int64_t ld, const slate_hip_rope_t* rope);
+/* The w_i (host double[rot_dim/2]) and the magnitude behind rope_scaled;
+ * host only, needs no device.  -1 for a configuration rope_scaled refuses. */
+int   slate_hip_rope_frequencies(double* w, double* magnitude, const slate_hip_rope_t* rope);
+
+/* ---- packed batches over an 8-bit K/V cache, and drafted tokens ------------
+ * The entries below take a batch as pack_batch lays it out: B sequences
+ * (1 .. 1024) of T token rows in all, sequence b's tokens being the rows
+ * tok_off[b] .. tok_off[b+1]-1 (device int32[B+1], not falling); pos0[b]
+ * (device int32[B]) rows of it are cached already, and its token i belongs to
+ * cache row pos0[b] + i.  Row p of kv head h starts at element
+ * kv_base[b] + h * head_stride + p * head_dim of a pool (device int64[B];
+ * offsets may pass 32 bits).  A sequence may have no token in a call.  One whose
+ * numbers do not fit (tok_off falling or outside 0 .. T, more than max_new
+ * tokens where the call has that bound, pos0 < 0, pos0 + tokens > max_seq,
+ * kv_base < 0) is left out: nothing of it is read or written.  Rows of the
+ * outputs that no sequence owns stay as they were.
+ * The 8-bit pools: int8 codes (device, 16-byte aligned), and the f16 steps
+ * (uint16_t bits, 16-byte aligned) of each 32 codes, the step of element e
+ * at index e / 32.  A value is step * code: the values of Q8_0, in two pools
+ * so that rows are read in whole 16-byte loads.  In these pools kv_base and
+ * head_stride are multiples of head_dim (a kv_base that is not is rounded down
+ * to one) and head_dim is a multiple of 32. */
+
+/* Quantise new K and V rows into the cache: k, v [T, n_kv_heads * head_dim]
+ * f32 (16-byte aligned), rows ld floats apart (ld % 4 == 0).  Per 32 elements
+ * step = f16(max|x| / 127) (at most 65504) and code = x / step to the nearest
+ * whole number, ties to even, within -127 .. 127; a block whose step rounds
+ * to 0 gets codes 0.  NaN counts as 0. */
+int   slate_hip_kv_store_q8(int8_t* Kq, uint16_t* Ks, int8_t* Vq, uint16_t* Vs, const float* k, const float* v,
+                            int64_t ld, const int32_t* tok_off, const int32_t* pos0, const int64_t* kv_base, int B,
+                            int T, int n_kv_heads, int head_dim, int64_t head_stride, int max_seq);
+/* The same rows of the cache back as f32 (step * code, exact in f32). */
+int   slate_hip_kv_load_q8(float* k, float* v, int64_t ld, const int8_t* Kq, const uint16_t* Ks, const int8_t* Vq,
+                           const uint16_t* Vs, const int32_t* tok_off, const int32_t* pos0, const int64_t* kv_base,
+                           int B, int T, int n_kv_heads, int head_dim, int64_t head_stride, int max_seq);
+/* Causal GQA attention over the 8-bit cache: q, out [T, n_q_heads * head_dim]
+ * f32 (out is not q); token i of sequence b attends to rows 0 .. pos0[b] + i
+ * (its own is stored before the call).  n_q_heads is a multiple of
+ * n_kv_heads; query head g belongs to kv head g / (n_q_heads / n_kv_heads).
+ * Scores are q.k / sqrt(head_dim), as attention_ragged's.  max_new bounds the
+ * tokens that one sequence brings (1 for a decode step); head_dim is at most
+ * 512.  Queries must be finite and below 2^100 in size.  What the cache holds
+ * in rows a token does not see never matters.
+ * ws: device scratch of slate_hip_attention_packed_bytes, 16-byte aligned, for calls that run beside
+ * each other or are captured into graphs that do; NULL takes the backend's
+ * own, which calls on the backend stream share (a call under stream capture
+ * is then refused with -5). */
+int   slate_hip_attention_ragged_q8(float* out, const float* q, const int8_t* Kq, const uint16_t* Ks,
+                                    const int8_t* Vq, const uint16_t* Vs, const int32_t* tok_off,
+                                    const int32_t* pos0, const int64_t* kv_base, int B, int T, int max_new,
+                                    int n_q_heads, int n_kv_heads, int head_dim, int64_t head_stride, int max_seq,
+                                    void* ws, size_t ws_bytes);
+/* Attention of drafted tokens that form trees: sequence b's tokens are drafts
+ * after its pos0[b] committed rows, K/V of draft i stored in row pos0[b] + i.
+ * parent[t] (device int32[T]) is the draft, counted within its sequence, that
+ * token t continues, or -1 where it continues the committed text; it comes
+ * before its child (parent[t] < the token's own number; any other value is
+ * taken as -1).  A token attends to the committed rows, to its ancestors and
+ * to itself.  max_new <= 1024.  K/V in f32 pools as attention_ragged's
+ * (kv_base and head_stride any), or in the 8-bit pools; head_dim of f32
+ * pools is a multiple of 16. */
+int   slate_hip_attention_tree(float* out, const float* q, const float* Kpool, const float* Vpool,
+                               const int32_t* tok_off, const int32_t* pos0, const int64_t* kv_base,
+                               const int32_t* parent, int B, int T, int max_new, int n_q_heads, int n_kv_heads,
+                               int head_dim, int64_t head_stride, int max_seq, void* ws, size_t ws_bytes);
+int   slate_hip_attention_tree_q8(float* out, const float* q, const int8_t* Kq, const uint16_t* Ks,
+                                  const int8_t* Vq, const uint16_t* Vs, const int32_t* tok_off,
+                                  const int32_t* pos0, const int64_t* kv_base, const int32_t* parent, int B, int T,
+                                  int max_new, int n_q_heads, int n_kv_heads, int head_dim, int64_t head_stride,
+                                  int max_seq, void* ws, size_t ws_bytes);
+/* Bytes of ws that the three take for these heads, whatever the batch; -1 for
+ * heads they refuse. */
+int64_t slate_hip_attention_packed_bytes(int n_q_heads, int n_kv_heads, int head_dim);
+
 /* Synthetic weights generated on the device (seeded, ~N(0, std)):
  * f32 values, or rows x cols quantised to Q4_K. */
 int   slate_hip_synth_f32(float* dst, int64_t n, uint64_t seed, float std);

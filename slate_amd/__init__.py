@@ -55,6 +55,12 @@ class LlamaLayer(C.Structure):          # slate_hip_llama_layer_t == llama.h:69-
                                        "ffn_down_dtype")]
 
 
+class RopeConfig(C.Structure):          # slate_hip_rope_t
+    _fields_ = [("layout", C.c_int), ("rot_dim", C.c_int), ("scaling", C.c_int), ("orig_ctx", C.c_int),
+                ("theta_base", C.c_double), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("magnitude", C.c_double)]
+
+
 # name -> (restype, argtypes) for every exported entry point
 SIGNATURES = {
     "slate_backend_hip": (C.POINTER(BackendStruct), []),
@@ -95,6 +101,15 @@ SIGNATURES = {
                                        vp, vp, vp, vp, vp, vp]),
     "slate_hip_attention_ragged": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, C.c_int, C.c_int,
                                              C.c_int, C.c_int, C.c_int64, C.c_int]),
+    "slate_hip_rope_scaled": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int64,
+                                        C.POINTER(RopeConfig)]),
+    "slate_hip_rope_frequencies": (C.c_int, [vp, C.POINTER(C.c_double), C.POINTER(RopeConfig)]),
+    "slate_hip_kv_store_q8": (C.c_int, [vp] * 6 + [C.c_int64] + [vp] * 3 + [C.c_int] * 4 + [C.c_int64, C.c_int]),
+    "slate_hip_kv_load_q8": (C.c_int, [vp] * 2 + [C.c_int64] + [vp] * 7 + [C.c_int] * 4 + [C.c_int64, C.c_int]),
+    "slate_hip_attention_ragged_q8": (C.c_int, [vp] * 9 + [C.c_int] * 6 + [C.c_int64, C.c_int, vp, C.c_size_t]),
+    "slate_hip_attention_tree": (C.c_int, [vp] * 8 + [C.c_int] * 6 + [C.c_int64, C.c_int, vp, C.c_size_t]),
+    "slate_hip_attention_tree_q8": (C.c_int, [vp] * 10 + [C.c_int] * 6 + [C.c_int64, C.c_int, vp, C.c_size_t]),
+    "slate_hip_attention_packed_bytes": (C.c_int64, [C.c_int] * 3),
     "slate_hip_synth_f32": (C.c_int, [vp, C.c_int64, C.c_uint64, C.c_float]),
     "slate_hip_synth_q4k": (C.c_int, [vp, C.c_int64, C.c_int64, C.c_uint64, C.c_float]),
     "slate_hip_llama_new": (vp, [C.POINTER(LlamaConfig), vp, vp, vp, C.c_int,
