@@ -3,12 +3,10 @@
 //
 // out = sum_k exp(s_k - m) V_k / sum_k exp(s_k - m), s_k = q.K_k / sqrt(hd),
 // over the keys that the token sees.
+#include "attn_plan.h"
 #include "lanes.h"
-#include "packed.h"
 
 namespace slate_hip {
-
-constexpr float LOG2E = 1.4426950408889634f;
 
 // One workgroup per (token, query head), its four waves taking every fourth
 // key: a wave's lanes share the key's elements, with an online softmax per
@@ -95,9 +93,14 @@ __global__ __launch_bounds__(256) void attn_packed_rows_kernel(PackedAttn a, Pac
     }
 }
 
-int64_t attention_packed_bytes(int, int, int) { return 0; }
+int64_t attention_packed_bytes(int Hq, int Hkv, int hd) {
+    return attention_q8_few_shape(hd, Hq / Hkv) ? attention_q8_few_bytes(hd) : 0;
+}
 
 int launch_attention_packed(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
+    const int G = a.Hq / a.Hkv;
+    if (!a.kf && attention_q8_few_shape(a.hd, G) && pb.max_new * (int64_t)G <= 16)
+        return launch_attention_q8_few(a, pb, s);
     hipLaunchKernelGGL(attn_packed_rows_kernel, dim3(pb.T, a.Hq), dim3(256), 0, s, a, pb);
     SH_CHECK_LAUNCH();
     return 0;

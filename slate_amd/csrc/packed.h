@@ -72,6 +72,11 @@ struct PackedAttn {
     void* ws;
 };
 int64_t attention_packed_bytes(int Hq, int Hkv, int hd);
+// k_attn_q8.hip: the sequences of at most 16 query rows per kv head, 8-bit
+// pools; the others' rows stay as they are.
+bool attention_q8_few_shape(int hd, int G);
+int64_t attention_q8_few_bytes(int hd);
+int launch_attention_q8_few(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
 int launch_attention_packed(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
 
 }  // namespace slate_hip
