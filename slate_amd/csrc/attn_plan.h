@@ -3,31 +3,31 @@
 // The keys of every (sequence, kv head, block of query rows) are counted in
 // granules and laid end to end; workgroup w of P takes the granules
 // [N w / P, N (w+1) / P) of that line.  So every workgroup reads the same
-// amount to within a granule whatever the lengths are, and at most the first
-// and the last piece of its range are parts of a block whose rest lies in a
-// neighbour's: two slots of partial results per workgroup, whatever the
+// amount to within a granule whatever the lengths are, and only the first
+// and the last piece of its range can be parts of a block whose rest lies in
+// its neighbours': two slots of partial results per workgroup, whatever the
 // batch.  A block that lies inside one range is written straight out.
-// Every wave works the plan out by itself from the descriptors.
+// Every wave works the plan out by itself from the descriptors, which a lane
+// each loads once; N < 2^31 (the entries check it).
 #pragma once
+#include "lanes.h"
 #include "packed.h"
 
 namespace slate_hip {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
+// Inclusive sum over the wave's lanes (DPP: within rows of 16, then across).
+__device__ __forceinline__ int wave_scan(int v) {
+#define SH_SCAN_STEP(ctrl, rows) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xF, false)
+    SH_SCAN_STEP(0x111, 0xF);          // row_shr:1, 2, 4, 8
+    SH_SCAN_STEP(0x112, 0xF);
+    SH_SCAN_STEP(0x114, 0xF);
+    SH_SCAN_STEP(0x118, 0xF);
+    SH_SCAN_STEP(0x142, 0xA);          // row_bcast:15 into rows 1 and 3
+    SH_SCAN_STEP(0x143, 0xC);          // row_bcast:31 into rows 2 and 3
+#undef SH_SCAN_STEP
     return v;
-}
-__device__ __forceinline__ int64_t read_lane64(int64_t v, int lane) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
-    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)v >> 32), lane);
-    return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
 // A value that is the same in all lanes, for the scalar registers.
@@ -38,49 +38,79 @@ __device__ __forceinline__ T* uniform(T* p) {
                 (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 
-// A place on the line: granule `at` of sequence b's `count`.
+// A place on the line: granule `at` of the sequence's `own`.
 struct Place {
-    int b;
-    int64_t at;
+    SeqView seq;
+    int64_t base;                      // kv_base
+    int at;
 };
 
 // Count(SeqView) -> granules of a sequence (all its heads and blocks).
 template <class Count>
-struct Plan {
-    const PackedBatch& pb;
-    const Count count;
-    int64_t own, upto;                 // the lane's sequence (of the first 64), and with those before it
-    int64_t total;
+class Plan {
+  public:
+    int total;
 
-    __device__ __forceinline__ Plan(const PackedBatch& pb_, const Count& c) : pb(pb_), count(c) {
-        load(0);
-        total = read_lane64(upto, 63);
-        for (int b0 = 64; b0 < pb.B; b0 += 64) total += read_lane64(wave_scan(of(b0)), 63);
-    }
-    __device__ __forceinline__ int64_t of(int b0) const {
-        const int b = b0 + (int)(threadIdx.x & 63);
-        return b < pb.B ? count(seq_view(pb, b)) : 0;
-    }
-    __device__ __forceinline__ void load(int b0) {
-        own = of(b0);
-        upto = wave_scan(own);
+    __device__ __forceinline__ Plan(const PackedBatch& pb, const Count& count) : pb_(pb), count_(count) {
+        first_ = load(0);
+        total = __builtin_amdgcn_readlane(first_.upto, 63);
+        for (int b0 = 64; b0 < pb.B; b0 += 64) total += __builtin_amdgcn_readlane(load(b0).upto, 63);
     }
     // 0 <= x < total
-    __device__ __forceinline__ Place find(int64_t x) const {
-        int64_t c = own, u = upto, base = 0;
-        for (int b0 = 0;;) {
-            const uint64_t past = __builtin_amdgcn_ballot_w64(base + u > x);
+    __device__ __forceinline__ Place find(int x) const {
+        Lane s = first_;
+        for (int b0 = 0, base = 0;;) {
+            const uint64_t past = __builtin_amdgcn_ballot_w64(base + s.upto > x);
             if (past) {
                 const int l = __builtin_ctzll(past);
-                return Place{b0 + l, x - base - (read_lane64(u, l) - read_lane64(c, l))};
+                const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)s.base, l);
+                const uint32_t hi = __builtin_amdgcn_readlane((int)((uint64_t)s.base >> 32), l);
+                return Place{{__builtin_amdgcn_readlane(s.seq.t0, l), __builtin_amdgcn_readlane(s.seq.n, l),
+                              __builtin_amdgcn_readlane(s.seq.p0, l)},
+                             (int64_t)((uint64_t)hi << 32 | lo),
+                             x - base - __builtin_amdgcn_readlane(s.upto - s.own, l)};
             }
-            base += read_lane64(u, 63);
+            base += __builtin_amdgcn_readlane(s.upto, 63);
             b0 += 64;
-            c = of(b0);
-            u = wave_scan(c);
+            s = load(b0);
         }
     }
-    __device__ __forceinline__ int64_t begin(int64_t w, int64_t P) const { return total * w / P; }
+    // First granule of workgroup w of P; with fewer granules than workgroups
+    // the first ones get one each.
+    __device__ __forceinline__ int begin(int w, int P) const {
+        return total < P ? min(w, total) : (int)((uint64_t)(uint32_t)total * (uint32_t)w / (uint32_t)P);
+    }
+
+  private:
+    struct Lane {
+        SeqView seq;
+        int64_t base;
+        int own, upto;                 // granules of the lane's sequence, and with those of the lanes before it
+    };
+    __device__ __forceinline__ Lane load(int b0) const {
+        const int b = b0 + (int)(threadIdx.x & 63);
+        Lane s{};
+        if (b < pb_.B) {
+            s.seq = seq_view(pb_, b);
+            s.base = pb_.kv_base[b];
+            s.own = count_(s.seq);
+        }
+        s.upto = wave_scan(s.own);
+        return s;
+    }
+    const PackedBatch& pb_;
+    const Count count_;
+    Lane first_;
+};
+
+// What the join kernel does at the boundary before workgroup w, left in the
+// workspace by that workgroup: the block that is cut there (if this is its first
+// cut), rows >= 1 of them.
+struct JoinEntry {
+    int t0, rows;                      // first token of the sequence, query rows (0: nothing to join)
+    int r0, h;                         // first row of the block, kv head
+    int pieces;                        // workgroups w - 1 .. w - 2 + pieces hold a part each
+    int slot0;                         // the slot of the first part
 };
 
 }  // namespace slate_hip

@@ -32,6 +32,7 @@ constexpr int AQ_ROWS = 16;            // query rows of a block
 constexpr int AQ_KEYS = 32;            // keys of a wave's step
 constexpr int AQ_GRAN = 4 * AQ_KEYS;   // keys of a workgroup's step
 constexpr int AQ_WGS = 512;            // two workgroups per CU (LDS)
+constexpr int AQ_KEEP = 4;             // blocks of up to this many granules are not cut
 constexpr float AQ_SLACK = 4.0f;       // log2 of the largest weight before the maximum moves
 constexpr int AQ_PEXP = 11;            // weights are scaled so that weight 1 times the largest V step is in [2^10, 2^11]
 
@@ -47,7 +48,9 @@ struct Q8Geom {
     static constexpr int ROWB = HD;                    // bytes of a row of codes
     static constexpr int TILE = AQ_KEYS * HD;          // bytes of a wave's K (or V) codes
     static constexpr int STEPS = AQ_KEYS * NB * 2;     // bytes of their steps
-    static constexpr int BUF = 2 * TILE + 2 * STEPS;
+    static constexpr int OS = HD + 4;                  // row stride of a wave's results in LDS (floats)
+    static constexpr int USED = 2 * TILE + 2 * STEPS;
+    static constexpr int BUF = USED > AQ_ROWS * OS * 4 ? USED : AQ_ROWS * OS * 4;
     static constexpr int CH = HD / 16;                 // 16-byte chunks of a row
     static constexpr int SH = HD == 128 ? 1 : HD == 64 ? 2 : 3;
 };
@@ -100,88 +103,148 @@ __device__ __forceinline__ int step_bits(_Float16 d) {
     return b < 0x7c00 ? b : 0;
 }
 
-// Granules of a sequence whose rows fit a block.
+__host__ __device__ inline int few_granules(int keys) { return (keys + AQ_GRAN - 1) / AQ_GRAN; }
+
+// Granules of a sequence whose rows fit a block (one block per kv head).
 struct FewCount {
     int G, Hkv;
-    __device__ __forceinline__ int64_t operator()(const SeqView& s) const {
-        if (s.n < 1 || (int64_t)s.n * G > AQ_ROWS) return 0;
-        return (int64_t)Hkv * ((s.p0 + s.n + AQ_GRAN - 1) / AQ_GRAN);
+    __device__ __forceinline__ int operator()(const SeqView& s) const {
+        return s.n < 1 || (int64_t)s.n * G > AQ_ROWS ? 0 : Hkv * few_granules(s.p0 + s.n);
     }
 };
+using FewPlan = Plan<FewCount>;
 
-// Partial slot: AQ_ROWS rows of HD outputs, then AQ_ROWS pairs (m, l).
+// Where workgroup w's range begins: N w / P, or the start of the block there
+// if it is short (it is not cut: the last workgroup that would begin in it
+// takes it whole).
+__device__ __forceinline__ int few_begin(const FewPlan& plan, int w) {
+    const int x = plan.begin(w, AQ_WGS);
+    if (x >= plan.total) return plan.total;
+    const Place pl = plan.find(x);
+    const int gran = few_granules(pl.seq.p0 + pl.seq.n), in = pl.at % gran;
+    return gran <= AQ_KEEP ? x - in : x;
+}
+
+// Workspace: a JoinEntry per workgroup, then two slots each of AQ_ROWS rows
+// of HD outputs and AQ_ROWS pairs (m, l).
 __host__ __device__ constexpr int64_t few_slot_floats(int hd) { return (int64_t)AQ_ROWS * (hd + 2); }
+constexpr int64_t FEW_ENTRIES = (int64_t)AQ_WGS * 32;  // bytes
+__device__ __forceinline__ float* few_slot(void* ws, int i, int hd) {
+    return (float*)((char*)ws + FEW_ENTRIES) + i * few_slot_floats(hd);
+}
 
 template <int HD>
 __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, PackedBatch pb) {
     using Geo = Q8Geom<HD>;
-    constexpr int NB = Geo::NB, ND = Geo::ND;
-    constexpr int OS = HD + 4;                         // row stride of the waves' results in LDS
+    constexpr int NB = Geo::NB, ND = Geo::ND, OS = Geo::OS;
+    struct alignas(2 * NB) Steps { _Float16 s[NB]; };
     __shared__ __attribute__((aligned(16))) unsigned char smem[8 * Geo::BUF];
     __shared__ float s_m[4][AQ_ROWS], s_l[4][AQ_ROWS];
-    static_assert(8 * Geo::BUF >= 4 * AQ_ROWS * OS * (int)sizeof(float), "results fit");
+    __shared__ int s_at[4];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, j = lane & 15;
     const int G = a.Hq / a.Hkv;
-    const Plan<FewCount> plan(pb, FewCount{G, a.Hkv});
-    const int64_t x0 = plan.begin(blockIdx.x, AQ_WGS), x1 = plan.begin(blockIdx.x + 1, AQ_WGS);
+    const FewPlan plan(pb, FewCount{G, a.Hkv});
+    const int x0 = few_begin(plan, blockIdx.x), x1 = few_begin(plan, blockIdx.x + 1);
+    JoinEntry* entry = (JoinEntry*)((char*)a.ws + 32 * blockIdx.x);
+    if (x0 >= x1) {
+        if (threadIdx.x == 0) entry->rows = 0;
+        return;
+    }
     const float scale2 = (1.0f / sqrtf((float)HD)) * LOG2E;
     unsigned char* buf0 = smem + w * 2 * Geo::BUF;
 
-    for (int64_t x = x0; x < x1;) {
+    // the piece being worked on, and the loads that are under way for one
+    struct Piece {
+        SeqView seq;
+        int h, gran, g0, g1;
+        const int8_t *kq, *vq;
+        const _Float16 *ks, *vs;
+    };
+    auto piece_at = [&](int x) {
         const Place pl = plan.find(x);
-        const SeqView sv = seq_view(pb, pl.b);
-        const int keys = sv.p0 + sv.n;
-        const int gran = (keys + AQ_GRAN - 1) / AQ_GRAN;
-        const int h = (int)(pl.at / gran), g0 = (int)(pl.at % gran);
-        const int g1 = (int)min((int64_t)gran, g0 + (x1 - x));
-        const int64_t row0 = (pb.kv_base[pl.b] + h * a.head_stride) / HD;
-        const int8_t *kq = a.kv8.kq + row0 * HD, *vq = a.kv8.vq + row0 * HD;
-        const _Float16 *ks = a.kv8.ks + row0 * NB, *vs = a.kv8.vs + row0 * NB;
-
-        // K and V rows of the wave's 32 keys from k0 on, into buffer `to`;
-        // rows past the last key repeat it (their weights are zero)
-        struct alignas(2 * NB) Steps { _Float16 s[NB]; };
-        Steps st;
-        auto issue = [&](int k0, int to) {
-            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(buf0 + to * Geo::BUF));
-            const int8_t *kb = uniform(kq + (int64_t)k0 * HD), *vb = uniform(vq + (int64_t)k0 * HD);
+        Piece p;
+        p.seq = pl.seq;
+        p.gran = few_granules(pl.seq.p0 + pl.seq.n);
+        p.h = pl.at / p.gran;
+        p.g0 = pl.at % p.gran;
+        p.g1 = min(p.gran, p.g0 + (x1 - x));
+        const int64_t row0 = pl.base / HD + p.h * (a.head_stride / HD);
+        p.kq = a.kv8.kq + row0 * HD;
+        p.vq = a.kv8.vq + row0 * HD;
+        p.ks = a.kv8.ks + row0 * NB;
+        p.vs = a.kv8.vs + row0 * NB;
+        return p;
+    };
+    Steps st;
+    // K and V rows of the wave's 32 keys of granule gr, into buffer `to`;
+    // rows past the last key repeat it (their weights are zero)
+    auto key0 = [&](int gr) { return gr * AQ_GRAN + w * AQ_KEYS; };
+    auto issue = [&](const Piece& p, int gr, int to) {
+        const int k0 = key0(gr), last = p.seq.p0 + p.seq.n - 1;
+        if (k0 > last) return;
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(buf0 + to * Geo::BUF));
+        const int8_t *kb = uniform(p.kq + (int64_t)k0 * HD), *vb = uniform(p.vq + (int64_t)k0 * HD);
 #pragma unroll
-            for (int i = 0; i < Geo::TILE / 1024; ++i) {
-                const int at = 64 * i + lane, key = at / Geo::CH, c = at % Geo::CH;
-                const uint32_t off = (uint32_t)min(key, keys - 1 - k0) * HD + 16 * (c ^ swz<HD>(key));
-                lds_copy16(kb, off, dst + 1024 * i);
-                lds_copy16(vb, off, dst + Geo::TILE + 1024 * i);
-            }
-            // lanes 0..31 carry the steps of a K row each, 32..63 of a V row
-            const int64_t r = min(k0 + (lane & 31), keys - 1);
-            st = *(const Steps*)((lane < 32 ? ks : vs) + r * NB);
-        };
-        auto key0 = [&](int gr) { return gr * AQ_GRAN + w * AQ_KEYS; };
-        int to = 0;
-        if (key0(g0) < keys) issue(key0(g0), 0);
+        for (int i = 0; i < Geo::TILE / 1024; ++i) {
+            const int at = 64 * i + lane, key = at / Geo::CH, c = at % Geo::CH;
+            const uint32_t off = (uint32_t)min(key, last - k0) * HD + 16 * (c ^ swz<HD>(key));
+            lds_copy16(kb, off, dst + 1024 * i);
+            lds_copy16(vb, off, dst + Geo::TILE + 1024 * i);
+        }
+        // lanes 0..31 carry the steps of a K row each, 32..63 of a V row
+        const int64_t r = min(k0 + (lane & 31), last);
+        st = *(const Steps*)((lane < 32 ? p.ks : p.vs) + r * NB);
+    };
+    // q of row j, elements 32t + 8g .. +7
+    float4u qraw[NB][2];
+    auto load_q = [&](const Piece& p) {
+        const bool live = j < p.seq.n * G;
+        const float* qp =
+            a.q + ((int64_t)(p.seq.t0 + (live ? j / G : 0)) * a.Hq + p.h * G + (live ? j % G : 0)) * HD + 8 * g;
+#pragma unroll
+        for (int t = 0; t < NB; ++t) {
+            qraw[t][0] = *(const float4u*)(qp + 32 * t);
+            qraw[t][1] = *(const float4u*)(qp + 32 * t + 4);
+        }
+    };
 
+    Piece pc = piece_at(x0);
+    int to = 0;
+    issue(pc, pc.g0, 0);
+    load_q(pc);
+    if (w == 0) {                                      // is the boundary x0 a block's first cut?
+        // (all lanes work it out: the plan's searches are the wave's)
+        const int start = x0 - pc.g0, end = start + pc.gran, before = (int)blockIdx.x - 1;
+        const int from = pc.g0 > 0 ? few_begin(plan, before) : 0;
+        int pieces = 0;
+        if (pc.g0 > 0 && from <= start) {
+            pieces = 2;
+            while (before + pieces < AQ_WGS && plan.begin(before + pieces, AQ_WGS) < end) ++pieces;
+        }
+        if (lane == 0)
+            *entry = JoinEntry{pc.seq.t0, pieces ? pc.seq.n * G : 0, 0, pc.h, pieces, 2 * before + (from != start)};
+    }
+
+    for (int x = x0;;) {
+        const SeqView sv = pc.seq;
+        const int keys = sv.p0 + sv.n, h = pc.h;
         // Q^T as the B operand: lane (g, j) holds row j, elements 32t + 8g .. +7,
         // scaled to [2^13, 2^14) at its largest so that lo keeps 11 bits of
         // any element within 2^-14 of it
         const int rows = sv.n * G;
-        const int tok = j / G, hq = h * G + j % G;
+        const int tok = j / G;
         const bool live = j < rows;
         float qv[NB][8];
         float top = 0.f;
-        const float* qp = a.q + ((int64_t)(sv.t0 + (live ? tok : 0)) * a.Hq + (live ? hq : 0)) * HD + 8 * g;
 #pragma unroll
-        for (int t = 0; t < NB; ++t) {
-            const float4u u0 = *(const float4u*)(qp + 32 * t), u1 = *(const float4u*)(qp + 32 * t + 4);
+        for (int t = 0; t < NB; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                qv[t][e] = live ? u0[e] * scale2 : 0.f;
-                qv[t][4 + e] = live ? u1[e] * scale2 : 0.f;
+            for (int e = 0; e < 8; ++e) {
+                qv[t][e] = live ? qraw[t][e >> 2][e & 3] * scale2 : 0.f;
+                top = fmaxf(top, fabsf(qv[t][e]));
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qv[t][e]));
-        }
         top = cols_max(top);
         const int qe = top > 0.f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
         const float unq = ldexpf(1.0f, -qe);
@@ -217,16 +280,15 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
         int lim = 0;                                   // f16 bits of the largest V step seen so far
         float pexp = 0.f;                              // the row's weights are 2^(score - m + pexp)
 
-        for (int gr = g0; gr < g1; ++gr) {
+        for (int gr = pc.g0; gr < pc.g1; ++gr) {
             const int k0 = key0(gr);
             if (k0 >= keys) break;                     // only in the last granule
             unsigned char* buf = buf0 + to * Geo::BUF;
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             const Steps mine = st;
             *(Steps*)(buf + 2 * Geo::TILE + lane * (int)sizeof(Steps)) = mine;
-            const int kn = key0(gr + 1);
-            if (gr + 1 < g1 && kn < keys) issue(kn, to ^ 1);
             to ^= 1;
+            if (gr + 1 < pc.g1) issue(pc, gr + 1, to);
 
             // scores of 32 keys: lane (g, j) has keys 16 hf + 4g + i of row j
             const _Float16* sk = (const _Float16*)(buf + 2 * Geo::TILE);
@@ -331,21 +393,28 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
             }
         }
 
-        // the four waves' results joined through LDS
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();                               // nobody still reads its rows
+        // the next piece's first loads go out, then the four waves' results
+        // are joined through LDS: each leaves them where its last keys were
+        const int xn = x + pc.g1 - pc.g0;
+        const bool more = xn < x1, whole = pc.g0 == 0 && pc.g1 == pc.gran;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) {
+            pc = piece_at(xn);
+            issue(pc, pc.g0, to);
+            load_q(pc);
+        }
         l = cols_sum(l);
         const float back = __builtin_amdgcn_exp2f(-pexp);
-        float* so = (float*)smem;
+        float* mine = (float*)(buf0 + (to ^ 1) * Geo::BUF);
         if (g == 0) {
             s_m[w][j] = m;
             s_l[w][j] = l * back;
+            s_at[w] = (int)((unsigned char*)mine - smem);
         }
 #pragma unroll
-        for (int n = 0; n < ND; ++n) *(floatx4*)(so + (w * AQ_ROWS + j) * OS + 16 * n + 4 * g) = o[n] * back;
+        for (int n = 0; n < ND; ++n) *(floatx4*)(mine + j * OS + 16 * n + 4 * g) = o[n] * back;
         __syncthreads();
-        const bool whole = g0 == 0 && g1 == gran;
-        float* slot = (float*)a.ws + (2 * (int64_t)blockIdx.x + (x == x0 ? 0 : 1)) * few_slot_floats(HD);
+        float* slot = few_slot(a.ws, 2 * blockIdx.x + (x == x0 ? 0 : 1), HD);
         for (int u = threadIdx.x; u < rows * (HD / 4); u += 256) {
             const int r = u / (HD / 4), c = 4 * (u % (HD / 4));
             const float mt = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
@@ -355,88 +424,83 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
             for (int k = 0; k < 4; ++k) {
                 const float f = s_m[k][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[k][r] - mt);
                 lt += f * s_l[k][r];
-                const floatx4 ok = *(const floatx4*)(so + (k * AQ_ROWS + r) * OS + c);
+                const floatx4 ok = *(const floatx4*)((const float*)(smem + s_at[k]) + r * OS + c);
                 sum += f == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : f * ok;
             }
             if (whole) {
-                const int64_t at = ((int64_t)(sv.t0 + r / G) * a.Hq + h * G + r % G) * HD + c;
                 const float inv = 1.0f / lt;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a.out[at + e] = sum[e] * inv;
+                *(float4u*)(a.out + ((int64_t)(sv.t0 + r / G) * a.Hq + h * G + r % G) * HD + c) = sum * inv;
             } else {
                 *(floatx4*)(slot + r * HD + c) = sum;
                 if (c == 0) *(float2*)(slot + AQ_ROWS * HD + 2 * r) = make_float2(mt, lt);
             }
         }
-        __syncthreads();                               // before the next piece's copies land
-        x += g1 - g0;
+        if (!more) break;
+        __syncthreads();                               // before these rows' places are copied over
+        x = xn;
     }
 }
 
-// Joins the partials of a block that lies in several workgroups' ranges.
-// Workgroup m - 1 looks at the boundary N m / P: where it is the first one
-// inside a block, the block's pieces are joined here, a wave per row.
+// Joins the partials of a block that lies in several workgroups' ranges, a
+// wave per row: workgroup b takes the block that is first cut before
+// workgroup b + 1.
 template <int HD>
-__global__ __launch_bounds__(256) void attn_q8_few_join_kernel(PackedAttn a, PackedBatch pb) {
-    constexpr int P = AQ_WGS;
+__global__ __launch_bounds__(256) void attn_q8_few_join_kernel(PackedAttn a) {
+    constexpr int EL = (HD + 63) / 64;                 // outputs per lane
+    const JoinEntry en = *(const JoinEntry*)((const char*)a.ws + 32 * (blockIdx.x + 1));
+    if (en.rows == 0) return;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int G = a.Hq / a.Hkv;
-    const Plan<FewCount> plan(pb, FewCount{G, a.Hkv});
-    const int64_t x = plan.begin(blockIdx.x + 1, P), before = plan.begin(blockIdx.x, P);
-    if (x >= plan.total) return;
-    const Place pl = plan.find(x);
-    const SeqView sv = seq_view(pb, pl.b);
-    const int gran = (sv.p0 + sv.n + AQ_GRAN - 1) / AQ_GRAN;
-    const int h = (int)(pl.at / gran), in = (int)(pl.at % gran);
-    const int64_t start = x - in, end = start + gran;
-    if (in == 0 || before > start) return;             // no block is cut here, or an earlier boundary cuts it
-    const int first = blockIdx.x;                      // the pieces: this workgroup's last, then whole first slots
-    int pieces = 1;
-    while (first + pieces < P && plan.begin(first + pieces, P) < end) ++pieces;
-    const float* ws = (const float*)a.ws;
-    auto slot = [&](int k) {
-        return ws + (2 * (int64_t)(first + k) + (k == 0 && before != start ? 1 : 0)) * few_slot_floats(HD);
-    };
-    auto some = [&](int k) { return plan.begin(first + k + 1, P) > plan.begin(first + k, P); };
-    for (int r = w; r < sv.n * G; r += 4) {
-        float mt = -INFINITY;
-        for (int k = lane; k < pieces; k += 64)
-            if (some(k)) mt = fmaxf(mt, slot(k)[AQ_ROWS * HD + 2 * r]);
-        mt = wave_max(mt);
-        float lt = 0.f, acc[2] = {0.f, 0.f};
-        for (int k0 = 0; k0 < pieces; k0 += 64) {
-            float f = 0.f;
-            if (k0 + lane < pieces && some(k0 + lane)) {
-                const float2 ml = *(const float2*)(slot(k0 + lane) + AQ_ROWS * HD + 2 * r);
-                f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mt);
-                lt += f * ml.y;
-            }
-            const int n = min(64, pieces - k0);
-            for (int k = 0; k < n; ++k) {
-                const float fk = lane_read(f, k);
-                if (fk == 0.f) continue;
-                const float* op = slot(k0 + k) + r * HD;
+    // the first part's slot, then the first slot of each workgroup after it
+    auto slot = [&](int k) { return few_slot(a.ws, k == 0 ? en.slot0 : 2 * ((int)blockIdx.x + k), HD); };
+    for (int r = w; r < en.rows; r += 4) {
+        float m = -INFINITY, l = 0.f, o[EL];
 #pragma unroll
-                for (int e = 0; e < (HD + 63) / 64; ++e)
-                    if (64 * e + lane < HD) acc[e] += fk * op[64 * e + lane];
+        for (int e = 0; e < EL; ++e) o[e] = 0.f;
+        for (int k0 = 0; k0 < en.pieces; k0 += 8) {
+            float2 ml[8];
+            float v[8][EL];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float* sl = slot(min(k0 + k, en.pieces - 1));
+                ml[k] = *(const float2*)(sl + AQ_ROWS * HD + 2 * r);
+#pragma unroll
+                for (int e = 0; e < EL; ++e) v[k][e] = sl[r * HD + min(64 * e + lane, HD - 1)];
+            }
+            float mt = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mt = fmaxf(mt, ml[k].x);
+            if (mt == -INFINITY) continue;             // nothing seen yet
+            const float f = __builtin_amdgcn_exp2f(m - mt);
+            m = mt;
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < EL; ++e) o[e] *= f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float fk = k0 + k < en.pieces ? __builtin_amdgcn_exp2f(ml[k].x - mt) : 0.f;
+                l += fk * ml[k].y;
+#pragma unroll
+                for (int e = 0; e < EL; ++e) o[e] += fk * v[k][e];
             }
         }
-        lt = wave_sum(lt);
-        const int64_t at = ((int64_t)(sv.t0 + r / G) * a.Hq + h * G + r % G) * HD;
+        const int64_t at = ((int64_t)(en.t0 + r / G) * a.Hq + en.h * G + r % G) * HD;
 #pragma unroll
-        for (int e = 0; e < (HD + 63) / 64; ++e)
-            if (64 * e + lane < HD) a.out[at + 64 * e + lane] = acc[e] / lt;
+        for (int e = 0; e < EL; ++e)
+            if (64 * e + lane < HD) a.out[at + 64 * e + lane] = o[e] / l;
     }
 }
 
 bool attention_q8_few_shape(int hd, int G) { return (hd == 32 || hd == 64 || hd == 128) && G <= AQ_ROWS; }
-int64_t attention_q8_few_bytes(int hd) { return 2 * AQ_WGS * few_slot_floats(hd) * (int64_t)sizeof(float); }
+int64_t attention_q8_few_bytes(int hd) {
+    return FEW_ENTRIES + 2 * AQ_WGS * few_slot_floats(hd) * (int64_t)sizeof(float);
+}
 
 template <int HD>
 static void launch_few(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
     hipLaunchKernelGGL(attn_q8_few_kernel<HD>, dim3(AQ_WGS), dim3(256), 0, s, a, pb);
-    if (pb.max_seq > AQ_GRAN)          // a block of one granule is never cut
-        hipLaunchKernelGGL(attn_q8_few_join_kernel<HD>, dim3(AQ_WGS - 1), dim3(256), 0, s, a, pb);
+    if (few_granules(pb.max_seq) > AQ_KEEP)            // else no block is cut
+        hipLaunchKernelGGL(attn_q8_few_join_kernel<HD>, dim3(AQ_WGS - 1), dim3(256), 0, s, a);
 }
 
 int launch_attention_q8_few(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
