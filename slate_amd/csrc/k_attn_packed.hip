@@ -93,14 +93,79 @@ __global__ __launch_bounds__(256) void attn_packed_rows_kernel(PackedAttn a, Pac
     }
 }
 
-int64_t attention_packed_bytes(int Hq, int Hkv, int hd) {
-    return attention_q8_few_shape(hd, Hq / Hkv) ? attention_q8_few_bytes(hd) : 0;
+// Joins the parts of a block that lies in several workgroups' ranges:
+// workgroup b takes the block that is first cut before workgroup b + 1 of the
+// attention kernel, HD / 4 lanes a row, eight parts' loads at a time.
+template <int HD, int TH>
+__global__ __launch_bounds__(TH) void attn_join_kernel(float* __restrict__ out, void* ws, int Hq, int G,
+                                                       int slot_rows) {
+    const JoinEntry en = *entry_of(ws, blockIdx.x + 1);
+    const int c = 4 * (threadIdx.x % (HD / 4));
+    // the first part's slot, then the first slot of each workgroup after it
+    auto slot = [&](int k) { return slot_of(ws, k == 0 ? en.slot0 : 2 * ((int)blockIdx.x + k), slot_rows, HD); };
+    for (int r = threadIdx.x / (HD / 4); r < en.rows; r += TH / (HD / 4)) {
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < en.pieces; k0 += 8) {
+            float2 ml[8];
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float* sl = slot(min(k0 + k, en.pieces - 1));
+                ml[k] = *(const float2*)(sl + slot_rows * HD + 2 * r);
+                v[k] = *(const float4*)(sl + r * HD + c);
+            }
+            float mt = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mt = fmaxf(mt, ml[k].x);
+            if (mt == -INFINITY) continue;             // nothing seen yet
+            const float f = __builtin_amdgcn_exp2f(m - mt);
+            m = mt;
+            l *= f;
+            o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float fk = k0 + k < en.pieces ? __builtin_amdgcn_exp2f(ml[k].x - mt) : 0.f;
+                if (fk == 0.f) continue;
+                l += fk * ml[k].y;
+                o.x += fk * v[k].x;
+                o.y += fk * v[k].y;
+                o.z += fk * v[k].z;
+                o.w += fk * v[k].w;
+            }
+        }
+        const float inv = 1.0f / l;
+        float* op = out + ((int64_t)(en.t0 + (en.r0 + r) / G) * Hq + en.h * G + (en.r0 + r) % G) * HD + c;
+        op[0] = o.x * inv;
+        op[1] = o.y * inv;
+        op[2] = o.z * inv;
+        op[3] = o.w * inv;
+    }
 }
 
+template <int HD>
+static void launch_join_hd(float* out, void* ws, int Hq, int Hkv, int slot_rows, hipStream_t s) {
+    if (slot_rows <= 32)
+        hipLaunchKernelGGL((attn_join_kernel<HD, 256>), dim3(AP_WGS - 1), dim3(256), 0, s, out, ws, Hq, Hq / Hkv,
+                           slot_rows);
+    else
+        hipLaunchKernelGGL((attn_join_kernel<HD, 1024>), dim3(AP_WGS - 1), dim3(1024), 0, s, out, ws, Hq, Hq / Hkv,
+                           slot_rows);
+}
+
+void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, hipStream_t s) {
+    if (hd == 128)
+        launch_join_hd<128>(out, ws, Hq, Hkv, slot_rows, s);
+    else if (hd == 64)
+        launch_join_hd<64>(out, ws, Hq, Hkv, slot_rows, s);
+    else
+        launch_join_hd<32>(out, ws, Hq, Hkv, slot_rows, s);
+}
+
+int64_t attention_packed_bytes(int Hq, int Hkv, int hd) { return attention_q8_shape(hd) ? attention_q8_bytes(hd) : 0; }
+
 int launch_attention_packed(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
-    const int G = a.Hq / a.Hkv;
-    if (!a.kf && attention_q8_few_shape(a.hd, G) && pb.max_new * (int64_t)G <= 16)
-        return launch_attention_q8_few(a, pb, s);
+    if (!a.kf && attention_q8_shape(a.hd)) return launch_attention_q8(a, pb, s);
     hipLaunchKernelGGL(attn_packed_rows_kernel, dim3(pb.T, a.Hq), dim3(256), 0, s, a, pb);
     SH_CHECK_LAUNCH();
     return 0;
