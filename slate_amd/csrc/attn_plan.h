@@ -103,8 +103,6 @@ class Plan {
     Lane first_;
 };
 
-constexpr int AP_WGS = 512;            // workgroups of a packed attention kernel: two per CU
-
 // What the join kernel does about the boundary before a workgroup, left in
 // the workspace by that workgroup: the block that is first cut there.
 struct JoinEntry {
@@ -113,32 +111,31 @@ struct JoinEntry {
     int pieces;                        // this many neighbours hold a part each, from the workgroup before on
     int slot0;                         // the slot of the first part
 };
-constexpr int64_t JOIN_BYTES = (int64_t)AP_WGS * 32;
 
-// Workspace: a JoinEntry per workgroup, then two slots each of `rows` rows of
+// Workspace of P workgroups: a JoinEntry each, then two slots each of `rows` rows of
 // hd outputs and a pair (m, l) per row.  Outputs and l are relative to 2^m.
 __host__ __device__ constexpr int64_t slot_floats(int rows, int hd) { return (int64_t)rows * (hd + 2); }
-__device__ __forceinline__ float* slot_of(void* ws, int i, int rows, int hd) {
-    return (float*)((char*)ws + JOIN_BYTES) + i * slot_floats(rows, hd);
+__device__ __forceinline__ float* slot_of(void* ws, int P, int i, int rows, int hd) {
+    return (float*)((char*)ws + 32 * P) + i * slot_floats(rows, hd);
 }
 __device__ __forceinline__ JoinEntry* entry_of(void* ws, int w) { return (JoinEntry*)((char*)ws + 32 * w); }
-inline int64_t plan_bytes(int rows, int hd) {
-    return JOIN_BYTES + 2 * AP_WGS * slot_floats(rows, hd) * (int64_t)sizeof(float);
+inline int64_t plan_bytes(int P, int rows, int hd) {
+    return 32 * P + 2 * P * slot_floats(rows, hd) * (int64_t)sizeof(float);
 }
-// slot_rows: rows of a slot; cut into pieces for the shapes hd 32, 64, 128.
-void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, hipStream_t s);
+// hd 32, 64 or 128.
+void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, int P, hipStream_t s);
 
 // The entry of workgroup w, whose range begins at x0 in granule `in` of a
 // block of `gran`; begin(w) are the ranges' beginnings.  Called by a whole
 // wave (the searches are the wave's).
 template <class Begin>
-__device__ __forceinline__ void leave_entry(void* ws, int w, int x0, int in, int gran, const Begin& begin, JoinEntry e) {
+__device__ __forceinline__ void leave_entry(void* ws, int P, int w, int x0, int in, int gran, const Begin& begin, JoinEntry e) {
     const int start = x0 - in, end = start + gran;
     const int from = in > 0 ? begin(w - 1) : 0;
     e.pieces = 0;
     if (in > 0 && from <= start) {
         e.pieces = 2;
-        while (w - 1 + e.pieces < AP_WGS && begin(w - 1 + e.pieces) < end) ++e.pieces;
+        while (w - 1 + e.pieces < P && begin(w - 1 + e.pieces) < end) ++e.pieces;
     }
     if (e.pieces == 0) e.rows = 0;
     e.slot0 = 2 * (w - 1) + (from != start);

@@ -1,0 +1,524 @@
+// k_attn_many.hip -- attention of packed batches with more than a few query
+// rows per (sequence, kv head), over the 8-bit cache or f32 pools: prompt
+// chunks, mixed steps, drafted trees.  The arithmetic: attn_rows.h, how the
+// keys are shared out: attn_plan.h.
+//
+// A workgroup of eight waves takes a block of 128 query rows, 16 a wave, over
+// a range of keys.  A stage of keys is brought into LDS as f16 once for all
+// waves, while the stage before is worked on and the one after is on its way
+// in registers; one barrier a stage.
+//   8-bit: the codes (exact in f16); a key's scores and weights go by its
+//       steps, block by block of 32 elements.  Two MFMAs a product.
+//   f32: a row of K or V is scaled by a power of two to [2^13, 2^14) at its
+//       largest element and split into halves hi + lo of 22 bits; three MFMAs
+//       a product (lo * lo is below what f32 sums keep).
+// Rows stay as they are stored, [key][element]: V^T comes out of LDS by the
+// transposing read.  16-byte chunks of a row are permuted, chunk c of key k
+// at place c ^ turn(k), so that both kinds of reads spread over the banks.
+#include "attn_plan.h"
+#include "attn_q8.h"
+
+namespace slate_hip {
+
+constexpr int AM_WGS = 256;            // one workgroup per CU
+constexpr int AM_TH = 512;
+constexpr int AM_ROWS = 8 * AR_TILE;   // query rows of a block
+constexpr int AM_KEEP = 512;           // blocks of up to this many keys are not cut
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+// Transposing LDS read of 16-bit numbers: the 16 lanes of a group name four
+// rows of 32 bytes, lane i quarter i % 4 of row i / 4; lane i gets number i of
+// each row.
+__device__ __forceinline__ half4_t read_columns16(const _Float16* p) {
+    return __builtin_bit_cast(half4_t,
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p)));
+}
+
+template <int HD>
+__device__ __forceinline__ int turn(int key) {
+    if (HD == 128) return ((key << 1) | (key >> 3 & 1)) & 15;
+    if (HD == 64) return ((key & 6) | (key >> 3 & 1)) & 7;
+    return key >> 2 & 3;
+}
+
+// Where element 8c of key k sits in a stage's plane (in halves).
+template <int HD>
+__device__ __forceinline__ int place(int key, int c) {
+    return key * HD + 8 * (c ^ turn<HD>(key));
+}
+
+template <int HD, bool F32>
+struct ManyGeom {
+    static constexpr int KEYS = F32 ? 32 : 64;         // keys of a stage
+    static constexpr int PLANE = KEYS * HD;            // halves
+    static constexpr int PLANES = F32 ? 4 : 2;         // K hi (lo), V hi (lo)
+    static constexpr int CH = HD / 8;                  // 8-element chunks of a row
+    // what a thread brings in: 16 codes of a row, or 8 f32
+    static constexpr int UNIT = F32 ? 8 : 16;
+    static constexpr int UNITS = KEYS * HD / UNIT;     // of K, and of V
+};
+
+// Blocks of a sequence and their granules (stages).
+struct ManyCount {
+    int G, Hkv, keys;                  // keys of a stage
+    bool causal;
+    __device__ __forceinline__ int blocks(const SeqView& s) const { return (s.n * G + AM_ROWS - 1) / AM_ROWS; }
+    // keys that block i's rows see
+    __device__ __forceinline__ int seen(const SeqView& s, int i) const {
+        return s.p0 + (causal ? (min(s.n * G, (i + 1) * AM_ROWS) - 1) / G + 1 : s.n);
+    }
+    __device__ __forceinline__ int granules(const SeqView& s, int i) const { return (seen(s, i) + keys - 1) / keys; }
+    __device__ __forceinline__ int per_head(const SeqView& s) const {
+        const int nb = blocks(s);
+        if (!causal || nb <= 1) return nb * granules(s, 0);
+        int sum = 0;
+        for (int i = 0; i < nb; ++i) sum += granules(s, i);
+        return sum;
+    }
+    __device__ __forceinline__ int operator()(const SeqView& s) const { return s.n < 1 ? 0 : Hkv * per_head(s); }
+};
+using ManyPlan = Plan<ManyCount>;
+
+struct ManyPlace {
+    SeqView seq;
+    int64_t base;
+    int h, block, gran, in;            // kv head, block, its granules, granule of it
+};
+__device__ __forceinline__ ManyPlace many_find(const ManyPlan& plan, const ManyCount& c, int x) {
+    const Place pl = plan.find(x);
+    ManyPlace r{pl.seq, pl.base, 0, 0, 0, 0};
+    const int nb = c.blocks(pl.seq);
+    if (!c.causal || nb <= 1) {
+        r.gran = c.granules(pl.seq, 0);
+        const int b = pl.at / r.gran;
+        r.h = b / nb;
+        r.block = b % nb;
+        r.in = pl.at % r.gran;
+        return r;
+    }
+    const int per = c.per_head(pl.seq);
+    r.h = pl.at / per;
+    r.in = pl.at % per;
+    for (int i0 = 0;; i0 += 64) {                      // 64 blocks at a time
+        const int i = i0 + (int)(threadIdx.x & 63);
+        const int own = i < nb ? c.granules(pl.seq, i) : 0, upto = wave_scan(own);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > r.in);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            r.block = i0 + l;
+            r.gran = __builtin_amdgcn_readlane(own, l);
+            r.in -= __builtin_amdgcn_readlane(upto - own, l);
+            return r;
+        }
+        r.in -= __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+__device__ __forceinline__ int many_begin(const ManyPlan& plan, const ManyCount& c, int w) {
+    const int x = plan.begin(w, AM_WGS);
+    if (x >= plan.total) return plan.total;
+    const ManyPlace p = many_find(plan, c, x);
+    return p.gran * c.keys <= AM_KEEP ? x - p.in : x;
+}
+
+// 32 keys of a stage against the wave's rows.
+template <int HD, bool F32>
+struct ManyRows : AttnRows<HD> {
+    using AttnRows<HD>::qh;
+    using AttnRows<HD>::ql;
+    using AttnRows<HD>::o;
+    static constexpr int NB = HD / 32, ND = HD / 16, CH = HD / 8;
+    using Steps = Q8Steps<HD>;
+
+    // planes: K hi (lo), V hi (lo); ks, vs: the keys' steps (Steps, or the
+    // power of two of a row as a float).  MASKED as in Q8Rows.  bad: keys
+    // whose V row has an element that is not finite (it is 0 in the plane),
+    // vrow the first key's row (f32).
+    template <bool MASKED>
+    __device__ __forceinline__ void keys32(const _Float16* planes, int at, const void* ks_, const void* vs_,
+                                           uint32_t seen, uint32_t bad, const float* vrow) {
+        using Geo = ManyGeom<HD, F32>;
+        const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+        const _Float16 *k = planes + at * HD, *v = k + (F32 ? 2 : 1) * Geo::PLANE;
+        const Steps *ks = (const Steps*)ks_, *vs = (const Steps*)vs_;
+        const float *kf = (const float*)ks_, *vf = (const float*)vs_;
+        floatx4 s[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            const int key = 16 * hf + j;
+            s[hf] = floatx4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < NB; ++t) {
+                    const half8_t kh = *(const half8_t*)(k + place<HD>(key, 4 * t + g));
+                    const half8_t kl = *(const half8_t*)(k + Geo::PLANE + place<HD>(key, 4 * t + g));
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[t], s[hf], 0, 0, 0);
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[t], s[hf], 0, 0, 0);
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[t], s[hf], 0, 0, 0);
+                }
+                s[hf] *= *(const floatx4*)(kf + 16 * hf + 4 * g);
+            } else {
+                Steps d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = ks[16 * hf + 4 * g + i];
+#pragma unroll
+                for (int t = 0; t < NB; ++t) {
+                    const half8_t kc = *(const half8_t*)(k + place<HD>(key, 4 * t + g));
+                    floatx4 r = {0.f, 0.f, 0.f, 0.f};
+                    r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[t], r, 0, 0, 0);
+                    r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qh[t], r, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[hf][e] = fmaf((float)d[e].s[t], r[e], s[hf][e]);
+                }
+            }
+        }
+        // bit 16 (e / 4) + e % 4 of `bits`: the row sees the lane's key e
+        const uint32_t bits = MASKED ? seen >> (4 * g) : 0;
+        auto sees = [&](int e) { return (bits >> (16 * (e >> 2) + (e & 3)) & 1) != 0; };
+        float p[8], x[8];
+        // lane i of a group names quarter i % 4 of the 16 columns of the
+        // i / 4-th of its four keys (slots 8g .. +3 hold keys 4g + i, slots
+        // 8g + 4 .. +7 keys 16 + 4g + i)
+        const int tkey = 4 * g + (j >> 2), tc = (j & 3) >> 1, te = 4 * (j & 1);
+        auto columns = [&](const _Float16* plane, int n) {
+            const half4_t a = read_columns16(plane + place<HD>(tkey, 2 * n + tc) + te);
+            const half4_t b = read_columns16(plane + place<HD>(tkey + 16, 2 * n + tc) + te);
+            return half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        };
+        half8_t ph, pl;
+        if constexpr (F32) {
+            const floatx4 d[2] = {*(const floatx4*)(vf + 4 * g), *(const floatx4*)(vf + 16 + 4 * g)};
+            int big = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool see = !MASKED || sees(e);
+                if (MASKED && !see) s[e >> 2][e & 3] = -INFINITY;
+                if (see) big = max(big, __builtin_bit_cast(int, d[e >> 2][e & 3]));
+            }
+            this->template weights<true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = p[e] * (MASKED && !sees(e) ? 0.f : d[e >> 2][e & 3]);
+            halves(x, ph, pl);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                const half8_t vh = columns(v, n), vl = columns(v + Geo::PLANE, n);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[n], 0, 0, 0);
+            }
+            if (MASKED)
+                for (uint32_t left = bad; left; left &= left - 1) {   // for the rows that do see such a row
+                    const int key = __builtin_ctz(left);
+                    if (!(seen >> key & 1)) continue;
+#pragma unroll
+                    for (int n = 0; n < ND; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float val = vrow[(int64_t)key * HD + 16 * n + 4 * g + e];
+                            if (!(fabsf(val) < INFINITY)) o[n][e] += val;
+                        }
+                }
+        } else {
+            Steps dv[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dv[e] = vs[16 * (e >> 2) + 4 * g + (e & 3)];
+            int big = 0;
+            if (MASKED) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!sees(e)) {
+                        s[e >> 2][e & 3] = -INFINITY;
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < NB; ++t) big = max(big, step_bits(dv[e].s[t]));
+                    }
+            } else {                                   // a lane looks at one key's V steps
+                const Steps one = vs[lane & 31];
+#pragma unroll
+                for (int t = 0; t < NB; ++t) big = max(big, step_bits(one.s[t]));
+            }
+            this->template weights<MASKED>(s, big, step_exponent, p);
+#pragma unroll
+            for (int t = 0; t < NB; ++t) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float d = (float)dv[e].s[t];
+                    if (MASKED) d = sees(e) ? d : 0.f;   // a step that the row does not see may be anything
+                    x[e] = p[e] * d;
+                }
+                halves(x, ph, pl);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int n = 2 * t + u;
+                    const half8_t vc = columns(v, n);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pl, o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, ph, o[n], 0, 0, 0);
+                }
+            }
+        }
+    }
+};
+
+// The largest of the lanes that share a row (16, 8 or 4 of them).
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
+    if (N == 16) return row16_max(v);
+    if (N == 8) return group8_max(v);
+    v = fmaxf(v, dpp_mov<DPP_QUAD_XOR1>(v));
+    return fmaxf(v, dpp_mov<DPP_QUAD_XOR2>(v));
+}
+
+template <int HD, bool F32>
+__global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
+    using Geo = ManyGeom<HD, F32>;
+    using Steps = Q8Steps<HD>;
+    constexpr int NB = HD / 32, ND = HD / 16, KEYS = Geo::KEYS, PLANE = Geo::PLANE;
+    constexpr int STEP = F32 ? 4 : (int)sizeof(Steps);
+    __shared__ __attribute__((aligned(16))) _Float16 s_rows[2][Geo::PLANES * PLANE];
+    __shared__ __attribute__((aligned(16))) unsigned char s_step[2][2 * KEYS * STEP];
+    __shared__ uint32_t s_seen[PK_MAX_DRAFT / 32][AM_ROWS];   // the drafts that a block's token sees
+    __shared__ int16_t s_par[PK_MAX_DRAFT];
+    __shared__ uint32_t s_bad[4];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, j = lane & 15;
+    const int G = a.Hq / a.Hkv;
+    // neighbouring ranges on one XCD: blocks that share keys find them in its L2
+    const int wg = (blockIdx.x % 8) * (AM_WGS / 8) + blockIdx.x / 8;
+    const ManyCount count{G, a.Hkv, KEYS, a.parent == nullptr};
+    const ManyPlan plan(pb, count);
+    auto begin = [&](int v) { return many_begin(plan, count, v); };
+    const int x0 = begin(wg), x1 = begin(wg + 1);
+    if (x0 >= x1) {
+        if (tid == 0) entry_of(a.ws, wg)->rows = 0;
+        return;
+    }
+    const float scale2 = (1.0f / sqrtf((float)HD)) * LOG2E;
+    if (tid < 4) s_bad[tid] = 0;
+
+    struct Piece {
+        SeqView seq;
+        int h, block, gran, g0, g1, last;
+        int64_t at;                    // first element of the head's rows
+    };
+    auto piece_at = [&](int x) {
+        const ManyPlace pl = many_find(plan, count, x);
+        const int64_t base = F32 ? pl.base : pl.base / HD * HD;
+        return Piece{pl.seq, pl.h, pl.block, pl.gran, pl.in, min(pl.gran, pl.in + (x1 - x)),
+                     count.seen(pl.seq, pl.block) - 1, base + pl.h * a.head_stride};
+    };
+    // a stage's rows on their way: the thread's unit of K and of V, and steps
+    // (rows past the last key repeat it: nobody sees them)
+    typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+    uint4v raw_k, raw_v;
+    float4u f_k[2], f_v[2];
+    Steps st;
+    const int unit = tid * Geo::UNIT / HD, elem = tid * Geo::UNIT % HD;   // key and element of the thread's unit
+    const bool mine = tid < Geo::UNITS;
+    auto load = [&](const Piece& p, int gr) {
+        const int k0 = gr * KEYS;
+        const int64_t row = min(k0 + unit, p.last);
+        if (mine) {
+            const int64_t e = p.at + row * HD + elem;
+            if constexpr (F32) {
+                f_k[0] = *(const float4u*)(a.kf + e);
+                f_k[1] = *(const float4u*)(a.kf + e + 4);
+                f_v[0] = *(const float4u*)(a.vf + e);
+                f_v[1] = *(const float4u*)(a.vf + e + 4);
+            } else {
+                raw_k = *(const uint4v*)(a.kv8.kq + e);
+                raw_v = *(const uint4v*)(a.kv8.vq + e);
+            }
+        }
+        if (!F32 && tid < 2 * KEYS) {
+            const int64_t r = p.at / KV8_BLOCK + (int64_t)min(k0 + tid % KEYS, p.last) * NB;
+            st = *(const Steps*)((tid < KEYS ? a.kv8.ks : a.kv8.vs) + r);
+        }
+    };
+    // and into LDS; `masked`: some row may not see some key of it
+    auto put = [&](int to, int ring, bool masked) {
+        _Float16* rows = s_rows[to];
+        if constexpr (F32) {
+            if (mine) {
+                float* steps = (float*)s_step[to];
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    float x[8], top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = kv == 0 ? f_k[e >> 2][e & 3] : f_v[e >> 2][e & 3];
+                        if (kv == 1 && masked && !(fabsf(x[e]) < INFINITY)) {
+                            x[e] = 0.f;
+                            atomicOr(&s_bad[ring], 1u << unit);
+                        }
+                        top = fmaxf(top, fabsf(x[e]));
+                    }
+                    top = lanes_max<HD / 8>(top);
+                    const int e2 = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], e2);
+                    half8_t hi, lo;
+                    halves(x, hi, lo);
+                    _Float16* at = rows + 2 * kv * PLANE + place<HD>(unit, elem / 8);
+                    *(half8_t*)at = hi;
+                    *(half8_t*)(at + PLANE) = lo;
+                    if (elem == 0) steps[kv * KEYS + unit] = ldexpf(1.0f, -e2);
+                }
+            }
+        } else {
+            if (mine) {
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const uint4v r = kv == 0 ? raw_k : raw_v;
+                    _Float16* at = rows + kv * PLANE;
+                    *(half8_t*)(at + place<HD>(unit, elem / 8)) = codes_f16(uint2v{r[0], r[1]});
+                    *(half8_t*)(at + place<HD>(unit, elem / 8 + 1)) = codes_f16(uint2v{r[2], r[3]});
+                }
+            }
+            if (tid < 2 * KEYS) ((Steps*)s_step[to])[tid] = st;
+        }
+    };
+    // keys below it are seen by all rows of the piece's block
+    auto open_to = [&](const Piece& p) {
+        return a.parent ? p.seq.p0 : p.seq.p0 + p.block * AM_ROWS / G + 1;
+    };
+    auto put_piece = [&](const Piece& p, int gr, int to, int ring) { put(to, ring, (gr + 1) * KEYS > open_to(p)); };
+
+    Piece pc = piece_at(x0), nx = pc;                  // worked on; being loaded
+    int ngr = pc.g0, nx_x = x0;                        // the stage being loaded, its piece's place on the line
+    load(nx, ngr);
+    if (w == 0)
+        leave_entry(a.ws, AM_WGS, wg, x0, pc.g0, pc.gran, begin,
+                    JoinEntry{pc.seq.t0, min(AM_ROWS, pc.seq.n * G - pc.block * AM_ROWS), pc.block * AM_ROWS, pc.h, 0,
+                              0});
+    // the next stage after the one being loaded; false at the range's end
+    auto advance = [&]() {
+        if (ngr + 1 < nx.g1) {
+            ++ngr;
+            return true;
+        }
+        const int xn = nx_x + nx.g1 - nx.g0;
+        if (xn >= x1) return false;
+        nx_x = xn;
+        nx = piece_at(xn);
+        ngr = nx.g0;
+        return true;
+    };
+    __syncthreads();                                   // s_bad is clear
+    put_piece(nx, ngr, 0, 0);
+    bool coming = advance();
+    if (coming) load(nx, ngr);
+    int to = 0, ring = 0;
+
+    for (int x = x0;;) {
+        const SeqView sv = pc.seq;
+        const int h = pc.h, r0 = pc.block * AM_ROWS, rows = min(AM_ROWS, sv.n * G - r0);
+        const int rw = AR_TILE * w, tok0 = r0 / G;     // the wave's first row in the block, the block's first token
+        const int row = r0 + rw + j;
+        const bool live = rw + j < rows;
+        const int tok = row / G;
+        ManyRows<HD, F32> R;
+        R.start(a.q + ((int64_t)(sv.t0 + (live ? tok : 0)) * a.Hq + h * G + (live ? row % G : 0)) * HD, live, scale2);
+        // keys below `open` are seen by all of the wave's rows, from `end` on by none
+        const int open = a.parent ? sv.p0 : sv.p0 + (r0 + min(rw, rows - 1)) / G + 1;
+        const int end = rw >= rows ? 0 : a.parent ? sv.p0 + sv.n : sv.p0 + (r0 + min(rw + AR_TILE, rows) - 1) / G + 1;
+        const int words = (sv.n + 31) / 32;
+        if (a.parent && pc.g1 * KEYS > sv.p0) {        // the block's tokens' ancestors
+            __syncthreads();
+            for (int i = tid; i < sv.n; i += AM_TH) {
+                const int up = a.parent[sv.t0 + i];
+                s_par[i] = (int16_t)(up >= 0 && up < i ? up : -1);
+            }
+            __syncthreads();
+            if (tid < (r0 + rows - 1) / G - tok0 + 1) {
+                int cur = tok0 + tid;
+                for (int wd = words - 1; wd >= 0; --wd) {
+                    uint32_t bits = 0;
+                    while (cur >= 32 * wd) {
+                        bits |= 1u << (cur & 31);
+                        cur = s_par[cur];
+                    }
+                    s_seen[wd][tid] = bits;
+                }
+            }
+        }
+        for (int gr = pc.g0; gr < pc.g1; ++gr) {
+            __syncthreads();                           // the stage is in LDS; the other buffer is read through
+            const int now = to, now_ring = ring;
+            to ^= 1;
+            ring = (ring + 1) & 3;
+            if (tid == 0) s_bad[(ring + 1) & 3] = 0;   // last read two stages ago, next set after the next barrier
+            if (coming) {
+                put_piece(nx, ngr, to, ring);
+                if ((coming = advance())) load(nx, ngr);
+            }
+#pragma unroll 1
+            for (int at = 0; at < KEYS; at += AR_KEYS) {
+                const int k0 = gr * KEYS + at;
+                if (k0 >= end) break;
+                const unsigned char *ks = s_step[now] + at * STEP, *vs = ks + KEYS * STEP;
+                if (k0 + AR_KEYS <= open) {
+                    R.template keys32<false>(s_rows[now], at, ks, vs, 0, 0, nullptr);
+                    continue;
+                }
+                uint32_t seen = 0;
+                if (live && !a.parent) {
+                    const int n = min(32, max(0, sv.p0 + tok + 1 - k0));
+                    seen = n == 32 ? 0xffffffffu : (1u << n) - 1;
+                } else if (live) {
+                    const int d = k0 - sv.p0, wd = d >> 5;
+                    const uint32_t lo = wd < 0 ? 0xffffffffu : wd < words ? s_seen[wd][tok - tok0] : 0;
+                    const uint32_t hi = wd + 1 < 0 ? 0xffffffffu : wd + 1 < words ? s_seen[wd + 1][tok - tok0] : 0;
+                    seen = (uint32_t)(((uint64_t)hi << 32 | lo) >> (d & 31));
+                }
+                R.template keys32<true>(s_rows[now], at, ks, vs, seen, F32 ? s_bad[now_ring] : 0,
+                                        F32 ? a.vf + pc.at + (int64_t)k0 * HD : nullptr);
+            }
+        }
+        const bool whole = pc.g0 == 0 && pc.g1 == pc.gran;
+        const float back = R.back(), l = R.sum();
+        if (live) {
+            if (whole) {
+                float* op = a.out + ((int64_t)(sv.t0 + tok) * a.Hq + h * G + row % G) * HD + 4 * g;
+                const float inv = back / l;
+#pragma unroll
+                for (int n = 0; n < ND; ++n) *(float4u*)(op + 16 * n) = R.o[n] * inv;
+            } else {
+                float* slot = slot_of(a.ws, AM_WGS, 2 * wg + (x == x0 ? 0 : 1), AM_ROWS, HD);
+                const int r = rw + j;
+                if (g == 0) *(float2*)(slot + AM_ROWS * HD + 2 * r) = make_float2(R.m, l);
+#pragma unroll
+                for (int n = 0; n < ND; ++n) *(floatx4*)(slot + r * HD + 16 * n + 4 * g) = R.o[n] * back;
+            }
+        }
+        x += pc.g1 - pc.g0;
+        if (x >= x1) break;
+        pc = piece_at(x);
+    }
+}
+
+int64_t attention_many_bytes(int hd) { return plan_bytes(AM_WGS, AM_ROWS, hd); }
+bool attention_many_takes(const PackedAttn& a) { return a.hd == 32 || a.hd == 64 || a.hd == 128; }
+
+template <int HD>
+static void launch_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
+    if (a.kf)
+        hipLaunchKernelGGL((attn_many_kernel<HD, true>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
+    else
+        hipLaunchKernelGGL((attn_many_kernel<HD, false>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
+    if (pb.max_seq > AM_KEEP)                          // else no block is cut
+        launch_attn_join(a.out, a.ws, a.Hq, a.Hkv, HD, AM_ROWS, AM_WGS, s);
+}
+
+int launch_attention_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
+    if (a.hd == 128)
+        launch_many<128>(a, pb, s);
+    else if (a.hd == 64)
+        launch_many<64>(a, pb, s);
+    else
+        launch_many<32>(a, pb, s);
+    SH_CHECK_LAUNCH();
+    return 0;
+}
+
+}  // namespace slate_hip

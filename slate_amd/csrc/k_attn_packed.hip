@@ -98,11 +98,11 @@ __global__ __launch_bounds__(256) void attn_packed_rows_kernel(PackedAttn a, Pac
 // attention kernel, HD / 4 lanes a row, eight parts' loads at a time.
 template <int HD, int TH>
 __global__ __launch_bounds__(TH) void attn_join_kernel(float* __restrict__ out, void* ws, int Hq, int G,
-                                                       int slot_rows) {
+                                                       int slot_rows, int P) {
     const JoinEntry en = *entry_of(ws, blockIdx.x + 1);
     const int c = 4 * (threadIdx.x % (HD / 4));
     // the first part's slot, then the first slot of each workgroup after it
-    auto slot = [&](int k) { return slot_of(ws, k == 0 ? en.slot0 : 2 * ((int)blockIdx.x + k), slot_rows, HD); };
+    auto slot = [&](int k) { return slot_of(ws, P, k == 0 ? en.slot0 : 2 * ((int)blockIdx.x + k), slot_rows, HD); };
     for (int r = threadIdx.x / (HD / 4); r < en.rows; r += TH / (HD / 4)) {
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -144,28 +144,32 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(float* __restrict__ out, 
 }
 
 template <int HD>
-static void launch_join_hd(float* out, void* ws, int Hq, int Hkv, int slot_rows, hipStream_t s) {
-    if (slot_rows <= 32)
-        hipLaunchKernelGGL((attn_join_kernel<HD, 256>), dim3(AP_WGS - 1), dim3(256), 0, s, out, ws, Hq, Hq / Hkv,
-                           slot_rows);
+static void launch_join_hd(float* out, void* ws, int Hq, int Hkv, int slot_rows, int P, hipStream_t s) {
+    if (slot_rows <= 16)
+        hipLaunchKernelGGL((attn_join_kernel<HD, 256>), dim3(P - 1), dim3(256), 0, s, out, ws, Hq, Hq / Hkv, slot_rows,
+                           P);
     else
-        hipLaunchKernelGGL((attn_join_kernel<HD, 1024>), dim3(AP_WGS - 1), dim3(1024), 0, s, out, ws, Hq, Hq / Hkv,
-                           slot_rows);
+        hipLaunchKernelGGL((attn_join_kernel<HD, 1024>), dim3(P - 1), dim3(1024), 0, s, out, ws, Hq, Hq / Hkv,
+                           slot_rows, P);
 }
 
-void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, hipStream_t s) {
+void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, int P, hipStream_t s) {
     if (hd == 128)
-        launch_join_hd<128>(out, ws, Hq, Hkv, slot_rows, s);
+        launch_join_hd<128>(out, ws, Hq, Hkv, slot_rows, P, s);
     else if (hd == 64)
-        launch_join_hd<64>(out, ws, Hq, Hkv, slot_rows, s);
+        launch_join_hd<64>(out, ws, Hq, Hkv, slot_rows, P, s);
     else
-        launch_join_hd<32>(out, ws, Hq, Hkv, slot_rows, s);
+        launch_join_hd<32>(out, ws, Hq, Hkv, slot_rows, P, s);
 }
 
-int64_t attention_packed_bytes(int Hq, int Hkv, int hd) { return attention_q8_shape(hd) ? attention_q8_bytes(hd) : 0; }
+int64_t attention_packed_bytes(int Hq, int Hkv, int hd) {
+    if (hd != 32 && hd != 64 && hd != 128) return 0;
+    return max(attention_q8_few_bytes(hd), attention_many_bytes(hd));
+}
 
 int launch_attention_packed(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
-    if (!a.kf && attention_q8_shape(a.hd)) return launch_attention_q8(a, pb, s);
+    if (attention_q8_few_takes(a, pb)) return launch_attention_q8_few(a, pb, s);
+    if (attention_many_takes(a)) return launch_attention_many(a, pb, s);
     hipLaunchKernelGGL(attn_packed_rows_kernel, dim3(pb.T, a.Hq), dim3(256), 0, s, a, pb);
     SH_CHECK_LAUNCH();
     return 0;

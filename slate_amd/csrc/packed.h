@@ -72,10 +72,14 @@ struct PackedAttn {
     void* ws;
 };
 int64_t attention_packed_bytes(int Hq, int Hkv, int hd);
-// k_attn_q8.hip: 8-bit pools of head_dim 32, 64, 128.
-bool attention_q8_shape(int hd);
-int64_t attention_q8_bytes(int hd);
-int launch_attention_q8(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
+// k_attn_q8.hip: 8-bit pools, at most 16 query rows per (sequence, kv head).
+bool attention_q8_few_takes(const PackedAttn& a, const PackedBatch& pb);
+int64_t attention_q8_few_bytes(int hd);
+int launch_attention_q8_few(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
+// k_attn_many.hip: head_dim 32, 64, 128, either kind of pools, any rows.
+bool attention_many_takes(const PackedAttn& a);
+int64_t attention_many_bytes(int hd);
+int launch_attention_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
 int launch_attention_packed(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
 
 }  // namespace slate_hip
