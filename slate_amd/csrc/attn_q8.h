@@ -80,6 +80,7 @@ struct Q8Rows : AttnRows<HD> {
         const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
         // scores: lane (g, j) has keys 16 hf + 4g + i of row j
         floatx4 s[2];
+        const floatx4 zero = zeros();
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             Q8Steps<HD> d[4];
@@ -92,8 +93,7 @@ struct Q8Rows : AttnRows<HD> {
                 const int c = 2 * t + (g >> 1);
                 const half8_t kc =
                     codes_f16(*(const uint2v*)(k + key * HD + 16 * (c ^ swz<HD>(key)) + 8 * (g & 1)));
-                floatx4 r = {0.f, 0.f, 0.f, 0.f};
-                r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[t], r, 0, 0, 0);
+                floatx4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[t], zero, 0, 0, 0);
                 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qh[t], r, 0, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[hf][e] = fmaf((float)d[e].s[t], r[e], s[hf][e]);
@@ -120,7 +120,7 @@ struct Q8Rows : AttnRows<HD> {
             for (int t = 0; t < NB; ++t) big = max(big, step_bits(one.s[t]));
         }
         float p[8];
-        this->template weights<MASKED>(s, big, step_exponent, p);
+        this->template weights<2, MASKED>(s, big, step_exponent, p);
         // the transposing read: lane j of a group names half (j & 1) of the 16
         // columns of the key of slot 8g + j / 2 (slot 8g + e is the lane's e-th key)
         const int tkey = 16 * (j >> 3) + 4 * g + ((j >> 1) & 3);
@@ -129,10 +129,9 @@ struct Q8Rows : AttnRows<HD> {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float d = (float)dv[e].s[t];
+                x[e] = times(p[e], dv[e].s[t]);
                 // a step that the row does not see may be anything
-                if (MASKED) d = bits >> (16 * (e >> 2) + (e & 3)) & 1 ? d : 0.f;
-                x[e] = p[e] * d;
+                if (MASKED) x[e] = bits >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : 0.f;
             }
             half8_t ph, pl;
             halves(x, ph, pl);

@@ -37,6 +37,17 @@ __device__ __forceinline__ float cols_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// Zeros to start sums of products from, in registers that the MFMA leaves as
+// they are (as a constant the compiler writes them out for every chain).
+__device__ __forceinline__ floatx4 zeros() {
+    floatx4 z = {0.f, 0.f, 0.f, 0.f};
+    asm("" : "+v"(z));
+    return z;
+}
+
+// p times an f16 step in one operation (v_fma_mix_f32).
+__device__ __forceinline__ float times(float p, _Float16 d) { return fmaf(p, (float)d, 0.f); }
+
 // x = hi + lo to 22 bits.
 __device__ __forceinline__ void halves(const float* x, half8_t& hi, half8_t& lo) {
 #pragma unroll
@@ -110,14 +121,14 @@ struct AttnRows {
         lim = 0;
     }
 
-    // The weights p of the lane's eight scores s (keys 16 hf + 4g + i of
-    // row j; -inf: not seen).  big: the largest V step, in the lane's own keys
+    // The weights p of the lane's 4 H scores s (keys 16 hf + 4g + i of row j;
+    // -inf: not seen).  big: the largest V step, in the lane's own keys
     // (EACH) or in any lane; exponent(big): e with that step in [2^(e-1), 2^e).
-    template <bool EACH, class Exponent>
+    template <int H, bool EACH, class Exponent>
     __device__ __forceinline__ void weights(const floatx4* s, int big, const Exponent& exponent, float* p) {
         float mx = s[0][0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+        for (int e = 1; e < 4 * H; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
         mx *= unq;
         if (__builtin_amdgcn_ballot_w64(mx > m + AR_SLACK || big > lim)) {
             const float mn = fmaxf(m, cols_max(mx));
@@ -142,7 +153,7 @@ struct AttnRows {
         }
         const float mref = pexp - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4 * H; ++e) {
             p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], unq, mref));
             l += p[e];
         }

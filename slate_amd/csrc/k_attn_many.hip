@@ -23,6 +23,7 @@ namespace slate_hip {
 constexpr int AM_WGS = 256;            // one workgroup per CU
 constexpr int AM_TH = 512;
 constexpr int AM_ROWS = 8 * AR_TILE;   // query rows of a block
+constexpr int AM_KEYS = 64;            // keys of a stage
 constexpr int AM_KEEP = 512;           // blocks of up to this many keys are not cut
 
 typedef short short4v __attribute__((ext_vector_type(4)));
@@ -50,25 +51,25 @@ __device__ __forceinline__ int place(int key, int c) {
 
 template <int HD, bool F32>
 struct ManyGeom {
-    static constexpr int KEYS = F32 ? 32 : 64;         // keys of a stage
-    static constexpr int PLANE = KEYS * HD;            // halves
+    static constexpr int PLANE = AM_KEYS * HD;         // halves
     static constexpr int PLANES = F32 ? 4 : 2;         // K hi (lo), V hi (lo)
     static constexpr int CH = HD / 8;                  // 8-element chunks of a row
     // what a thread brings in: 16 codes of a row, or 8 f32
     static constexpr int UNIT = F32 ? 8 : 16;
-    static constexpr int UNITS = KEYS * HD / UNIT;     // of K, and of V
+    static constexpr int UNITS = AM_KEYS * HD / UNIT;  // of K, and of V
+    static constexpr int EACH = (UNITS + AM_TH - 1) / AM_TH;   // a thread's
 };
 
 // Blocks of a sequence and their granules (stages).
 struct ManyCount {
-    int G, Hkv, keys;                  // keys of a stage
+    int G, Hkv;
     bool causal;
     __device__ __forceinline__ int blocks(const SeqView& s) const { return (s.n * G + AM_ROWS - 1) / AM_ROWS; }
     // keys that block i's rows see
     __device__ __forceinline__ int seen(const SeqView& s, int i) const {
         return s.p0 + (causal ? (min(s.n * G, (i + 1) * AM_ROWS) - 1) / G + 1 : s.n);
     }
-    __device__ __forceinline__ int granules(const SeqView& s, int i) const { return (seen(s, i) + keys - 1) / keys; }
+    __device__ __forceinline__ int granules(const SeqView& s, int i) const { return (seen(s, i) + AM_KEYS - 1) / AM_KEYS; }
     __device__ __forceinline__ int per_head(const SeqView& s) const {
         const int nb = blocks(s);
         if (!causal || nb <= 1) return nb * granules(s, 0);
@@ -118,43 +119,55 @@ __device__ __forceinline__ int many_begin(const ManyPlan& plan, const ManyCount&
     const int x = plan.begin(w, AM_WGS);
     if (x >= plan.total) return plan.total;
     const ManyPlace p = many_find(plan, c, x);
-    return p.gran * c.keys <= AM_KEEP ? x - p.in : x;
+    return p.gran * AM_KEYS <= AM_KEEP ? x - p.in : x;
 }
 
-// 32 keys of a stage against the wave's rows.
+// Keys of a stage against the wave's rows.
 template <int HD, bool F32>
 struct ManyRows : AttnRows<HD> {
     using AttnRows<HD>::qh;
     using AttnRows<HD>::ql;
     using AttnRows<HD>::o;
-    static constexpr int NB = HD / 32, ND = HD / 16, CH = HD / 8;
+    static constexpr int NB = HD / 32, ND = HD / 16;
     using Steps = Q8Steps<HD>;
+    int koff[NB], voff[ND];            // where the lane reads K's and V's operands in a plane (halves)
 
-    // planes: K hi (lo), V hi (lo); ks, vs: the keys' steps (Steps, or the
-    // power of two of a row as a float).  MASKED as in Q8Rows.  bad: keys
-    // whose V row has an element that is not finite (it is 0 in the plane),
-    // vrow the first key's row (f32).
-    template <bool MASKED>
-    __device__ __forceinline__ void keys32(const _Float16* planes, int at, const void* ks_, const void* vs_,
-                                           uint32_t seen, uint32_t bad, const float* vrow) {
-        using Geo = ManyGeom<HD, F32>;
-        const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-        const _Float16 *k = planes + at * HD, *v = k + (F32 ? 2 : 1) * Geo::PLANE;
-        const Steps *ks = (const Steps*)ks_, *vs = (const Steps*)vs_;
-        const float *kf = (const float*)ks_, *vf = (const float*)vs_;
-        floatx4 s[2];
+    __device__ __forceinline__ void offsets() {
+        const int g = (threadIdx.x & 63) >> 4, j = threadIdx.x & 15;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            const int key = 16 * hf + j;
-            s[hf] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NB; ++t) koff[t] = place<HD>(j, 4 * t + g);
+        // lane i of a group names quarter i % 4 of the 16 columns of the
+        // i / 4-th of its four keys (slots 8g .. +3 hold keys 4g + i, slots
+        // 8g + 4 .. +7 keys 16 + 4g + i)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) voff[n] = place<HD>(4 * g + (j >> 2), 2 * n + ((j & 3) >> 1)) + 4 * (j & 1);
+    }
+
+    // 16 H keys from key `at` of the stage on.  planes: K hi (lo), V hi (lo);
+    // ks, vs: the keys' steps (Steps, or the power of two of a row as a
+    // float).  MASKED as in Q8Rows (H = 2).  top: the largest V step among the
+    // keys (8-bit, all keys seen).  bad: keys whose V row has an element that
+    // is not finite (it is 0 in the plane), vrow the first key's row (f32).
+    template <int H, bool MASKED>
+    __device__ __forceinline__ void keys(const _Float16* planes, int at, const unsigned char* steps, int top,
+                                         uint32_t seen, uint32_t bad, const float* vrow) {
+        using Geo = ManyGeom<HD, F32>;
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const _Float16 *k = planes + at * HD, *v = k + (F32 ? 2 : 1) * Geo::PLANE;
+        const Steps *ks = (const Steps*)steps + at, *vs = ks + AM_KEYS;
+        const float *kf = (const float*)steps + at, *vf = kf + AM_KEYS;
+        floatx4 s[H];
+        const floatx4 zero = zeros();
+#pragma unroll
+        for (int hf = 0; hf < H; ++hf) {
+            const _Float16* kh = k + 16 * hf * HD;
             if constexpr (F32) {
 #pragma unroll
                 for (int t = 0; t < NB; ++t) {
-                    const half8_t kh = *(const half8_t*)(k + place<HD>(key, 4 * t + g));
-                    const half8_t kl = *(const half8_t*)(k + Geo::PLANE + place<HD>(key, 4 * t + g));
-                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[t], s[hf], 0, 0, 0);
-                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[t], s[hf], 0, 0, 0);
-                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[t], s[hf], 0, 0, 0);
+                    const half8_t hi = *(const half8_t*)(kh + koff[t]), lo = *(const half8_t*)(kh + Geo::PLANE + koff[t]);
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[t], t == 0 ? zero : s[hf], 0, 0, 0);
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[t], s[hf], 0, 0, 0);
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[t], s[hf], 0, 0, 0);
                 }
                 s[hf] *= *(const floatx4*)(kf + 16 * hf + 4 * g);
             } else {
@@ -163,48 +176,48 @@ struct ManyRows : AttnRows<HD> {
                 for (int i = 0; i < 4; ++i) d[i] = ks[16 * hf + 4 * g + i];
 #pragma unroll
                 for (int t = 0; t < NB; ++t) {
-                    const half8_t kc = *(const half8_t*)(k + place<HD>(key, 4 * t + g));
-                    floatx4 r = {0.f, 0.f, 0.f, 0.f};
-                    r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[t], r, 0, 0, 0);
+                    const half8_t kc = *(const half8_t*)(kh + koff[t]);
+                    floatx4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[t], zero, 0, 0, 0);
                     r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qh[t], r, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[hf][e] = fmaf((float)d[e].s[t], r[e], s[hf][e]);
+                    for (int e = 0; e < 4; ++e)
+                        s[hf][e] = t == 0 ? times(r[e], d[e].s[t]) : fmaf((float)d[e].s[t], r[e], s[hf][e]);
                 }
             }
         }
         // bit 16 (e / 4) + e % 4 of `bits`: the row sees the lane's key e
         const uint32_t bits = MASKED ? seen >> (4 * g) : 0;
-        auto sees = [&](int e) { return (bits >> (16 * (e >> 2) + (e & 3)) & 1) != 0; };
-        float p[8], x[8];
-        // lane i of a group names quarter i % 4 of the 16 columns of the
-        // i / 4-th of its four keys (slots 8g .. +3 hold keys 4g + i, slots
-        // 8g + 4 .. +7 keys 16 + 4g + i)
-        const int tkey = 4 * g + (j >> 2), tc = (j & 3) >> 1, te = 4 * (j & 1);
+        auto sees = [&](int e) { return !MASKED || (bits >> (16 * (e >> 2) + (e & 3)) & 1) != 0; };
         auto columns = [&](const _Float16* plane, int n) {
-            const half4_t a = read_columns16(plane + place<HD>(tkey, 2 * n + tc) + te);
-            const half4_t b = read_columns16(plane + place<HD>(tkey + 16, 2 * n + tc) + te);
+            const half4_t a = read_columns16(plane + voff[n]), b = read_columns16(plane + 16 * HD + voff[n]);
             return half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         };
+        float p[4 * H], x[8];
         half8_t ph, pl;
         if constexpr (F32) {
-            const floatx4 d[2] = {*(const floatx4*)(vf + 4 * g), *(const floatx4*)(vf + 16 + 4 * g)};
+            floatx4 d[H];
             int big = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool see = !MASKED || sees(e);
-                if (MASKED && !see) s[e >> 2][e & 3] = -INFINITY;
-                if (see) big = max(big, __builtin_bit_cast(int, d[e >> 2][e & 3]));
+            for (int hf = 0; hf < H; ++hf) d[hf] = *(const floatx4*)(vf + 16 * hf + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4 * H; ++e) {
+                if (!sees(e)) s[e >> 2][e & 3] = -INFINITY;
+                if (sees(e)) big = max(big, __builtin_bit_cast(int, d[e >> 2][e & 3]));
             }
-            this->template weights<true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
+            this->template weights<H, true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = p[e] * (MASKED && !sees(e) ? 0.f : d[e >> 2][e & 3]);
-            halves(x, ph, pl);
+            for (int b = 0; b < H / 2; ++b) {
+                const _Float16* vb = v + 32 * b * HD;
 #pragma unroll
-            for (int n = 0; n < ND; ++n) {
-                const half8_t vh = columns(v, n), vl = columns(v + Geo::PLANE, n);
-                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[n], 0, 0, 0);
-                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[n], 0, 0, 0);
-                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[n], 0, 0, 0);
+                for (int e = 0; e < 8; ++e) x[e] = p[8 * b + e] * (sees(e) ? d[2 * b + (e >> 2)][e & 3] : 0.f);
+                halves(x, ph, pl);
+#pragma unroll
+                for (int n = 0; n < ND; ++n) {
+                    const half8_t vh = columns(vb, n), vl = columns(vb + Geo::PLANE, n);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[n], 0, 0, 0);
+                }
             }
             if (MASKED)
                 for (uint32_t left = bad; left; left &= left - 1) {   // for the rows that do see such a row
@@ -219,40 +232,42 @@ struct ManyRows : AttnRows<HD> {
                         }
                 }
         } else {
-            Steps dv[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dv[e] = vs[16 * (e >> 2) + 4 * g + (e & 3)];
-            int big = 0;
+            int big = top;
             if (MASKED) {
+                big = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int e = 0; e < 8; ++e) {
+                    const Steps d = vs[16 * (e >> 2) + 4 * g + (e & 3)];
                     if (!sees(e)) {
                         s[e >> 2][e & 3] = -INFINITY;
                     } else {
 #pragma unroll
-                        for (int t = 0; t < NB; ++t) big = max(big, step_bits(dv[e].s[t]));
+                        for (int t = 0; t < NB; ++t) big = max(big, step_bits(d.s[t]));
                     }
-            } else {                                   // a lane looks at one key's V steps
-                const Steps one = vs[lane & 31];
-#pragma unroll
-                for (int t = 0; t < NB; ++t) big = max(big, step_bits(one.s[t]));
-            }
-            this->template weights<MASKED>(s, big, step_exponent, p);
-#pragma unroll
-            for (int t = 0; t < NB; ++t) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float d = (float)dv[e].s[t];
-                    if (MASKED) d = sees(e) ? d : 0.f;   // a step that the row does not see may be anything
-                    x[e] = p[e] * d;
                 }
-                halves(x, ph, pl);
+            }
+            this->template weights<H, true>(s, big, step_exponent, p);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int n = 2 * t + u;
-                    const half8_t vc = columns(v, n);
-                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pl, o[n], 0, 0, 0);
-                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, ph, o[n], 0, 0, 0);
+            for (int b = 0; b < H / 2; ++b) {
+                const _Float16* vb = v + 32 * b * HD;
+                Steps dv[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dv[e] = vs[32 * b + 16 * (e >> 2) + 4 * g + (e & 3)];
+#pragma unroll
+                for (int t = 0; t < NB; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = times(p[8 * b + e], dv[e].s[t]);
+                        if (MASKED) x[e] = sees(e) ? x[e] : 0.f;   // a step that the row does not see may be anything
+                    }
+                    halves(x, ph, pl);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int n = 2 * t + u;
+                        const half8_t vc = columns(vb, n);
+                        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pl, o[n], 0, 0, 0);
+                        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, ph, o[n], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -272,20 +287,21 @@ template <int HD, bool F32>
 __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
     using Geo = ManyGeom<HD, F32>;
     using Steps = Q8Steps<HD>;
-    constexpr int NB = HD / 32, ND = HD / 16, KEYS = Geo::KEYS, PLANE = Geo::PLANE;
-    constexpr int STEP = F32 ? 4 : (int)sizeof(Steps);
+    constexpr int NB = HD / 32, ND = HD / 16, KEYS = AM_KEYS, PLANE = Geo::PLANE, EACH = Geo::EACH;
+    constexpr int STEP = F32 ? 4 : (int)sizeof(Steps);   // bytes
     __shared__ __attribute__((aligned(16))) _Float16 s_rows[2][Geo::PLANES * PLANE];
     __shared__ __attribute__((aligned(16))) unsigned char s_step[2][2 * KEYS * STEP];
     __shared__ uint32_t s_seen[PK_MAX_DRAFT / 32][AM_ROWS];   // the drafts that a block's token sees
     __shared__ int16_t s_par[PK_MAX_DRAFT];
-    __shared__ uint32_t s_bad[4];
+    __shared__ uint32_t s_bad[4][2];                  // f32: keys whose V row has an element that is not finite
+    __shared__ int s_top[2][2];                       // 8-bit: the largest V step of each 32 keys
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, j = lane & 15;
     const int G = a.Hq / a.Hkv;
     // neighbouring ranges on one XCD: blocks that share keys find them in its L2
     const int wg = (blockIdx.x % 8) * (AM_WGS / 8) + blockIdx.x / 8;
-    const ManyCount count{G, a.Hkv, KEYS, a.parent == nullptr};
+    const ManyCount count{G, a.Hkv, a.parent == nullptr};
     const ManyPlan plan(pb, count);
     auto begin = [&](int v) { return many_begin(plan, count, v); };
     const int x0 = begin(wg), x1 = begin(wg + 1);
@@ -294,7 +310,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
         return;
     }
     const float scale2 = (1.0f / sqrtf((float)HD)) * LOG2E;
-    if (tid < 4) s_bad[tid] = 0;
+    if (tid < 8) s_bad[tid >> 1][tid & 1] = 0;
 
     struct Piece {
         SeqView seq;
@@ -310,24 +326,28 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     // a stage's rows on their way: the thread's unit of K and of V, and steps
     // (rows past the last key repeat it: nobody sees them)
     typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-    uint4v raw_k, raw_v;
-    float4u f_k[2], f_v[2];
+    uint4v raw[2][EACH];                               // 8-bit: K's and V's codes
+    float4u f32[2][EACH][2];
     Steps st;
-    const int unit = tid * Geo::UNIT / HD, elem = tid * Geo::UNIT % HD;   // key and element of the thread's unit
-    const bool mine = tid < Geo::UNITS;
+    // key and element of the thread's unit u
+    auto unit_key = [&](int u) { return (tid + AM_TH * u) * Geo::UNIT / HD; };
+    auto unit_elem = [&](int u) { return (tid + AM_TH * u) * Geo::UNIT % HD; };
+    const bool mine = Geo::UNITS >= AM_TH || tid < Geo::UNITS;
     auto load = [&](const Piece& p, int gr) {
         const int k0 = gr * KEYS;
-        const int64_t row = min(k0 + unit, p.last);
         if (mine) {
-            const int64_t e = p.at + row * HD + elem;
-            if constexpr (F32) {
-                f_k[0] = *(const float4u*)(a.kf + e);
-                f_k[1] = *(const float4u*)(a.kf + e + 4);
-                f_v[0] = *(const float4u*)(a.vf + e);
-                f_v[1] = *(const float4u*)(a.vf + e + 4);
-            } else {
-                raw_k = *(const uint4v*)(a.kv8.kq + e);
-                raw_v = *(const uint4v*)(a.kv8.vq + e);
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) {
+                const int64_t e = p.at + (int64_t)min(k0 + unit_key(u), p.last) * HD + unit_elem(u);
+                if constexpr (F32) {
+                    f32[0][u][0] = *(const float4u*)(a.kf + e);
+                    f32[0][u][1] = *(const float4u*)(a.kf + e + 4);
+                    f32[1][u][0] = *(const float4u*)(a.vf + e);
+                    f32[1][u][1] = *(const float4u*)(a.vf + e + 4);
+                } else {
+                    raw[0][u] = *(const uint4v*)(a.kv8.kq + e);
+                    raw[1][u] = *(const uint4v*)(a.kv8.vq + e);
+                }
             }
         }
         if (!F32 && tid < 2 * KEYS) {
@@ -338,44 +358,51 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     // and into LDS; `masked`: some row may not see some key of it
     auto put = [&](int to, int ring, bool masked) {
         _Float16* rows = s_rows[to];
-        if constexpr (F32) {
-            if (mine) {
-                float* steps = (float*)s_step[to];
+        if (mine) {
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) {
+                const int key = unit_key(u), elem = unit_elem(u);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
-                    float x[8], top = 0.f;
+                    _Float16* at = rows + kv * (Geo::PLANES / 2) * PLANE;
+                    if constexpr (F32) {
+                        float x[8], top = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = kv == 0 ? f_k[e >> 2][e & 3] : f_v[e >> 2][e & 3];
-                        if (kv == 1 && masked && !(fabsf(x[e]) < INFINITY)) {
-                            x[e] = 0.f;
-                            atomicOr(&s_bad[ring], 1u << unit);
+                        for (int e = 0; e < 8; ++e) {
+                            x[e] = f32[kv][u][e >> 2][e & 3];
+                            if (kv == 1 && masked && !(fabsf(x[e]) < INFINITY)) {
+                                x[e] = 0.f;
+                                atomicOr(&s_bad[ring][key >> 5], 1u << (key & 31));
+                            }
+                            top = fmaxf(top, fabsf(x[e]));
                         }
-                        top = fmaxf(top, fabsf(x[e]));
+                        top = lanes_max<HD / 8>(top);
+                        const int e2 = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], e2);
+                        half8_t hi, lo;
+                        halves(x, hi, lo);
+                        *(half8_t*)(at + place<HD>(key, elem / 8)) = hi;
+                        *(half8_t*)(at + PLANE + place<HD>(key, elem / 8)) = lo;
+                        if (elem == 0) ((float*)s_step[to])[kv * KEYS + key] = ldexpf(1.0f, -e2);
+                    } else {
+                        const uint4v r = raw[kv][u];
+                        *(half8_t*)(at + place<HD>(key, elem / 8)) = codes_f16(uint2v{r[0], r[1]});
+                        *(half8_t*)(at + place<HD>(key, elem / 8 + 1)) = codes_f16(uint2v{r[2], r[3]});
                     }
-                    top = lanes_max<HD / 8>(top);
-                    const int e2 = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], e2);
-                    half8_t hi, lo;
-                    halves(x, hi, lo);
-                    _Float16* at = rows + 2 * kv * PLANE + place<HD>(unit, elem / 8);
-                    *(half8_t*)at = hi;
-                    *(half8_t*)(at + PLANE) = lo;
-                    if (elem == 0) steps[kv * KEYS + unit] = ldexpf(1.0f, -e2);
                 }
             }
-        } else {
-            if (mine) {
+        }
+        if (!F32 && tid < 2 * KEYS) {
+            ((Steps*)s_step[to])[tid] = st;
+            if (tid >= KEYS) {                         // wave 1: a V row's steps per lane
+                int top = 0;
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const uint4v r = kv == 0 ? raw_k : raw_v;
-                    _Float16* at = rows + kv * PLANE;
-                    *(half8_t*)(at + place<HD>(unit, elem / 8)) = codes_f16(uint2v{r[0], r[1]});
-                    *(half8_t*)(at + place<HD>(unit, elem / 8 + 1)) = codes_f16(uint2v{r[2], r[3]});
-                }
+                for (int t = 0; t < NB; ++t) top = max(top, step_bits(st.s[t]));
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) top = max(top, __shfl_xor(top, off));
+                if ((lane & 31) == 0) s_top[to][lane >> 5] = top;
             }
-            if (tid < 2 * KEYS) ((Steps*)s_step[to])[tid] = st;
         }
     };
     // keys below it are seen by all rows of the piece's block
@@ -418,6 +445,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
         const bool live = rw + j < rows;
         const int tok = row / G;
         ManyRows<HD, F32> R;
+        R.offsets();
         R.start(a.q + ((int64_t)(sv.t0 + (live ? tok : 0)) * a.Hq + h * G + (live ? row % G : 0)) * HD, live, scale2);
         // keys below `open` are seen by all of the wave's rows, from `end` on by none
         const int open = a.parent ? sv.p0 : sv.p0 + (r0 + min(rw, rows - 1)) / G + 1;
@@ -447,32 +475,37 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             const int now = to, now_ring = ring;
             to ^= 1;
             ring = (ring + 1) & 3;
-            if (tid == 0) s_bad[(ring + 1) & 3] = 0;   // last read two stages ago, next set after the next barrier
+            if (F32 && tid < 2) s_bad[(ring + 1) & 3][tid] = 0;   // last read two stages ago, next set after a barrier
             if (coming) {
                 put_piece(nx, ngr, to, ring);
                 if ((coming = advance())) load(nx, ngr);
             }
+            const int k0 = gr * KEYS;
+            const _Float16* planes = s_rows[now];
+            const unsigned char* steps = s_step[now];
+            const int top0 = F32 ? 0 : s_top[now][0], top1 = F32 ? 0 : s_top[now][1];
+            if (k0 + KEYS <= open && k0 < end) {
+                R.template keys<4, false>(planes, 0, steps, max(top0, top1), 0, 0, nullptr);
+                continue;
+            }
 #pragma unroll 1
-            for (int at = 0; at < KEYS; at += AR_KEYS) {
-                const int k0 = gr * KEYS + at;
-                if (k0 >= end) break;
-                const unsigned char *ks = s_step[now] + at * STEP, *vs = ks + KEYS * STEP;
-                if (k0 + AR_KEYS <= open) {
-                    R.template keys32<false>(s_rows[now], at, ks, vs, 0, 0, nullptr);
+            for (int at = 0; at < KEYS && k0 + at < end; at += AR_KEYS) {
+                if (k0 + at + AR_KEYS <= open) {
+                    R.template keys<2, false>(planes, at, steps, at ? top1 : top0, 0, 0, nullptr);
                     continue;
                 }
                 uint32_t seen = 0;
                 if (live && !a.parent) {
-                    const int n = min(32, max(0, sv.p0 + tok + 1 - k0));
+                    const int n = min(32, max(0, sv.p0 + tok + 1 - k0 - at));
                     seen = n == 32 ? 0xffffffffu : (1u << n) - 1;
                 } else if (live) {
-                    const int d = k0 - sv.p0, wd = d >> 5;
+                    const int d = k0 + at - sv.p0, wd = d >> 5;
                     const uint32_t lo = wd < 0 ? 0xffffffffu : wd < words ? s_seen[wd][tok - tok0] : 0;
                     const uint32_t hi = wd + 1 < 0 ? 0xffffffffu : wd + 1 < words ? s_seen[wd + 1][tok - tok0] : 0;
                     seen = (uint32_t)(((uint64_t)hi << 32 | lo) >> (d & 31));
                 }
-                R.template keys32<true>(s_rows[now], at, ks, vs, seen, F32 ? s_bad[now_ring] : 0,
-                                        F32 ? a.vf + pc.at + (int64_t)k0 * HD : nullptr);
+                R.template keys<2, true>(planes, at, steps, 0, seen, F32 ? s_bad[now_ring][at >> 5] : 0,
+                                         F32 ? a.vf + pc.at + (int64_t)(k0 + at) * HD : nullptr);
             }
         }
         const bool whole = pc.g0 == 0 && pc.g1 == pc.gran;
