@@ -81,6 +81,11 @@ class Plan {
         return total < P ? min(w, total) : (int)((uint64_t)(uint32_t)total * (uint32_t)w / (uint32_t)P);
     }
 
+    // The first workgroup whose range begins at x or later.
+    __device__ __forceinline__ int first_from(int x, int P) const {
+        return total < P ? x : (int)(((uint64_t)(uint32_t)x * (uint32_t)P + (uint32_t)total - 1) / (uint32_t)total);
+    }
+
   private:
     struct Lane {
         SeqView seq;
@@ -128,15 +133,12 @@ void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_ro
 // The entry of workgroup w, whose range begins at x0 in granule `in` of a
 // block of `gran`; begin(w) are the ranges' beginnings.  Called by a whole
 // wave (the searches are the wave's).
-template <class Begin>
-__device__ __forceinline__ void leave_entry(void* ws, int P, int w, int x0, int in, int gran, const Begin& begin, JoinEntry e) {
-    const int start = x0 - in, end = start + gran;
+template <class PlanT, class Begin>
+__device__ __forceinline__ void leave_entry(void* ws, int P, int w, int x0, int in, int gran, const PlanT& plan,
+                                            const Begin& begin, JoinEntry e) {
+    const int start = x0 - in;
     const int from = in > 0 ? begin(w - 1) : 0;
-    e.pieces = 0;
-    if (in > 0 && from <= start) {
-        e.pieces = 2;
-        while (w - 1 + e.pieces < P && begin(w - 1 + e.pieces) < end) ++e.pieces;
-    }
+    e.pieces = in > 0 && from <= start ? min(P, plan.first_from(start + gran, P)) - (w - 1) : 0;
     if (e.pieces == 0) e.rows = 0;
     e.slot0 = 2 * (w - 1) + (from != start);
     if ((threadIdx.x & 63) == 0) *entry_of(ws, w) = e;

@@ -50,11 +50,15 @@ __device__ __forceinline__ float times(float p, _Float16 d) { return fmaf(p, (fl
 
 // x = hi + lo to 22 bits.
 __device__ __forceinline__ void halves(const float* x, half8_t& hi, half8_t& lo) {
+    float minus = -1.0f;               // the compiler does not see that it could subtract
+    asm("" : "+s"(minus));
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
         const float2v v = {x[e], x[e + 1]};
         const half2_t h = __builtin_convertvector(v, half2_t);
-        const half2_t l = __builtin_convertvector(v - __builtin_convertvector(h, float2v), half2_t);
+        // x - hi, exact, in one operation that takes hi as it is (v_fma_mix_f32)
+        const float2v r = {fmaf((float)h[0], minus, x[e]), fmaf((float)h[1], minus, x[e + 1])};
+        const half2_t l = __builtin_convertvector(r, half2_t);
         hi[e] = h[0];
         hi[e + 1] = h[1];
         lo[e] = l[0];

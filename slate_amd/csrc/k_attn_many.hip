@@ -3,10 +3,11 @@
 // chunks, mixed steps, drafted trees.  The arithmetic: attn_rows.h, how the
 // keys are shared out: attn_plan.h.
 //
-// A workgroup of eight waves takes a block of 128 query rows, 16 a wave, over
-// a range of keys.  A stage of keys is brought into LDS as f16 once for all
-// waves, while the stage before is worked on and the one after is on its way
-// in registers; one barrier a stage.
+// A workgroup of W waves takes a block of 16 W query rows over a range of
+// keys: a wave 16 rows, or, where the block has fewer rows, several waves the
+// same 16 rows and a part of the keys each.  A stage of keys is brought into
+// LDS as f16 once for all waves, while the stage before is worked on and the
+// one after is on its way in registers; one barrier a stage.
 //   8-bit: the codes (exact in f16); a key's scores and weights go by its
 //       steps, block by block of 32 elements.  Two MFMAs a product.
 //   f32: a row of K or V is scaled by a power of two to [2^13, 2^14) at its
@@ -20,9 +21,6 @@
 
 namespace slate_hip {
 
-constexpr int AM_WGS = 256;            // one workgroup per CU
-constexpr int AM_TH = 512;
-constexpr int AM_ROWS = 8 * AR_TILE;   // query rows of a block
 constexpr int AM_KEYS = 64;            // keys of a stage
 constexpr int AM_KEEP = 512;           // blocks of up to this many keys are not cut
 
@@ -49,25 +47,28 @@ __device__ __forceinline__ int place(int key, int c) {
     return key * HD + 8 * (c ^ turn<HD>(key));
 }
 
-template <int HD, bool F32>
+template <int HD, bool F32, int W>
 struct ManyGeom {
+    static constexpr int TH = 64 * W;                  // threads
+    static constexpr int ROWS = AR_TILE * W;           // query rows of a block
+    static constexpr int WGS = 2048 / W;               // eight waves per CU
     static constexpr int PLANE = AM_KEYS * HD;         // halves
     static constexpr int PLANES = F32 ? 4 : 2;         // K hi (lo), V hi (lo)
     static constexpr int CH = HD / 8;                  // 8-element chunks of a row
     // what a thread brings in: 16 codes of a row, or 8 f32
     static constexpr int UNIT = F32 ? 8 : 16;
     static constexpr int UNITS = AM_KEYS * HD / UNIT;  // of K, and of V
-    static constexpr int EACH = (UNITS + AM_TH - 1) / AM_TH;   // a thread's
+    static constexpr int EACH = (UNITS + TH - 1) / TH;   // a thread's
 };
 
 // Blocks of a sequence and their granules (stages).
 struct ManyCount {
-    int G, Hkv;
+    int G, Hkv, rows;                  // rows of a block
     bool causal;
-    __device__ __forceinline__ int blocks(const SeqView& s) const { return (s.n * G + AM_ROWS - 1) / AM_ROWS; }
+    __device__ __forceinline__ int blocks(const SeqView& s) const { return (s.n * G + rows - 1) / rows; }
     // keys that block i's rows see
     __device__ __forceinline__ int seen(const SeqView& s, int i) const {
-        return s.p0 + (causal ? (min(s.n * G, (i + 1) * AM_ROWS) - 1) / G + 1 : s.n);
+        return s.p0 + (causal ? (min(s.n * G, (i + 1) * rows) - 1) / G + 1 : s.n);
     }
     __device__ __forceinline__ int granules(const SeqView& s, int i) const { return (seen(s, i) + AM_KEYS - 1) / AM_KEYS; }
     __device__ __forceinline__ int per_head(const SeqView& s) const {
@@ -115,8 +116,8 @@ __device__ __forceinline__ ManyPlace many_find(const ManyPlan& plan, const ManyC
         r.in -= __builtin_amdgcn_readlane(upto, 63);
     }
 }
-__device__ __forceinline__ int many_begin(const ManyPlan& plan, const ManyCount& c, int w) {
-    const int x = plan.begin(w, AM_WGS);
+__device__ __forceinline__ int many_begin(const ManyPlan& plan, const ManyCount& c, int w, int P) {
+    const int x = plan.begin(w, P);
     if (x >= plan.total) return plan.total;
     const ManyPlace p = many_find(plan, c, x);
     return p.gran * AM_KEYS <= AM_KEEP ? x - p.in : x;
@@ -151,9 +152,9 @@ struct ManyRows : AttnRows<HD> {
     template <int H, bool MASKED>
     __device__ __forceinline__ void keys(const _Float16* planes, int at, const unsigned char* steps, int top,
                                          uint32_t seen, uint32_t bad, const float* vrow) {
-        using Geo = ManyGeom<HD, F32>;
+        constexpr int PLANE = AM_KEYS * HD;
         const int lane = threadIdx.x & 63, g = lane >> 4;
-        const _Float16 *k = planes + at * HD, *v = k + (F32 ? 2 : 1) * Geo::PLANE;
+        const _Float16 *k = planes + at * HD, *v = k + (F32 ? 2 : 1) * PLANE;
         const Steps *ks = (const Steps*)steps + at, *vs = ks + AM_KEYS;
         const float *kf = (const float*)steps + at, *vf = kf + AM_KEYS;
         floatx4 s[H];
@@ -164,7 +165,7 @@ struct ManyRows : AttnRows<HD> {
             if constexpr (F32) {
 #pragma unroll
                 for (int t = 0; t < NB; ++t) {
-                    const half8_t hi = *(const half8_t*)(kh + koff[t]), lo = *(const half8_t*)(kh + Geo::PLANE + koff[t]);
+                    const half8_t hi = *(const half8_t*)(kh + koff[t]), lo = *(const half8_t*)(kh + PLANE + koff[t]);
                     s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[t], t == 0 ? zero : s[hf], 0, 0, 0);
                     s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[t], s[hf], 0, 0, 0);
                     s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[t], s[hf], 0, 0, 0);
@@ -213,7 +214,7 @@ struct ManyRows : AttnRows<HD> {
                 halves(x, ph, pl);
 #pragma unroll
                 for (int n = 0; n < ND; ++n) {
-                    const half8_t vh = columns(vb, n), vl = columns(vb + Geo::PLANE, n);
+                    const half8_t vh = columns(vb, n), vl = columns(vb + PLANE, n);
                     o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[n], 0, 0, 0);
                     o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[n], 0, 0, 0);
                     o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[n], 0, 0, 0);
@@ -283,27 +284,34 @@ __device__ __forceinline__ float lanes_max(float v) {
     return fmaxf(v, dpp_mov<DPP_QUAD_XOR2>(v));
 }
 
-template <int HD, bool F32>
-__global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
-    using Geo = ManyGeom<HD, F32>;
+template <int HD, bool F32, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
+    using Geo = ManyGeom<HD, F32, W>;
+    constexpr int TH = Geo::TH, ROWS = Geo::ROWS, WGS = Geo::WGS;
     using Steps = Q8Steps<HD>;
     constexpr int NB = HD / 32, ND = HD / 16, KEYS = AM_KEYS, PLANE = Geo::PLANE, EACH = Geo::EACH;
     constexpr int STEP = F32 ? 4 : (int)sizeof(Steps);   // bytes
     __shared__ __attribute__((aligned(16))) _Float16 s_rows[2][Geo::PLANES * PLANE];
     __shared__ __attribute__((aligned(16))) unsigned char s_step[2][2 * KEYS * STEP];
-    __shared__ uint32_t s_seen[PK_MAX_DRAFT / 32][AM_ROWS];   // the drafts that a block's token sees
+    __shared__ uint32_t s_seen[PK_MAX_DRAFT / 32][ROWS];   // the drafts that a block's token sees
     __shared__ int16_t s_par[PK_MAX_DRAFT];
     __shared__ uint32_t s_bad[4][2];                  // f32: keys whose V row has an element that is not finite
     __shared__ int s_top[2][2];                       // 8-bit: the largest V step of each 32 keys
+    // what the waves that share rows leave for each other: where the stage
+    // that is worked through was, if it fits
+    constexpr int OS = HD + 4;
+    constexpr int JOIN_FLOATS = (W - 1) * AR_TILE * OS;
+    constexpr bool JOIN_IN_ROWS = JOIN_FLOATS * 4 <= Geo::PLANES * PLANE * 2;
+    __shared__ __attribute__((aligned(16))) float s_join[JOIN_IN_ROWS ? 4 : JOIN_FLOATS];
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, j = lane & 15;
     const int G = a.Hq / a.Hkv;
     // neighbouring ranges on one XCD: blocks that share keys find them in its L2
-    const int wg = (blockIdx.x % 8) * (AM_WGS / 8) + blockIdx.x / 8;
-    const ManyCount count{G, a.Hkv, a.parent == nullptr};
+    const int wg = (blockIdx.x % 8) * (WGS / 8) + blockIdx.x / 8;
+    const ManyCount count{G, a.Hkv, ROWS, a.parent == nullptr};
     const ManyPlan plan(pb, count);
-    auto begin = [&](int v) { return many_begin(plan, count, v); };
+    auto begin = [&](int v) { return many_begin(plan, count, v, WGS); };
     const int x0 = begin(wg), x1 = begin(wg + 1);
     if (x0 >= x1) {
         if (tid == 0) entry_of(a.ws, wg)->rows = 0;
@@ -330,9 +338,9 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     float4u f32[2][EACH][2];
     Steps st;
     // key and element of the thread's unit u
-    auto unit_key = [&](int u) { return (tid + AM_TH * u) * Geo::UNIT / HD; };
-    auto unit_elem = [&](int u) { return (tid + AM_TH * u) * Geo::UNIT % HD; };
-    const bool mine = Geo::UNITS >= AM_TH || tid < Geo::UNITS;
+    auto unit_key = [&](int u) { return (tid + TH * u) * Geo::UNIT / HD; };
+    auto unit_elem = [&](int u) { return (tid + TH * u) * Geo::UNIT % HD; };
+    const bool mine = Geo::UNITS >= TH || tid < Geo::UNITS;
     auto load = [&](const Piece& p, int gr) {
         const int k0 = gr * KEYS;
         if (mine) {
@@ -368,14 +376,19 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
                     if constexpr (F32) {
                         float x[8], top = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            x[e] = f32[kv][u][e >> 2][e & 3];
-                            if (kv == 1 && masked && !(fabsf(x[e]) < INFINITY)) {
-                                x[e] = 0.f;
-                                atomicOr(&s_bad[ring][key >> 5], 1u << (key & 31));
+                        for (int e = 0; e < 8; ++e) x[e] = f32[kv][u][e >> 2][e & 3];
+                        if (kv == 1 && masked) {
+                            bool bad = false;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const bool fine = fabsf(x[e]) < INFINITY;
+                                bad |= !fine;
+                                x[e] = fine ? x[e] : 0.f;
                             }
-                            top = fmaxf(top, fabsf(x[e]));
+                            if (bad) atomicOr(&s_bad[ring][key >> 5], 1u << (key & 31));
                         }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
                         top = lanes_max<HD / 8>(top);
                         const int e2 = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
 #pragma unroll
@@ -407,16 +420,26 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     };
     // keys below it are seen by all rows of the piece's block
     auto open_to = [&](const Piece& p) {
-        return a.parent ? p.seq.p0 : p.seq.p0 + p.block * AM_ROWS / G + 1;
+        return a.parent ? p.seq.p0 : p.seq.p0 + p.block * ROWS / G + 1;
     };
     auto put_piece = [&](const Piece& p, int gr, int to, int ring) { put(to, ring, (gr + 1) * KEYS > open_to(p)); };
 
+    // How a block's rows go to the waves: T tiles of 16 rows, each taken by
+    // W / T waves, which share the keys 32 by 32.
+    struct Share {
+        int part, parts, r;            // the wave's part of the keys, and how many there are; its first row in the block
+    };
+    auto share_of = [&](const Piece& p) {
+        const int rows = min(ROWS, p.seq.n * G - p.block * ROWS);
+        const int tiles = rows <= AR_TILE ? 1 : rows <= 2 * AR_TILE ? 2 : rows <= 4 * AR_TILE ? 4 : W;
+        return Share{w / tiles, W / tiles, AR_TILE * (w % tiles)};
+    };
     Piece pc = piece_at(x0), nx = pc;                  // worked on; being loaded
     int ngr = pc.g0, nx_x = x0;                        // the stage being loaded, its piece's place on the line
     load(nx, ngr);
     if (w == 0)
-        leave_entry(a.ws, AM_WGS, wg, x0, pc.g0, pc.gran, begin,
-                    JoinEntry{pc.seq.t0, min(AM_ROWS, pc.seq.n * G - pc.block * AM_ROWS), pc.block * AM_ROWS, pc.h, 0,
+        leave_entry(a.ws, WGS, wg, x0, pc.g0, pc.gran, plan, begin,
+                    JoinEntry{pc.seq.t0, min(ROWS, pc.seq.n * G - pc.block * ROWS), pc.block * ROWS, pc.h, 0,
                               0});
     // the next stage after the one being loaded; false at the range's end
     auto advance = [&]() {
@@ -431,29 +454,40 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
         ngr = nx.g0;
         return true;
     };
-    __syncthreads();                                   // s_bad is clear
-    put_piece(nx, ngr, 0, 0);
-    bool coming = advance();
-    if (coming) load(nx, ngr);
+    bool coming = true;
     int to = 0, ring = 0;
 
     for (int x = x0;;) {
         const SeqView sv = pc.seq;
-        const int h = pc.h, r0 = pc.block * AM_ROWS, rows = min(AM_ROWS, sv.n * G - r0);
-        const int rw = AR_TILE * w, tok0 = r0 / G;     // the wave's first row in the block, the block's first token
+        const int h = pc.h, r0 = pc.block * ROWS, rows = min(ROWS, sv.n * G - r0);
+        const Share sh = share_of(pc);
+        const int rw = sh.r, tok0 = r0 / G;            // the wave's first row in the block, the block's first token
         const int row = r0 + rw + j;
         const bool live = rw + j < rows;
         const int tok = row / G;
         ManyRows<HD, F32> R;
         R.offsets();
-        R.start(a.q + ((int64_t)(sv.t0 + (live ? tok : 0)) * a.Hq + h * G + (live ? row % G : 0)) * HD, live, scale2);
+        float4u qraw[NB][2];
+        const float* qp =
+            a.q + ((int64_t)(sv.t0 + (live ? tok : 0)) * a.Hq + h * G + (live ? row % G : 0)) * HD + 8 * g;
+#pragma unroll
+        for (int t = 0; t < NB; ++t) {
+            qraw[t][0] = *(const float4u*)(qp + 32 * t);
+            qraw[t][1] = *(const float4u*)(qp + 32 * t + 4);
+        }
+        if (x == x0) {                                 // the first stage, once q is on its way too
+            __syncthreads();                           // s_bad is clear
+            put_piece(nx, ngr, 0, 0);
+            if ((coming = advance())) load(nx, ngr);
+        }
+        R.start(qraw, live, scale2);
         // keys below `open` are seen by all of the wave's rows, from `end` on by none
         const int open = a.parent ? sv.p0 : sv.p0 + (r0 + min(rw, rows - 1)) / G + 1;
         const int end = rw >= rows ? 0 : a.parent ? sv.p0 + sv.n : sv.p0 + (r0 + min(rw + AR_TILE, rows) - 1) / G + 1;
         const int words = (sv.n + 31) / 32;
         if (a.parent && pc.g1 * KEYS > sv.p0) {        // the block's tokens' ancestors
             __syncthreads();
-            for (int i = tid; i < sv.n; i += AM_TH) {
+            for (int i = tid; i < sv.n; i += TH) {
                 const int up = a.parent[sv.t0 + i];
                 s_par[i] = (int16_t)(up >= 0 && up < i ? up : -1);
             }
@@ -484,12 +518,13 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             const _Float16* planes = s_rows[now];
             const unsigned char* steps = s_step[now];
             const int top0 = F32 ? 0 : s_top[now][0], top1 = F32 ? 0 : s_top[now][1];
-            if (k0 + KEYS <= open && k0 < end) {
+            if (sh.parts == 1 && k0 + KEYS <= open && k0 < end) {
                 R.template keys<4, false>(planes, 0, steps, max(top0, top1), 0, 0, nullptr);
                 continue;
             }
 #pragma unroll 1
             for (int at = 0; at < KEYS && k0 + at < end; at += AR_KEYS) {
+                if (((2 * gr + at / AR_KEYS) & (sh.parts - 1)) != sh.part) continue;
                 if (k0 + at + AR_KEYS <= open) {
                     R.template keys<2, false>(planes, at, steps, at ? top1 : top0, 0, 0, nullptr);
                     continue;
@@ -509,38 +544,79 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             }
         }
         const bool whole = pc.g0 == 0 && pc.g1 == pc.gran;
-        const float back = R.back(), l = R.sum();
-        if (live) {
+        const int xn = x + pc.g1 - pc.g0;
+        const float back = R.back();
+        float l = R.sum();
+#pragma unroll
+        for (int n = 0; n < ND; ++n) R.o[n] *= back;
+        if (sh.parts > 1) {                            // the parts of the keys joined
+            float* area = JOIN_IN_ROWS ? (float*)s_rows[to ^ 1] : s_join;
+            const int tiles = W / sh.parts, tile = rw / AR_TILE;
+            __syncthreads();
+            if (sh.part > 0) {
+                float* at = area + ((sh.part - 1) * tiles + tile) * AR_TILE * OS + j * OS;
+#pragma unroll
+                for (int n = 0; n < ND; ++n) *(floatx4*)(at + 16 * n + 4 * g) = R.o[n];
+                if (g == 0) *(float2*)(at + HD) = make_float2(R.m, l);
+            }
+            __syncthreads();
+            for (int k = 1; k < sh.parts && sh.part == 0; ++k) {
+                const float* at = area + ((k - 1) * tiles + tile) * AR_TILE * OS + j * OS;
+                const float2 ml = *(const float2*)(at + HD);
+                const float mt = fmaxf(R.m, ml.x);
+                const float f0 = R.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(R.m - mt);
+                const float f1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mt);
+                R.m = mt;
+                l = l * f0 + ml.y * f1;
+#pragma unroll
+                for (int n = 0; n < ND; ++n) {
+                    const floatx4 other = *(const floatx4*)(at + 16 * n + 4 * g);
+                    R.o[n] = (f0 == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : R.o[n] * f0) +
+                             (f1 == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : other * f1);
+                }
+            }
+        }
+        if (live && sh.part == 0) {
             if (whole) {
                 float* op = a.out + ((int64_t)(sv.t0 + tok) * a.Hq + h * G + row % G) * HD + 4 * g;
-                const float inv = back / l;
+                const float inv = 1.0f / l;
 #pragma unroll
                 for (int n = 0; n < ND; ++n) *(float4u*)(op + 16 * n) = R.o[n] * inv;
             } else {
-                float* slot = slot_of(a.ws, AM_WGS, 2 * wg + (x == x0 ? 0 : 1), AM_ROWS, HD);
+                float* slot = slot_of(a.ws, WGS, 2 * wg + (x == x0 ? 0 : 1), ROWS, HD);
                 const int r = rw + j;
-                if (g == 0) *(float2*)(slot + AM_ROWS * HD + 2 * r) = make_float2(R.m, l);
+                if (g == 0) *(float2*)(slot + ROWS * HD + 2 * r) = make_float2(R.m, l);
 #pragma unroll
-                for (int n = 0; n < ND; ++n) *(floatx4*)(slot + r * HD + 16 * n + 4 * g) = R.o[n] * back;
+                for (int n = 0; n < ND; ++n) *(floatx4*)(slot + r * HD + 16 * n + 4 * g) = R.o[n];
             }
         }
-        x += pc.g1 - pc.g0;
-        if (x >= x1) break;
+        if (xn >= x1) break;
+        x = xn;
         pc = piece_at(x);
     }
 }
 
-int64_t attention_many_bytes(int hd) { return plan_bytes(AM_WGS, AM_ROWS, hd); }
+int64_t attention_many_bytes(int hd) {
+    return max(plan_bytes(ManyGeom<128, true, 8>::WGS, ManyGeom<128, true, 8>::ROWS, hd),
+               plan_bytes(ManyGeom<128, true, 4>::WGS, ManyGeom<128, true, 4>::ROWS, hd));
+}
 bool attention_many_takes(const PackedAttn& a) { return a.hd == 32 || a.hd == 64 || a.hd == 128; }
 
+template <int HD, bool F32, int W>
+static void launch_many_w(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
+    using Geo = ManyGeom<HD, F32, W>;
+    hipLaunchKernelGGL((attn_many_kernel<HD, F32, W>), dim3(Geo::WGS), dim3(Geo::TH), 0, s, a, pb);
+    if (pb.max_seq > AM_KEEP)                          // else no block is cut
+        launch_attn_join(a.out, a.ws, a.Hq, a.Hkv, HD, Geo::ROWS, Geo::WGS, s);
+}
 template <int HD>
 static void launch_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
     if (a.kf)
-        hipLaunchKernelGGL((attn_many_kernel<HD, true>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
+        launch_many_w<HD, true, 8>(a, pb, s);
+    else if ((int64_t)pb.max_new * (a.Hq / a.Hkv) > ManyGeom<HD, false, 4>::ROWS)
+        launch_many_w<HD, false, 8>(a, pb, s);
     else
-        hipLaunchKernelGGL((attn_many_kernel<HD, false>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
-    if (pb.max_seq > AM_KEEP)                          // else no block is cut
-        launch_attn_join(a.out, a.ws, a.Hq, a.Hkv, HD, AM_ROWS, AM_WGS, s);
+        launch_many_w<HD, false, 4>(a, pb, s);
 }
 
 int launch_attention_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {

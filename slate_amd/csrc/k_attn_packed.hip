@@ -96,14 +96,16 @@ __global__ __launch_bounds__(256) void attn_packed_rows_kernel(PackedAttn a, Pac
 // Joins the parts of a block that lies in several workgroups' ranges:
 // workgroup b takes the block that is first cut before workgroup b + 1 of the
 // attention kernel, HD / 4 lanes a row, eight parts' loads at a time.
-template <int HD, int TH>
-__global__ __launch_bounds__(TH) void attn_join_kernel(float* __restrict__ out, void* ws, int Hq, int G,
+constexpr int JOIN_TH = 512;
+template <int HD>
+__global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ out, void* ws, int Hq, int G,
                                                        int slot_rows, int P) {
     const JoinEntry en = *entry_of(ws, blockIdx.x + 1);
     const int c = 4 * (threadIdx.x % (HD / 4));
     // the first part's slot, then the first slot of each workgroup after it
     auto slot = [&](int k) { return slot_of(ws, P, k == 0 ? en.slot0 : 2 * ((int)blockIdx.x + k), slot_rows, HD); };
-    for (int r = threadIdx.x / (HD / 4); r < en.rows; r += TH / (HD / 4)) {
+    const int r = blockIdx.y * (JOIN_TH / (HD / 4)) + threadIdx.x / (HD / 4);
+    if (r < en.rows) {
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k0 = 0; k0 < en.pieces; k0 += 8) {
@@ -145,12 +147,9 @@ __global__ __launch_bounds__(TH) void attn_join_kernel(float* __restrict__ out, 
 
 template <int HD>
 static void launch_join_hd(float* out, void* ws, int Hq, int Hkv, int slot_rows, int P, hipStream_t s) {
-    if (slot_rows <= 16)
-        hipLaunchKernelGGL((attn_join_kernel<HD, 256>), dim3(P - 1), dim3(256), 0, s, out, ws, Hq, Hq / Hkv, slot_rows,
-                           P);
-    else
-        hipLaunchKernelGGL((attn_join_kernel<HD, 1024>), dim3(P - 1), dim3(1024), 0, s, out, ws, Hq, Hq / Hkv,
-                           slot_rows, P);
+    constexpr int AT_ONCE = JOIN_TH / (HD / 4);        // rows of a workgroup
+    hipLaunchKernelGGL(attn_join_kernel<HD>, dim3(P - 1, (slot_rows + AT_ONCE - 1) / AT_ONCE), dim3(JOIN_TH), 0, s, out,
+                       ws, Hq, Hq / Hkv, slot_rows, P);
 }
 
 void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, int P, hipStream_t s) {

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
     issue(pc, pc.g0, 0);
     load_q(pc);
     if (w == 0)
-        leave_entry(a.ws, AF_WGS, blockIdx.x, x0, pc.g0, pc.gran, [&](int v) { return few_begin(plan, v); },
+        leave_entry(a.ws, AF_WGS, blockIdx.x, x0, pc.g0, pc.gran, plan, [&](int v) { return few_begin(plan, v); },
                     JoinEntry{pc.seq.t0, pc.seq.n * G, 0, pc.h, 0, 0});
 
     for (int x = x0;;) {
