@@ -11,72 +11,85 @@
 
 namespace slate_hip {
 
-typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));   // 16 bytes at any float
-
-// VEC = 4: a thread turns four neighbouring pairs by 16-byte loads and
-// stores, which needs rot % 8 == 0; VEC = 1 takes any even rot.  A thread
-// keeps its pairs' cosines for all the heads that it walks over, and a
-// workgroup takes one row, or a part of its heads.
+// A thread owns four neighbouring pairs (VEC = 4, rot % 8 == 0) or one (VEC = 1,
+// any even rot) and walks over heads with their cosines and sines: two
+// 16-byte loads and stores a head, two heads' loads at a time.  Where the rest
+// of the head is copied (y != x) and comes in groups of eight too, the
+// threads after the pairs' copy those the same way.  A workgroup takes one
+// row, or a part of its heads where rows are few.
+// Memory bound: 4096 rows of 72 heads of 128 (302 MB) in ROPE_CHUNK_US us.
 template <int VEC>
-__global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float* x,
-                                                          const int32_t* __restrict__ pos, int n_heads, int hd,
-                                                          int64_t ld, int layout, int rot, float magnitude,
-                                                          int heads_per_wg, const RopeTurns turns) {
+__global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float* x, const int32_t* __restrict__ pos,
+                                                          int n_heads, int hd, int64_t ld, int layout, int rot,
+                                                          float magnitude, int units, int heads_per_wg,
+                                                          const RopeTurns turns) {
+    constexpr int N = VEC == 4 ? 4 : 1;
+    typedef float vec __attribute__((ext_vector_type(N), aligned(4)));
     const int row = blockIdx.x;
     const int h0 = blockIdx.y * heads_per_wg, h1 = min(n_heads, h0 + heads_per_wg);
     const float* xr = x + (int64_t)row * ld;
     float* yr = y + (int64_t)row * ld;
-    const int half = rot / 2;
-    const int units = half / VEC;                      // threads that share a head
+    const int half = rot / 2, pairs = half / VEC;      // units that turn
     const int step = (int)blockDim.x / units;          // heads side by side (units <= blockDim.x)
     const int u = threadIdx.x % units, hh = threadIdx.x / units;
-    const int i0 = u * VEC;
     if (hh < step) {
-        const double p = (double)pos[row];
+        const bool turn = u < pairs;
+        const int i0 = u * VEC;
+        // the unit's two places in a head
+        const int ja = !turn || layout ? 2 * i0 : i0, jb = turn && !layout ? half + i0 : 2 * i0 + VEC;
         float c[VEC], s[VEC];
+        if (turn) {
+            const double p = (double)pos[row];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const double t = p * turns.w[i0 + e];
-            sincospif((float)(2.0 * (t - rint(t))), &s[e], &c[e]);
-            c[e] *= magnitude;
-            s[e] *= magnitude;
+            for (int e = 0; e < VEC; ++e) {
+                const double t = p * turns.w[i0 + e];
+                sincospif((float)(2.0 * (t - rint(t))), &s[e], &c[e]);
+                c[e] *= magnitude;
+                s[e] *= magnitude;
+            }
         }
-        for (int h = h0 + hh; h < h1; h += step) {
-            const float* xh = xr + (int64_t)h * hd;
-            float* yh = yr + (int64_t)h * hd;
-            if constexpr (VEC == 4) {
-                const int ja = layout == 0 ? i0 : 2 * i0, jb = layout == 0 ? half + i0 : 2 * i0 + 4;
-                const float4u a = *(const float4u*)(xh + ja), b = *(const float4u*)(xh + jb);
-                float4u ya, yb;
-                if (layout == 0) {
+        for (int h = h0 + hh; h < h1; h += 2 * step) {
+            vec a[2], b[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        ya[e] = a[e] * c[e] - b[e] * s[e];
-                        yb[e] = b[e] * c[e] + a[e] * s[e];
-                    }
-                } else {
+            for (int k = 0; k < 2; ++k) {
+                const float* xh = xr + (int64_t)min(h + k * step, h1 - 1) * hd;
+                a[k] = *(const vec*)(xh + ja);
+                b[k] = *(const vec*)(xh + jb);
+            }
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        ya[2 * e] = a[2 * e] * c[e] - a[2 * e + 1] * s[e];
-                        ya[2 * e + 1] = a[2 * e + 1] * c[e] + a[2 * e] * s[e];
-                        yb[2 * e] = b[2 * e] * c[e + 2] - b[2 * e + 1] * s[e + 2];
-                        yb[2 * e + 1] = b[2 * e + 1] * c[e + 2] + b[2 * e] * s[e + 2];
+            for (int k = 0; k < 2; ++k) {
+                if (h + k * step >= h1) break;
+                vec ya = a[k], yb = b[k];
+                if (turn) {
+                    if constexpr (VEC == 1) {
+                        ya[0] = a[k][0] * c[0] - b[k][0] * s[0];
+                        yb[0] = b[k][0] * c[0] + a[k][0] * s[0];
+                    } else if (layout == 0) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            ya[e] = a[k][e] * c[e] - b[k][e] * s[e];
+                            yb[e] = b[k][e] * c[e] + a[k][e] * s[e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            ya[e] = a[k][e] * c[e / 2] - a[k][e + 1] * s[e / 2];
+                            ya[e + 1] = a[k][e + 1] * c[e / 2] + a[k][e] * s[e / 2];
+                            yb[e] = b[k][e] * c[2 + e / 2] - b[k][e + 1] * s[2 + e / 2];
+                            yb[e + 1] = b[k][e + 1] * c[2 + e / 2] + b[k][e] * s[2 + e / 2];
+                        }
                     }
                 }
-                *(float4u*)(yh + ja) = ya;
-                *(float4u*)(yh + jb) = yb;
-            } else {
-                const int j = layout == 0 ? i0 : 2 * i0, k = layout == 0 ? half + i0 : 2 * i0 + 1;
-                const float a = xh[j], b = xh[k];
-                yh[j] = a * c[0] - b * s[0];
-                yh[k] = b * c[0] + a * s[0];
+                float* yh = yr + (int64_t)(h + k * step) * hd;
+                *(vec*)(yh + ja) = ya;
+                *(vec*)(yh + jb) = yb;
             }
         }
     }
-    const int tail = hd - rot;
+    const int done = 2 * VEC * units, tail = hd - done;   // what the units leave of a head
     if (tail > 0 && y != x) {
         for (int e = threadIdx.x; e < (h1 - h0) * tail; e += blockDim.x) {
-            const int64_t at = (int64_t)(h0 + e / tail) * hd + rot + e % tail;
+            const int64_t at = (int64_t)(h0 + e / tail) * hd + done + e % tail;
             yr[at] = xr[at];
         }
     }
@@ -85,16 +98,17 @@ __global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float*
 int launch_rope_scaled(float* y, const float* x, const int32_t* pos, int n_rows, int n_heads, int hd, int64_t ld,
                        int layout, int rot, float magnitude, const RopeTurns& turns, hipStream_t s) {
     const bool vec = rot % 8 == 0;
-    const int step = 256 / (rot / 2 / (vec ? 4 : 1));
+    const int units = !vec ? rot / 2 : y != x && hd <= 2048 ? hd / 8 : rot / 8;
+    const int step = 256 / units;
     // few rows: a workgroup takes as many heads as it has threads for
     const int per = n_rows < 512 ? step : n_heads;
     const dim3 grid(n_rows, (n_heads + per - 1) / per);
     if (vec)
         hipLaunchKernelGGL(rope_scaled_kernel<4>, grid, dim3(256), 0, s, y, x, pos, n_heads, hd, ld, layout, rot,
-                           magnitude, per, turns);
+                           magnitude, units, per, turns);
     else
         hipLaunchKernelGGL(rope_scaled_kernel<1>, grid, dim3(256), 0, s, y, x, pos, n_heads, hd, ld, layout, rot,
-                           magnitude, per, turns);
+                           magnitude, units, per, turns);
     SH_CHECK_LAUNCH();
     return 0;
 }
