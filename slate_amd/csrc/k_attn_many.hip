@@ -3,7 +3,7 @@
 // chunks, mixed steps, drafted trees.  The arithmetic: attn_rows.h, how the
 // keys are shared out: attn_plan.h.
 //
-// A workgroup of W waves takes a block of 16 W query rows over a range of
+// A workgroup of eight waves takes a block of 128 query rows over a range of
 // keys: a wave 16 rows, or, where the block has fewer rows, several waves the
 // same 16 rows and a part of the keys each.  A stage of keys is brought into
 // LDS as f16 once for all waves, while the stage before is worked on and the
@@ -21,6 +21,9 @@
 
 namespace slate_hip {
 
+constexpr int AM_WGS = 256;            // one workgroup per CU
+constexpr int AM_TH = 512;
+constexpr int AM_ROWS = 8 * AR_TILE;   // query rows of a block
 constexpr int AM_KEYS = 64;            // keys of a stage
 constexpr int AM_KEEP = 512;           // blocks of up to this many keys are not cut
 
@@ -47,18 +50,15 @@ __device__ __forceinline__ int place(int key, int c) {
     return key * HD + 8 * (c ^ turn<HD>(key));
 }
 
-template <int HD, bool F32, int W>
+template <int HD, bool F32>
 struct ManyGeom {
-    static constexpr int TH = 64 * W;                  // threads
-    static constexpr int ROWS = AR_TILE * W;           // query rows of a block
-    static constexpr int WGS = 2048 / W;               // eight waves per CU
     static constexpr int PLANE = AM_KEYS * HD;         // halves
     static constexpr int PLANES = F32 ? 4 : 2;         // K hi (lo), V hi (lo)
     static constexpr int CH = HD / 8;                  // 8-element chunks of a row
     // what a thread brings in: 16 codes of a row, or 8 f32
     static constexpr int UNIT = F32 ? 8 : 16;
     static constexpr int UNITS = AM_KEYS * HD / UNIT;  // of K, and of V
-    static constexpr int EACH = (UNITS + TH - 1) / TH;   // a thread's
+    static constexpr int EACH = (UNITS + AM_TH - 1) / AM_TH;   // a thread's
 };
 
 // Blocks of a sequence and their granules (stages).
@@ -284,10 +284,10 @@ __device__ __forceinline__ float lanes_max(float v) {
     return fmaxf(v, dpp_mov<DPP_QUAD_XOR2>(v));
 }
 
-template <int HD, bool F32, int W>
-__global__ __launch_bounds__(64 * W, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
-    using Geo = ManyGeom<HD, F32, W>;
-    constexpr int TH = Geo::TH, ROWS = Geo::ROWS, WGS = Geo::WGS;
+template <int HD, bool F32>
+__global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
+    using Geo = ManyGeom<HD, F32>;
+    constexpr int TH = AM_TH, W = AM_TH / 64, ROWS = AM_ROWS, WGS = AM_WGS;
     using Steps = Q8Steps<HD>;
     constexpr int NB = HD / 32, ND = HD / 16, KEYS = AM_KEYS, PLANE = Geo::PLANE, EACH = Geo::EACH;
     constexpr int STEP = F32 ? 4 : (int)sizeof(Steps);   // bytes
@@ -424,8 +424,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_many_kernel(PackedAttn a, Pack
     };
     auto put_piece = [&](const Piece& p, int gr, int to, int ring) { put(to, ring, (gr + 1) * KEYS > open_to(p)); };
 
-    // How a block's rows go to the waves: T tiles of 16 rows, each taken by
-    // W / T waves, which share the keys 32 by 32.
+    // How a block's rows go to the waves: tiles of 16 rows, each taken by
+    // W / tiles waves, which share the keys 32 by 32.
     struct Share {
         int part, parts, r;            // the wave's part of the keys, and how many there are; its first row in the block
     };
@@ -596,27 +596,17 @@ __global__ __launch_bounds__(64 * W, 2) void attn_many_kernel(PackedAttn a, Pack
     }
 }
 
-int64_t attention_many_bytes(int hd) {
-    return max(plan_bytes(ManyGeom<128, true, 8>::WGS, ManyGeom<128, true, 8>::ROWS, hd),
-               plan_bytes(ManyGeom<128, true, 4>::WGS, ManyGeom<128, true, 4>::ROWS, hd));
-}
+int64_t attention_many_bytes(int hd) { return plan_bytes(AM_WGS, AM_ROWS, hd); }
 bool attention_many_takes(const PackedAttn& a) { return a.hd == 32 || a.hd == 64 || a.hd == 128; }
 
-template <int HD, bool F32, int W>
-static void launch_many_w(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
-    using Geo = ManyGeom<HD, F32, W>;
-    hipLaunchKernelGGL((attn_many_kernel<HD, F32, W>), dim3(Geo::WGS), dim3(Geo::TH), 0, s, a, pb);
-    if (pb.max_seq > AM_KEEP)                          // else no block is cut
-        launch_attn_join(a.out, a.ws, a.Hq, a.Hkv, HD, Geo::ROWS, Geo::WGS, s);
-}
 template <int HD>
 static void launch_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
     if (a.kf)
-        launch_many_w<HD, true, 8>(a, pb, s);
-    else if ((int64_t)pb.max_new * (a.Hq / a.Hkv) > ManyGeom<HD, false, 4>::ROWS)
-        launch_many_w<HD, false, 8>(a, pb, s);
+        hipLaunchKernelGGL((attn_many_kernel<HD, true>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
     else
-        launch_many_w<HD, false, 4>(a, pb, s);
+        hipLaunchKernelGGL((attn_many_kernel<HD, false>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
+    if (pb.max_seq > AM_KEEP)                          // else no block is cut
+        launch_attn_join(a.out, a.ws, a.Hq, a.Hkv, HD, AM_ROWS, AM_WGS, s);
 }
 
 int launch_attention_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {

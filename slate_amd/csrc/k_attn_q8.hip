@@ -1,9 +1,10 @@
 // k_attn_q8.hip -- attention over the 8-bit cache for few query rows per
 // (sequence, kv head): a decode step's tokens times the query heads of a kv
-// head, small trees.  The arithmetic: attn_q8.h, how the keys are shared out:
-// attn_plan.h.
+// head, trees of up to 96 rows.  The arithmetic: attn_q8.h, how the keys are
+// shared out: attn_plan.h.
 //
-// Each of a workgroup's four waves takes every fourth 32 keys, for all rows.
+// A workgroup takes a block of 16 rows over a range of keys, each of its four
+// waves every fourth 32 of them.
 // Memory bound: 2.125 bytes per key and element against two f16 MFMAs and about
 // 400 VALU operations per 32 keys and wave.  So the design is about loads:
 // each wave copies its next 32 keys' rows straight into LDS (16 bytes per
@@ -20,11 +21,12 @@ constexpr int AF_KEEP = 4;             // blocks of up to this many granules are
 
 __host__ __device__ inline int few_granules(int keys) { return (keys + AF_GRAN - 1) / AF_GRAN; }
 
-// Granules of a sequence: one block per kv head, if its rows fit one.
+// Granules of a sequence: blocks of 16 rows, of each kv head.
 struct FewCount {
     int G, Hkv;
+    __device__ __forceinline__ int blocks(const SeqView& s) const { return (s.n * G + AR_TILE - 1) / AR_TILE; }
     __device__ __forceinline__ int operator()(const SeqView& s) const {
-        return s.n < 1 || (int64_t)s.n * G > AR_TILE ? 0 : Hkv * few_granules(s.p0 + s.n);
+        return s.n < 1 ? 0 : Hkv * blocks(s) * few_granules(s.p0 + s.n);
     }
 };
 using FewPlan = Plan<FewCount>;
@@ -56,7 +58,8 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, j = lane & 15;
     const int G = a.Hq / a.Hkv;
-    const FewPlan plan(pb, FewCount{G, a.Hkv});
+    const FewCount count{G, a.Hkv};
+    const FewPlan plan(pb, count);
     const int x0 = few_begin(plan, blockIdx.x), x1 = few_begin(plan, blockIdx.x + 1);
     if (x0 >= x1) {
         if (threadIdx.x == 0) entry_of(a.ws, blockIdx.x)->rows = 0;
@@ -68,7 +71,7 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
     // the piece being worked on, and the loads that are under way for one
     struct Piece {
         SeqView seq;
-        int h, gran, g0, g1;
+        int h, r0, gran, g0, g1;       // kv head, first row of the block
         const int8_t *kq, *vq;
         const _Float16 *ks, *vs;
     };
@@ -77,7 +80,9 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
         Piece p;
         p.seq = pl.seq;
         p.gran = few_granules(pl.seq.p0 + pl.seq.n);
-        p.h = pl.at / p.gran;
+        const int nb = count.blocks(pl.seq), b = pl.at / p.gran;
+        p.h = b / nb;
+        p.r0 = AR_TILE * (b % nb);
         p.g0 = pl.at % p.gran;
         p.g1 = min(p.gran, p.g0 + (x1 - x));
         const int64_t row0 = pl.base / HD + p.h * (a.head_stride / HD);
@@ -110,9 +115,10 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
     // q of row j, elements 32t + 8g .. +7
     float4u qraw[NB][2];
     auto load_q = [&](const Piece& p) {
-        const bool live = j < p.seq.n * G;
+        const int r = p.r0 + j;
+        const bool live = r < p.seq.n * G;
         const float* qp =
-            a.q + ((int64_t)(p.seq.t0 + (live ? j / G : 0)) * a.Hq + p.h * G + (live ? j % G : 0)) * HD + 8 * g;
+            a.q + ((int64_t)(p.seq.t0 + (live ? r / G : 0)) * a.Hq + p.h * G + (live ? r % G : 0)) * HD + 8 * g;
 #pragma unroll
         for (int t = 0; t < NB; ++t) {
             qraw[t][0] = *(const float4u*)(qp + 32 * t);
@@ -126,18 +132,18 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
     load_q(pc);
     if (w == 0)
         leave_entry(a.ws, AF_WGS, blockIdx.x, x0, pc.g0, pc.gran, plan, [&](int v) { return few_begin(plan, v); },
-                    JoinEntry{pc.seq.t0, pc.seq.n * G, 0, pc.h, 0, 0});
+                    JoinEntry{pc.seq.t0, min(AR_TILE, pc.seq.n * G - pc.r0), pc.r0, pc.h, 0, 0});
 
     for (int x = x0;;) {
         const SeqView sv = pc.seq;
-        const int keys = sv.p0 + sv.n, h = pc.h, rows = sv.n * G;
-        const int tok = j / G;
+        const int keys = sv.p0 + sv.n, h = pc.h, r0 = pc.r0, rows = min(AR_TILE, sv.n * G - r0);
+        const int tok = (r0 + j) / G;
         const bool live = j < rows;
         Q8Rows<HD> R;
         R.start(qraw, live, scale2);
-        // the drafts that row j's token sees (n <= 16): itself and, causal,
+        // the drafts that row j's token sees (n <= 32): itself and, causal,
         // all before it, or its ancestors
-        uint32_t drafts = (2u << tok) - 1;
+        uint32_t drafts = (2u << min(tok, 31)) - 1;
         if (a.parent) {
             const int par = a.parent[sv.t0 + min(lane, sv.n - 1)];
             drafts = 0;
@@ -200,7 +206,8 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
             }
             if (whole) {
                 const float inv = 1.0f / lt;
-                *(float4u*)(a.out + ((int64_t)(sv.t0 + r / G) * a.Hq + h * G + r % G) * HD + c) = sum * inv;
+                const int row = r0 + r;
+                *(float4u*)(a.out + ((int64_t)(sv.t0 + row / G) * a.Hq + h * G + row % G) * HD + c) = sum * inv;
             } else {
                 *(floatx4*)(slot + r * HD + c) = sum;
                 if (c == 0) *(float2*)(slot + AR_TILE * HD + 2 * r) = make_float2(mt, lt);
@@ -214,8 +221,15 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
 
 // ---------------------------------------------------------------------------
 int64_t attention_q8_few_bytes(int hd) { return plan_bytes(AF_WGS, AR_TILE, hd); }
+// Blocks of 16 rows read the keys again for every block, but without a
+// barrier: 48 rows (12 drafts, 4 heads a kv head, 16 sequences of up to 4096)
+// 55 us here and 61 in the many-row kernel, 80 rows 85 and 88, 96 rows 87 and
+// 84, 128 rows 110 and 93; one sequence of 16384 39 and 46, 47 and 44, 47 and
+// 44, 52 and 49.  A row's drafts are kept in 32 bits.
+constexpr int AF_MAX_ROWS = 96, AF_MAX_NEW = 32;
 bool attention_q8_few_takes(const PackedAttn& a, const PackedBatch& pb) {
-    return !a.kf && (a.hd == 32 || a.hd == 64 || a.hd == 128) && (int64_t)pb.max_new * (a.Hq / a.Hkv) <= AR_TILE;
+    return !a.kf && (a.hd == 32 || a.hd == 64 || a.hd == 128) && pb.max_new <= AF_MAX_NEW &&
+           pb.max_new * (int64_t)(a.Hq / a.Hkv) <= AF_MAX_ROWS;
 }
 
 template <int HD>

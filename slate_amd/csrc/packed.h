@@ -72,7 +72,7 @@ struct PackedAttn {
     void* ws;
 };
 int64_t attention_packed_bytes(int Hq, int Hkv, int hd);
-// k_attn_q8.hip: 8-bit pools, at most 16 query rows per (sequence, kv head).
+// k_attn_q8.hip: 8-bit pools, few query rows per (sequence, kv head).
 bool attention_q8_few_takes(const PackedAttn& a, const PackedBatch& pb);
 int64_t attention_q8_few_bytes(int hd);
 int launch_attention_q8_few(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
