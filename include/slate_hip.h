@@ -258,7 +258,8 @@ int   slate_hip_rope_frequencies(double* w, double* magnitude, const slate_hip_r
  * f32 (16-byte aligned), rows ld floats apart (ld % 4 == 0).  Per 32 elements
  * step = f16(max|x| / 127) (at most 65504) and code = x / step to the nearest
  * whole number, ties to even, within -127 .. 127; a block whose step rounds
- * to 0 gets codes 0.  NaN counts as 0. */
+ * to 0 gets codes 0.  NaN counts as 0.  Rows that two sequences of one call
+ * both write (they share cache rows) end up undefined. */
 int   slate_hip_kv_store_q8(int8_t* Kq, uint16_t* Ks, int8_t* Vq, uint16_t* Vs, const float* k, const float* v,
                             int64_t ld, const int32_t* tok_off, const int32_t* pos0, const int64_t* kv_base, int B,
                             int T, int n_kv_heads, int head_dim, int64_t head_stride, int max_seq);
@@ -272,12 +273,14 @@ int   slate_hip_kv_load_q8(float* k, float* v, int64_t ld, const int8_t* Kq, con
  * n_kv_heads; query head g belongs to kv head g / (n_q_heads / n_kv_heads).
  * Scores are q.k / sqrt(head_dim), as attention_ragged's.  max_new bounds the
  * tokens that one sequence brings (1 for a decode step); head_dim is at most
- * 512.  Queries must be finite and below 2^100 in size.  What the cache holds
- * in rows a token does not see never matters.
- * ws: device scratch of slate_hip_attention_packed_bytes, 16-byte aligned, for calls that run beside
- * each other or are captured into graphs that do; NULL takes the backend's
- * own, which calls on the backend stream share (a call under stream capture
- * is then refused with -5). */
+ * 512; 32, 64 and 128 run on the matrix instructions, the others on a plain
+ * kernel.  Queries must be finite and, like the cache's values, below 2^100
+ * in size.  What the cache holds in rows a token does not see never matters.
+ * ws: device scratch of slate_hip_attention_packed_bytes, 16-byte aligned,
+ * its content of no matter, for calls that run beside each other or are
+ * captured into graphs that do; NULL takes the backend's own, which calls on
+ * the backend stream share (a call under stream capture is then refused with
+ * -5). */
 int   slate_hip_attention_ragged_q8(float* out, const float* q, const int8_t* Kq, const uint16_t* Ks,
                                     const int8_t* Vq, const uint16_t* Vs, const int32_t* tok_off,
                                     const int32_t* pos0, const int64_t* kv_base, int B, int T, int max_new,

@@ -4,8 +4,11 @@
 //   step = f16(max |x| / 127),  code = x / step to the nearest, ties to even
 //
 // Eight lanes share a block of 32 elements, four of them each: the maximum
-// stays inside a DPP row, loads and stores are whole lines.  A workgroup
-// takes one token's K or V row (grid.y).
+// stays inside a DPP row, loads and stores are whole lines.  Memory bound: K
+// and V rows of about 5000 tokens (8 heads of 128) are stored in 16 us (52 MB
+// read and written, 3.3 TB/s; a store per token and exact divisions took 21)
+// and loaded in 13.5 us (3.9 TB/s); rows of 16 tokens in 3 us each, launch and
+// two rounds of load latency.
 #include "lanes.h"
 #include "packed.h"
 

@@ -17,7 +17,10 @@ namespace slate_hip {
 // of the head is copied (y != x) and comes in groups of eight too, the
 // threads after the pairs' copy those the same way.  A workgroup takes one
 // row, or a part of its heads where rows are few.
-// Memory bound: 4096 rows of 72 heads of 128 (302 MB) in ROPE_CHUNK_US us.
+// Memory bound: 4096 rows of 72 heads of 128 (302 MB) take 60.3 us, 5.0 TB/s
+// (a 4 GiB copy reaches 4.7); one pass over heads at a time and scalar copies
+// of the rest took 66.9.  16 rows of 40 heads: 3 us, the launch and two rounds
+// of load latency.
 template <int VEC>
 __global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float* x, const int32_t* __restrict__ pos,
                                                           int n_heads, int hd, int64_t ld, int layout, int rot,
@@ -101,7 +104,7 @@ int launch_rope_scaled(float* y, const float* x, const int32_t* pos, int n_rows,
     const int units = !vec ? rot / 2 : y != x && hd <= 2048 ? hd / 8 : rot / 8;
     const int step = 256 / units;
     // few rows: a workgroup takes as many heads as it has threads for
-    const int per = n_rows < 512 ? step : n_heads;
+    const int per = n_rows < 512 ? max(step, n_heads / 32768) : n_heads;
     const dim3 grid(n_rows, (n_heads + per - 1) / per);
     if (vec)
         hipLaunchKernelGGL(rope_scaled_kernel<4>, grid, dim3(256), 0, s, y, x, pos, n_heads, hd, ld, layout, rot,

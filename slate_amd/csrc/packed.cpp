@@ -87,7 +87,7 @@ int attention_packed(const char* what, const PackedAttn& a, const PackedBatch& p
                "%s: pools are not 16-byte aligned", what);
     // the kernels count key granules of at least 32 per block of at least 16 query rows in 32 bits
     const double granules = (double)a.Hkv * ((double)pb.T * (a.Hq / a.Hkv) / 16 + pb.B) * (pb.max_seq / 32 + 1.0);
-    SH_REQUIRE(granules < 2147483648.0, "%s: %d tokens over max_seq=%d are too much for one call", what, pb.T,
+    SH_REQUIRE(granules < 2147483648.0 && (int64_t)pb.T * a.Hq <= INT32_MAX, "%s: %d tokens over max_seq=%d are too much for one call", what, pb.T,
                pb.max_seq);
     const size_t bytes = (size_t)pb.T * a.Hq * a.hd * sizeof(float);
     SH_REQUIRE(!overlap(a.out, bytes, a.q, bytes), "%s: out overlaps q", what);

@@ -53,6 +53,8 @@ ROPES = [
     (600, 2, 64, 0, 4096, dict(layout=0, rot_dim=64, magnitude=0.5)),
     (5, 9, 33, 0, 100, dict(layout=0, rot_dim=2)),
     (515, 11, 96, 5, 1 << 17, dict(layout=1, rot_dim=96)),
+    (3, 40000, 16, 0, 3000, dict(layout=0, rot_dim=16)),
+    (4, 7, 2056, 0, 900, dict(layout=1, rot_dim=512)),
 ]
 
 
@@ -291,6 +293,81 @@ def test_ragged_q8_bound_on_tokens(hip):
     r.check()
 
 
+def test_empty_batch(hip):
+    """Sequences without tokens, or with numbers that do not fit: nothing is written, cut entries of an earlier call
+    are not taken for this one's."""
+    rng = np.random.default_rng(2)
+    bt = Batch([(9000, 1), (3000, 1)], 1, 64, 9002, rng)
+    r = Run(bt, 4, True, 5)
+    r.call(own_ws=True)
+    r.check()
+    for off, pos in (([0, 0, 0], [5, 5]), ([0, 1, 0], [9002, 0]), ([0, -1, -1], [0, 0]), ([2, 3, 4], [0, 0]),
+                     ([0, 1, 2], [-1, 1 << 30])):
+        bt.d_off.upload(np.array(off, np.int32))
+        bt.d_pos.upload(np.array(pos, np.int32))
+        r.out.upload(np.full_like(r.q, SENTINEL))
+        r.call(own_ws=True)
+        assert np.all(r.result() == SENTINEL), (off, pos)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_workspace_content_does_not_matter(hip, q8):
+    """A workspace full of NaN and of large numbers, as another call may leave it."""
+    rng = np.random.default_rng(3)
+    for n in (5, 40):
+        bt = Batch([(5000, n), (700, 3), (0, 1)], 1, 128, 5100, rng)
+        r = Run(bt, 4, q8, 31, random_parents(bt, rng, "random"))
+        for fill in (np.float32(np.nan), np.float32(3e38)):
+            r.ws.upload(np.full(r.need // 4, fill, np.float32))
+            r.call(own_ws=True)
+            r.check()
+
+
+def test_more_sequences_than_fit_a_wave(hip):
+    rng = np.random.default_rng(4)
+    seqs = [(int(rng.integers(0, 90)), int(rng.integers(0, 2))) for _ in range(1023)] + [(2000, 1)]
+    bt = Batch(seqs, 1, 32, 2001, rng)
+    r = Run(bt, 2, True, 4)
+    r.call()
+    r.check()
+
+
+def test_sequences_that_share_cached_rows(hip):
+    """Two sequences over one slot, as beams over a shared prompt read it."""
+    rng = np.random.default_rng(14)
+    bt = Batch([(800, 1), (800, 1), (300, 1)], 2, 64, 801, rng)
+    bt.first[1] = bt.first[0]
+    bt.d_base.upload(bt.first)
+    r = Run(bt, 4, True, 6)
+    r.call()
+    r.check()
+
+
+def test_base_is_rounded_down_to_a_row(hip):
+    rng = np.random.default_rng(15)
+    bt = Batch([(40, 2), (100, 1)], 1, 64, 128, rng)
+    r = Run(bt, 4, True, 6)
+    bt.d_base.upload(bt.first + np.array([63, 17]))
+    r.call()
+    r.check()
+    bt.d_base.upload(np.array([-1, bt.first[1]]))
+    bt.bad = {0}
+    r.out.upload(np.full_like(r.q, SENTINEL))
+    r.call()
+    r.check()
+
+
+@pytest.mark.parametrize("G,n", [(1, 32), (1, 33), (3, 32), (4, 24), (4, 25), (16, 6), (16, 7), (96, 1), (97, 1)])
+def test_rows_around_the_kernels_border(hip, G, n):
+    """96 query rows per kv head and 32 tokens are where one kernel hands over to the other."""
+    rng = np.random.default_rng(16)
+    bt = Batch([(700, n), (31, max(1, n - 1)), (5, 1)], 1, 64, 800, rng)
+    for kind in ("causal", "tree"):
+        r = Run(bt, G, True, 6, random_parents(bt, rng, "random") if kind == "tree" else None)
+        r.call()
+        r.check()
+
+
 def random_parents(bt, rng, kind):
     out = np.full(bt.T, -1, np.int32)
     for b in range(bt.B):
@@ -446,6 +523,23 @@ def test_kv_store_and_load(hip, hd, Hkv, extra):
         assert np.array_equal(back, want)
 
 
+def test_kv_many_tokens(hip):
+    """More tokens than one per workgroup, more sequences than lanes, rows left out among them."""
+    rng = np.random.default_rng(7)
+    for B, most in ((9, 400), (80, 40)):
+        seqs = [(int(rng.integers(0, 30)), int(rng.integers(0, most))) for _ in range(B)]
+        bt = Batch(seqs, 2, 64, 460, rng, behind=5, bad=(2,))
+        k, v = (rng.normal(0, 1, (bt.T, 128)).astype(np.float32) for _ in "KV")
+        assert bt.T >= 1024
+        _, back = store_load(bt, k, v, 128)
+        for x, y in ((k, back[0]), (v, back[1])):
+            want = pr.values(*pr.quantise(x)).astype(np.float32)
+            owned = np.zeros(bt.T, bool)
+            for b in range(B):
+                owned[list(bt.tokens(b))] = True
+            assert np.array_equal(y[owned], want[owned]) and np.all(y[~owned] == SENTINEL)
+
+
 def test_kv_codes_at_every_tie(hip):
     """Elements at and next to each tie of the rounding, for many steps: the nearest code, ties to even."""
     rng = np.random.default_rng(2)
@@ -521,13 +615,13 @@ class _Graph:
 
 
 def test_captured_calls(hip):
-    """Two captured attention calls with a workspace each, replayed between eager calls, on new queries; one
+    """Captured attention calls with a workspace each, replayed between eager calls, on new queries; one
     without a workspace is refused and leaves the stream usable."""
     rng = np.random.default_rng(6)
     runs = []
-    for k in range(2):
-        bt = Batch([(2000 + 700 * k, 9), (50, 5)], 1, 128, 4000, rng)
-        runs.append(Run(bt, 4, True, 40 + k, random_parents(bt, rng, "random")))
+    for k, (q8, n) in enumerate(((True, 9), (True, 40), (False, 9))):
+        bt = Batch([(2000 + 700 * k, n), (50, 5)], 1, 128, 4000, rng)
+        runs.append(Run(bt, 4, q8, 40 + k, random_parents(bt, rng, "random")))
     for r in runs:
         r.call(own_ws=True)
     refused = _Graph(lambda: runs[0].call())

@@ -133,7 +133,8 @@ KINDS = ("ragged_q8", "tree", "tree_q8")
 BAD_ATTN = [dict(out=None), dict(q=None), dict(tok_off=None), dict(pos0=None), dict(kv_base=None), dict(B=0),
             dict(B=1025), dict(T=0), dict(max_new=0), dict(max_seq=0), dict(Hq=9), dict(Hkv=0), dict(Hq=1),
             dict(hd=24), dict(hd=528), dict(stride=-128), dict(q=A), dict(q=A + 4 * (5 * 8 * 128 - 1)),
-            dict(ws=A + 8, ws_bytes=1 << 40), dict(B=1000, T=100000, max_seq=1 << 30)]
+            dict(ws=A + 8, ws_bytes=1 << 40), dict(B=1000, T=100000, max_seq=1 << 30),
+            dict(T=1 << 28, Hq=16, q=A + (1 << 45))]
 BAD_Q8 = [{n: None} for n in ("Kq", "Ks", "Vq", "Vs")] + [{n: A + 8} for n in ("Kq", "Ks", "Vq", "Vs")] + \
          [dict(stride=100), dict(hd=48, stride=48)]
 
