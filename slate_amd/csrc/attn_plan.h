@@ -56,6 +56,15 @@ class Plan {
         total = __builtin_amdgcn_readlane(first_.upto, 63);
         for (int b0 = 64; b0 < pb.B; b0 += 64) total += __builtin_amdgcn_readlane(load(b0).upto, 63);
     }
+    // The plan's first 64 sequences can wait in LDS instead of in registers.
+    struct Lane {
+        SeqView seq;
+        int64_t base;
+        int own, upto;                 // granules of the lane's sequence, and with those of the lanes before it
+    };
+    __device__ __forceinline__ Plan(const PackedBatch& pb, const Count& count, int total_, const Lane& first)
+        : total(total_), pb_(pb), count_(count), first_(first) {}
+    __device__ __forceinline__ const Lane& first() const { return first_; }
     // 0 <= x < total
     __device__ __forceinline__ Place find(int x) const {
         Lane s = first_;
@@ -87,11 +96,6 @@ class Plan {
     }
 
   private:
-    struct Lane {
-        SeqView seq;
-        int64_t base;
-        int own, upto;                 // granules of the lane's sequence, and with those of the lanes before it
-    };
     __device__ __forceinline__ Lane load(int b0) const {
         const int b = b0 + (int)(threadIdx.x & 63);
         Lane s{};

@@ -71,14 +71,20 @@ struct ManyCount {
         return s.p0 + (causal ? (min(s.n * G, (i + 1) * rows) - 1) / G + 1 : s.n);
     }
     __device__ __forceinline__ int granules(const SeqView& s, int i) const { return (seen(s, i) + AM_KEYS - 1) / AM_KEYS; }
-    __device__ __forceinline__ int per_head(const SeqView& s) const {
+    // granules of a sequence, counted by the one lane that holds it: the keys
+    // that a block sees step by rows / G and carry the rest
+    __device__ __forceinline__ int operator()(const SeqView& s) const {
+        if (s.n < 1) return 0;
         const int nb = blocks(s);
-        if (!causal || nb <= 1) return nb * granules(s, 0);
-        int sum = 0;
-        for (int i = 0; i < nb; ++i) sum += granules(s, i);
-        return sum;
+        if (!causal) return Hkv * nb * granules(s, 0);
+        const int step = rows / G, rest = rows - step * G;
+        int sum = granules(s, nb - 1);
+        for (int i = 1, r = rest - 1, t = s.p0 + step; i < nb; ++i, t += step, r += rest) {
+            if (r >= G) r -= G, ++t;                   // (i rows - 1) / G = t - p0 + floor(r / G), r < 2 G
+            sum += (t + (r >= 0) + AM_KEYS - 1) / AM_KEYS;
+        }
+        return Hkv * sum;
     }
-    __device__ __forceinline__ int operator()(const SeqView& s) const { return s.n < 1 ? 0 : Hkv * per_head(s); }
 };
 using ManyPlan = Plan<ManyCount>;
 
@@ -99,12 +105,17 @@ __device__ __forceinline__ ManyPlace many_find(const ManyPlan& plan, const ManyC
         r.in = pl.at % r.gran;
         return r;
     }
-    const int per = c.per_head(pl.seq);
+    const int lane = threadIdx.x & 63;
+    auto scan_from = [&](int i0, int& own) {           // blocks i0 .., a lane each
+        own = i0 + lane < nb ? c.granules(pl.seq, i0 + lane) : 0;
+        return wave_scan(own);
+    };
+    int own, per = 0;                                  // granules of a kv head
+    for (int i0 = 0; i0 < nb; i0 += 64) per += __builtin_amdgcn_readlane(scan_from(i0, own), 63);
     r.h = pl.at / per;
     r.in = pl.at % per;
-    for (int i0 = 0;; i0 += 64) {                      // 64 blocks at a time
-        const int i = i0 + (int)(threadIdx.x & 63);
-        const int own = i < nb ? c.granules(pl.seq, i) : 0, upto = wave_scan(own);
+    for (int i0 = 0;; i0 += 64) {
+        const int upto = scan_from(i0, own);
         const uint64_t past = __builtin_amdgcn_ballot_w64(upto > r.in);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -159,41 +170,71 @@ struct ManyRows : AttnRows<HD> {
         const float *kf = (const float*)steps + at, *vf = kf + AM_KEYS;
         floatx4 s[H];
         const floatx4 zero = zeros();
-        if (!MASKED && H == 4) __builtin_amdgcn_iglp_opt(1);   // LDS reads between the MFMAs: 2-3 %
+        // Operands come out of LDS one group of MFMAs ahead; the fences keep
+        // the order (the scheduler undoes it where registers get scarce).
+        // A group of K: 16 keys, for f32 at most 64 elements of them.
+        constexpr int KT = F32 && NB > 2 ? 2 : NB, KG = NB / KT, LO = F32 ? KT : 0;
+        half8_t kr[2][KT + LO];
+        auto read_k = [&](int q) {
+            const _Float16* kh = k + 16 * (q / KG) * HD;
 #pragma unroll
-        for (int hf = 0; hf < H; ++hf) {
-            const _Float16* kh = k + 16 * hf * HD;
-            if constexpr (F32) {
-#pragma unroll
-                for (int t = 0; t < NB; ++t) {
-                    const half8_t hi = *(const half8_t*)(kh + koff[t]), lo = *(const half8_t*)(kh + PLANE + koff[t]);
-                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[t], t == 0 ? zero : s[hf], 0, 0, 0);
-                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[t], s[hf], 0, 0, 0);
-                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[t], s[hf], 0, 0, 0);
-                }
-                s[hf] *= *(const floatx4*)(kf + 16 * hf + 4 * g);
-            } else {
-                Steps d[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d[i] = ks[16 * hf + 4 * g + i];
-#pragma unroll
-                for (int t = 0; t < NB; ++t) {
-                    const half8_t kc = *(const half8_t*)(kh + koff[t]);
-                    floatx4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[t], zero, 0, 0, 0);
-                    r = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qh[t], r, 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[hf][e] = t == 0 ? times(r[e], d[e].s[t]) : fmaf((float)d[e].s[t], r[e], s[hf][e]);
-                }
+            for (int t = 0; t < KT; ++t) {
+                kr[q & 1][t] = *(const half8_t*)(kh + koff[q % KG * KT + t]);
+                if constexpr (F32) kr[q & 1][LO + t] = *(const half8_t*)(kh + PLANE + koff[q % KG * KT + t]);
             }
-        }
-        // bit 16 (e / 4) + e % 4 of `bits`: the row sees the lane's key e
-        const uint32_t bits = MASKED ? seen >> (4 * g) : 0;
-        auto sees = [&](int e) { return !MASKED || (bits >> (16 * (e >> 2) + (e & 3)) & 1) != 0; };
+        };
         auto columns = [&](const _Float16* plane, int n) {
             const half4_t a = read_columns16(plane + voff[n]), b = read_columns16(plane + 16 * HD + voff[n]);
             return half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         };
+        // A group of V: 32 keys, 16 or 32 elements.
+        constexpr int VU = F32 ? 1 : 2, VG = ND / VU, GROUPS = H / 2 * VG;
+        half8_t vr[2][2];
+        auto read_v = [&](int q) {
+            const _Float16* vb = v + 32 * (q / VG) * HD;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                vr[q & 1][u] = columns(F32 ? vb + u * PLANE : vb, F32 ? q % VG : VU * (q % VG) + u);
+        };
+        read_k(0);
+#pragma unroll
+        for (int q = 0; q < H * KG; ++q) {
+            const int hf = q / KG, t0 = q % KG * KT;
+            if (q + 1 < H * KG)
+                read_k(q + 1);
+            else
+                read_v(0);
+            __builtin_amdgcn_sched_barrier(0);
+            const half8_t* kc = kr[q & 1];
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[LO + t], qh[t0 + t], t0 + t == 0 ? zero : s[hf], 0,
+                                                                   0, 0);
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[t], ql[t0 + t], s[hf], 0, 0, 0);
+                    s[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[t], qh[t0 + t], s[hf], 0, 0, 0);
+                }
+                if (q % KG == KG - 1) s[hf] *= *(const floatx4*)(kf + 16 * hf + 4 * g);
+            } else {
+                Steps d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = ks[16 * hf + 4 * g + i];
+                floatx4 r[NB];
+#pragma unroll
+                for (int t = 0; t < NB; ++t) r[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[t], ql[t], zero, 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < NB; ++t) r[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[t], qh[t], r[t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < NB; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[hf][e] = t == 0 ? times(r[0][e], d[e].s[0]) : fmaf((float)d[e].s[t], r[t][e], s[hf][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // bit 16 (e / 4) + e % 4 of `bits`: the row sees the lane's key e
+        const uint32_t bits = MASKED ? seen >> (4 * g) : 0;
+        auto sees = [&](int e) { return !MASKED || (bits >> (16 * (e >> 2) + (e & 3)) & 1) != 0; };
         float p[4 * H], x[8];
         half8_t ph, pl;
         if constexpr (F32) {
@@ -209,16 +250,18 @@ struct ManyRows : AttnRows<HD> {
             this->template weights<H, true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
 #pragma unroll
             for (int b = 0; b < H / 2; ++b) {
-                const _Float16* vb = v + 32 * b * HD;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = p[8 * b + e] * (sees(e) ? d[2 * b + (e >> 2)][e & 3] : 0.f);
                 halves(x, ph, pl);
 #pragma unroll
                 for (int n = 0; n < ND; ++n) {
-                    const half8_t vh = columns(vb, n), vl = columns(vb + PLANE, n);
-                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[n], 0, 0, 0);
-                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[n], 0, 0, 0);
-                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[n], 0, 0, 0);
+                    const int q = b * ND + n;
+                    if (q + 1 < GROUPS) read_v(q + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][1], ph, o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][0], pl, o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][0], ph, o[n], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (MASKED)
@@ -251,12 +294,14 @@ struct ManyRows : AttnRows<HD> {
             this->template weights<H, true>(s, big, step_exponent, p);
 #pragma unroll
             for (int b = 0; b < H / 2; ++b) {
-                const _Float16* vb = v + 32 * b * HD;
                 Steps dv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dv[e] = vs[32 * b + 16 * (e >> 2) + 4 * g + (e & 3)];
 #pragma unroll
                 for (int t = 0; t < NB; ++t) {
+                    const int q = b * NB + t;
+                    if (q + 1 < GROUPS) read_v(q + 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         x[e] = times(p[8 * b + e], dv[e].s[t]);
@@ -264,12 +309,11 @@ struct ManyRows : AttnRows<HD> {
                     }
                     halves(x, ph, pl);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int n = 2 * t + u;
-                        const half8_t vc = columns(vb, n);
-                        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, pl, o[n], 0, 0, 0);
-                        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, ph, o[n], 0, 0, 0);
-                    }
+                    for (int u = 0; u < 2; ++u)
+                        o[2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][u], pl, o[2 * t + u], 0, 0, 0);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        o[2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][u], ph, o[2 * t + u], 0, 0, 0);
                 }
             }
         }
@@ -285,7 +329,7 @@ __device__ __forceinline__ float lanes_max(float v) {
     return fmaxf(v, dpp_mov<DPP_QUAD_XOR2>(v));
 }
 
-template <int HD, bool F32>
+template <int HD, bool F32, bool TREE>
 __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
     using Geo = ManyGeom<HD, F32>;
     constexpr int TH = AM_TH, W = AM_TH / 64, ROWS = AM_ROWS, WGS = AM_WGS;
@@ -296,6 +340,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     __shared__ __attribute__((aligned(16))) unsigned char s_step[2][2 * KEYS * STEP];
     __shared__ uint32_t s_seen[PK_MAX_DRAFT / 32][ROWS];   // the drafts that a block's token sees
     __shared__ int16_t s_par[PK_MAX_DRAFT];
+    __shared__ ManyPlan::Lane s_plan[64];
     __shared__ uint32_t s_bad[4][2];                  // f32: keys whose V row has an element that is not finite
     __shared__ int s_top[2][2];                       // 8-bit: the largest V step of each 32 keys
     // what the waves that share rows leave for each other: where the stage
@@ -310,7 +355,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     const int G = a.Hq / a.Hkv;
     // neighbouring ranges on one XCD: blocks that share keys find them in its L2
     const int wg = (blockIdx.x % 8) * (WGS / 8) + blockIdx.x / 8;
-    const ManyCount count{G, a.Hkv, ROWS, a.parent == nullptr};
+    const ManyCount count{G, a.Hkv, ROWS, !TREE};
     const ManyPlan plan(pb, count);
     auto begin = [&](int v) { return many_begin(plan, count, v, WGS); };
     const int x0 = begin(wg), x1 = begin(wg + 1);
@@ -322,15 +367,23 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     if (tid < 8) s_bad[tid >> 1][tid & 1] = 0;
 
     struct Piece {
+        int x;                         // its place on the line; >= x1: none
         SeqView seq;
         int h, block, gran, g0, g1, last;
+        int open;                      // keys below it are seen by all rows of the block
         int64_t at;                    // first element of the head's rows
     };
-    auto piece_at = [&](int x) {
+    auto piece_in = [&](const ManyPlan& plan, int x) {
         const ManyPlace pl = many_find(plan, count, x);
         const int64_t base = F32 ? pl.base : pl.base / HD * HD;
-        return Piece{pl.seq, pl.h, pl.block, pl.gran, pl.in, min(pl.gran, pl.in + (x1 - x)),
-                     count.seen(pl.seq, pl.block) - 1, base + pl.h * a.head_stride};
+        return Piece{x, pl.seq, pl.h, pl.block, pl.gran, pl.in, min(pl.gran, pl.in + (x1 - x)),
+                     count.seen(pl.seq, pl.block) - 1,
+                     TREE ? pl.seq.p0 : pl.seq.p0 + pl.block * ROWS / G + 1, base + pl.h * a.head_stride};
+    };
+    const int total = plan.total;
+    auto piece_after = [&](const Piece& p) {
+        const int x = p.x + p.g1 - p.g0;
+        return x < x1 ? piece_in(ManyPlan(pb, count, total, s_plan[lane]), x) : Piece{x1};
     };
     // a stage's rows on their way: the thread's unit of K and of V, and steps
     // (rows past the last key repeat it: nobody sees them)
@@ -419,11 +472,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             }
         }
     };
-    // keys below it are seen by all rows of the piece's block
-    auto open_to = [&](const Piece& p) {
-        return a.parent ? p.seq.p0 : p.seq.p0 + p.block * ROWS / G + 1;
-    };
-    auto put_piece = [&](const Piece& p, int gr, int to, int ring) { put(to, ring, (gr + 1) * KEYS > open_to(p)); };
+    auto put_piece = [&](const Piece& p, int gr, int to, int ring) { put(to, ring, (gr + 1) * KEYS > p.open); };
 
     // How a block's rows go to the waves: tiles of 16 rows, each taken by
     // W / tiles waves, which share the keys 32 by 32.
@@ -435,30 +484,34 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
         const int tiles = rows <= AR_TILE ? 1 : rows <= 2 * AR_TILE ? 2 : rows <= 4 * AR_TILE ? 4 : W;
         return Share{w / tiles, W / tiles, AR_TILE * (w % tiles)};
     };
-    Piece pc = piece_at(x0), nx = pc;                  // worked on; being loaded
-    int ngr = pc.g0, nx_x = x0;                        // the stage being loaded, its piece's place on the line
-    load(nx, ngr);
+    // The piece worked on and the two after it: the stage being loaded is two
+    // ahead, so in one of them, and no search stands in the loop over stages.
+    Piece pc = piece_in(plan, x0);
+    load(pc, pc.g0);
     if (w == 0)
         leave_entry(a.ws, WGS, wg, x0, pc.g0, pc.gran, plan, begin,
                     JoinEntry{pc.seq.t0, min(ROWS, pc.seq.n * G - pc.block * ROWS), pc.block * ROWS, pc.h, 0,
                               0});
+    if (w == 0) s_plan[lane] = plan.first();
+    __syncthreads();                                   // (s_bad is clear, too)
+    Piece p1 = piece_after(pc), p2 = piece_after(p1);
+    Piece nx = pc;                                     // the piece of the stage being loaded
+    int ngr = pc.g0, ahead = 0;                        // that stage; the piece is pc, p1 or p2
     // the next stage after the one being loaded; false at the range's end
     auto advance = [&]() {
         if (ngr + 1 < nx.g1) {
             ++ngr;
             return true;
         }
-        const int xn = nx_x + nx.g1 - nx.g0;
-        if (xn >= x1) return false;
-        nx_x = xn;
-        nx = piece_at(xn);
+        nx = ahead == 0 ? p1 : p2;
+        ++ahead;
         ngr = nx.g0;
-        return true;
+        return nx.x < x1;
     };
     bool coming = true;
     int to = 0, ring = 0;
 
-    for (int x = x0;;) {
+    for (;;) {
         const SeqView sv = pc.seq;
         const int h = pc.h, r0 = pc.block * ROWS, rows = min(ROWS, sv.n * G - r0);
         const Share sh = share_of(pc);
@@ -476,17 +529,16 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             qraw[t][0] = *(const float4u*)(qp + 32 * t);
             qraw[t][1] = *(const float4u*)(qp + 32 * t + 4);
         }
-        if (x == x0) {                                 // the first stage, once q is on its way too
-            __syncthreads();                           // s_bad is clear
+        if (pc.x == x0) {                               // the first stage, once q is on its way too
             put_piece(nx, ngr, 0, 0);
             if ((coming = advance())) load(nx, ngr);
         }
         R.start(qraw, live, scale2);
         // keys below `open` are seen by all of the wave's rows, from `end` on by none
-        const int open = a.parent ? sv.p0 : sv.p0 + (r0 + min(rw, rows - 1)) / G + 1;
-        const int end = rw >= rows ? 0 : a.parent ? sv.p0 + sv.n : sv.p0 + (r0 + min(rw + AR_TILE, rows) - 1) / G + 1;
+        const int open = TREE ? sv.p0 : sv.p0 + (r0 + min(rw, rows - 1)) / G + 1;
+        const int end = rw >= rows ? 0 : TREE ? sv.p0 + sv.n : sv.p0 + (r0 + min(rw + AR_TILE, rows) - 1) / G + 1;
         const int words = (sv.n + 31) / 32;
-        if (a.parent && pc.g1 * KEYS > sv.p0) {        // the block's tokens' ancestors
+        if (TREE && pc.g1 * KEYS > sv.p0) {        // the block's tokens' ancestors
             __syncthreads();
             for (int i = tid; i < sv.n; i += TH) {
                 const int up = a.parent[sv.t0 + i];
@@ -534,7 +586,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
                     continue;
                 }
                 uint32_t seen = 0;
-                if (live && !a.parent) {
+                if (live && !TREE) {
                     const int n = min(32, max(0, sv.p0 + tok + 1 - k0 - at));
                     seen = n == 32 ? 0xffffffffu : (1u << n) - 1;
                 } else if (live) {
@@ -549,7 +601,6 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             if (had && !early) bring();
         }
         const bool whole = pc.g0 == 0 && pc.g1 == pc.gran;
-        const int xn = x + pc.g1 - pc.g0;
         const float back = R.back();
         float l = R.sum();
 #pragma unroll
@@ -588,16 +639,18 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
 #pragma unroll
                 for (int n = 0; n < ND; ++n) *(float4u*)(op + 16 * n) = R.o[n] * inv;
             } else {
-                float* slot = slot_of(a.ws, WGS, 2 * wg + (x == x0 ? 0 : 1), ROWS, HD);
+                float* slot = slot_of(a.ws, WGS, 2 * wg + (pc.x == x0 ? 0 : 1), ROWS, HD);
                 const int r = rw + j;
                 if (g == 0) *(float2*)(slot + ROWS * HD + 2 * r) = make_float2(R.m, l);
 #pragma unroll
                 for (int n = 0; n < ND; ++n) *(floatx4*)(slot + r * HD + 16 * n + 4 * g) = R.o[n];
             }
         }
-        if (xn >= x1) break;
-        x = xn;
-        pc = piece_at(x);
+        if (p1.x >= x1) break;
+        pc = p1;
+        p1 = p2;
+        p2 = piece_after(p2);
+        --ahead;
     }
 }
 
@@ -606,10 +659,9 @@ bool attention_many_takes(const PackedAttn& a) { return a.hd == 32 || a.hd == 64
 
 template <int HD>
 static void launch_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
-    if (a.kf)
-        hipLaunchKernelGGL((attn_many_kernel<HD, true>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
-    else
-        hipLaunchKernelGGL((attn_many_kernel<HD, false>), dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
+    auto kernel = a.kf ? attn_many_kernel<HD, true, true>
+                       : a.parent ? attn_many_kernel<HD, false, true> : attn_many_kernel<HD, false, false>;
+    hipLaunchKernelGGL(kernel, dim3(AM_WGS), dim3(AM_TH), 0, s, a, pb);
     if (pb.max_seq > AM_KEEP)                          // else no block is cut
         launch_attn_join(a.out, a.ws, a.Hq, a.Hkv, HD, AM_ROWS, AM_WGS, s);
 }
