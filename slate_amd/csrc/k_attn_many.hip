@@ -196,6 +196,17 @@ struct ManyRows : AttnRows<HD> {
             for (int u = 0; u < 2; ++u)
                 vr[q & 1][u] = columns(F32 ? vb + u * PLANE : vb, F32 ? q % VG : VU * (q % VG) + u);
         };
+        // 8-bit: a group's products, by the keys' steps
+        floatx4 kp[2][NB];
+        Steps kd[2][4];
+        auto by_steps = [&](int hf) {
+#pragma unroll
+            for (int t = 0; t < NB; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[hf][e] = t == 0 ? times(kp[hf & 1][0][e], kd[hf & 1][e].s[0])
+                                      : fmaf((float)kd[hf & 1][e].s[t], kp[hf & 1][t][e], s[hf][e]);
+        };
         read_k(0);
 #pragma unroll
         for (int q = 0; q < H * KG; ++q) {
@@ -216,22 +227,25 @@ struct ManyRows : AttnRows<HD> {
                 }
                 if (q % KG == KG - 1) s[hf] *= *(const floatx4*)(kf + 16 * hf + 4 * g);
             } else {
-                Steps d[4];
+                floatx4* r = kp[q & 1];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[i] = ks[16 * hf + 4 * g + i];
-                floatx4 r[NB];
+                for (int i = 0; i < 4; ++i) kd[q & 1][i] = ks[16 * hf + 4 * g + i];
 #pragma unroll
                 for (int t = 0; t < NB; ++t) r[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[t], ql[t], zero, 0, 0, 0);
 #pragma unroll
                 for (int t = 0; t < NB; ++t) r[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[t], qh[t], r[t], 0, 0, 0);
+                if (hf > 0) {
+                    by_steps(hf - 1);
 #pragma unroll
-                for (int t = 0; t < NB; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[hf][e] = t == 0 ? times(r[0][e], d[e].s[0]) : fmaf((float)d[e].s[t], r[t][e], s[hf][e]);
+                    for (int i = 0; i < 2 * NB; ++i) {  // a MFMA, then what the group before left to the vector unit
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+                    }
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (!F32) by_steps(H - 1);
         // bit 16 (e / 4) + e % 4 of `bits`: the row sees the lane's key e
         const uint32_t bits = MASKED ? seen >> (4 * g) : 0;
         auto sees = [&](int e) { return !MASKED || (bits >> (16 * (e >> 2) + (e & 3)) & 1) != 0; };
@@ -292,29 +306,44 @@ struct ManyRows : AttnRows<HD> {
                 }
             }
             this->template weights<H, true>(s, big, step_exponent, p);
+            // The weights by group q's steps, as halves, while group q - 1 is multiplied.
+            Steps dv[2][8];
+            auto read_dv = [&](int b) {
 #pragma unroll
-            for (int b = 0; b < H / 2; ++b) {
-                Steps dv[8];
+                for (int e = 0; e < 8; ++e) dv[b & 1][e] = vs[32 * b + 16 * (e >> 2) + 4 * g + (e & 3)];
+            };
+            half8_t wh[2], wl[2];
+            auto split = [&](int q) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dv[e] = vs[32 * b + 16 * (e >> 2) + 4 * g + (e & 3)];
-#pragma unroll
-                for (int t = 0; t < NB; ++t) {
-                    const int q = b * NB + t;
-                    if (q + 1 < GROUPS) read_v(q + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = times(p[8 * b + e], dv[e].s[t]);
-                        if (MASKED) x[e] = sees(e) ? x[e] : 0.f;   // a step that the row does not see may be anything
-                    }
-                    halves(x, ph, pl);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        o[2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][u], pl, o[2 * t + u], 0, 0, 0);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        o[2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][u], ph, o[2 * t + u], 0, 0, 0);
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = times(p[8 * (q / NB) + e], dv[q / NB & 1][e].s[q % NB]);
+                    if (MASKED) x[e] = sees(e) ? x[e] : 0.f;   // a step that the row does not see may be anything
                 }
+                halves(x, wh[q & 1], wl[q & 1]);
+            };
+            read_dv(0);
+            split(0);
+#pragma unroll
+            for (int q = 0; q < GROUPS; ++q) {
+                const int t = q % NB;
+                if (q + 1 < GROUPS) read_v(q + 1);
+                if (t == (NB > 1 ? NB - 2 : 0) && q + NB < GROUPS + t) read_dv(q / NB + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        o[2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][u], k ? wh[q & 1] : wl[q & 1],
+                                                                              o[2 * t + u], 0, 0, 0);
+                if (q + 1 < GROUPS) {
+                    split(q + 1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
