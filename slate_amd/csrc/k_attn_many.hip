@@ -13,6 +13,14 @@
 //   f32: a row of K or V is scaled by a power of two to [2^13, 2^14) at its
 //       largest element and split into halves hi + lo of 22 bits; three MFMAs
 //       a product (lo * lo is below what f32 sums keep).
+// What bounds it: over the 8-bit cache the vector unit (58 % of the cycles:
+// 64 x 4 products by steps, the weights and their halves, the conversion;
+// MFMA 28 %, LDS 37 %, the rest waits for the stage's barrier), over f32 pools
+// the bytes.  Head_dim 128, 8 kv heads: a mixed step of 13 decoding users and
+// three 1024-token chunks 360 us (242 TFLOP/s), one 4096-token prompt 340 us,
+// 4 users' 64-token trees over 9000 keys 241 us (304 TFLOP/s); 16 users'
+// 26-token trees over 645 MB of f32 caches 158 us (4.1 TB/s).  12 or 16
+// waves, or two tiles a wave, do not fit the registers.
 // Rows stay as they are stored, [key][element]: V^T comes out of LDS by the
 // transposing read.  16-byte chunks of a row are permuted, chunk c of key k
 // at place c ^ turn(k), so that both kinds of reads spread over the banks.
@@ -171,7 +179,9 @@ struct ManyRows : AttnRows<HD> {
         floatx4 s[H];
         const floatx4 zero = zeros();
         // Operands come out of LDS one group of MFMAs ahead; the fences keep
-        // the order (the scheduler undoes it where registers get scarce).
+        // the order, which the scheduler gives up where registers get scarce
+        // (mixed step 405 -> 368 us, trees over f32 172 -> 158 us).  8-bit: what a group leaves to
+        // the vector unit goes between the MFMAs of the next (368 -> 360 us).
         // A group of K: 16 keys, for f32 at most 64 elements of them.
         constexpr int KT = F32 && NB > 2 ? 2 : NB, KG = NB / KT, LO = F32 ? KT : 0;
         half8_t kr[2][KT + LO];
@@ -358,6 +368,8 @@ __device__ __forceinline__ float lanes_max(float v) {
     return fmaxf(v, dpp_mov<DPP_QUAD_XOR2>(v));
 }
 
+// TREE: rows see their ancestors, else what lies before them (one kernel for
+// both holds the registers of both: 418 against 406 us for the mixed step).
 template <int HD, bool F32, bool TREE>
 __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, PackedBatch pb) {
     using Geo = ManyGeom<HD, F32>;
