@@ -1,6 +1,6 @@
 // k_attn_q8.hip -- attention over the 8-bit cache for few query rows per
 // (sequence, kv head): a decode step's tokens times the query heads of a kv
-// head, trees of up to 96 rows.  The arithmetic: attn_q8.h, how the keys are
+// head, trees of up to 80 rows.  The arithmetic: attn_q8.h, how the keys are
 // shared out: attn_plan.h.
 //
 // A workgroup takes a block of 16 rows over a range of keys, each of its four
@@ -226,10 +226,11 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
 int64_t attention_q8_few_bytes(int hd) { return plan_bytes(AF_WGS, AR_TILE, hd); }
 // Blocks of 16 rows read the keys again for every block, but without a
 // barrier: 48 rows (12 drafts, 4 heads a kv head, 16 sequences of up to 4096)
-// 55 us here and 61 in the many-row kernel, 80 rows 85 and 88, 96 rows 87 and
-// 84, 128 rows 110 and 93; one sequence of 16384 39 and 46, 47 and 44, 47 and
-// 44, 52 and 49.  A row's drafts are kept in 32 bits.
-constexpr int AF_MAX_ROWS = 96, AF_MAX_NEW = 32;
+// 56 us here and 64 in the many-row kernel, 80 rows 77 and 80, 96 rows 87 and
+// 81; 64 sequences of up to 2000 107 and 123, 144 and 144, 173 and 152; of
+// head_dim 64 36 and 44, 49 and 50, 55 and 51; one sequence of 16384 39 and 35,
+// 47 and 43, 47 and 43.  A row's drafts are kept in 32 bits.
+constexpr int AF_MAX_ROWS = 80, AF_MAX_NEW = 32;
 bool attention_q8_few_takes(const PackedAttn& a, const PackedBatch& pb) {
     return !a.kf && (a.hd == 32 || a.hd == 64 || a.hd == 128) && pb.max_new <= AF_MAX_NEW &&
            pb.max_new * (int64_t)(a.Hq / a.Hkv) <= AF_MAX_ROWS;

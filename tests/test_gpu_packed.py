@@ -284,6 +284,16 @@ def test_ragged_q8_long(hip):
     r.check()
 
 
+@pytest.mark.parametrize("G,seqs", [(8, [(300, 1100), (0, 1)]), (3, [(40, 2800)]), (130, [(0, 70), (513, 3)]),
+                                    (1, [(0, 600), (2000, 129), (0, 9000)])])
+def test_prompts_of_many_blocks(hip, G, seqs):
+    """More blocks of 128 query rows than a wave has lanes; blocks that begin and end inside a token's heads."""
+    bt = Batch(seqs, 1, 32, max(p + n for p, n in seqs) + 1, np.random.default_rng(G))
+    r = Run(bt, G, True, 9)
+    r.call()
+    r.check()
+
+
 def test_ragged_q8_bound_on_tokens(hip):
     """A sequence with more tokens than max_new is left out; the others are computed."""
     bt = Batch([(10, 1), (20, 5), (30, 2)], 1, 64, 64, np.random.default_rng(1))
@@ -357,9 +367,10 @@ def test_base_is_rounded_down_to_a_row(hip):
     r.check()
 
 
-@pytest.mark.parametrize("G,n", [(1, 32), (1, 33), (3, 32), (4, 24), (4, 25), (16, 6), (16, 7), (96, 1), (97, 1)])
+@pytest.mark.parametrize("G,n", [(1, 32), (1, 33), (3, 26), (3, 27), (3, 32), (4, 20), (4, 21), (4, 24), (4, 25), (16, 5),
+                                 (16, 6), (16, 7), (80, 1), (81, 1), (96, 1), (97, 1)])
 def test_rows_around_the_kernels_border(hip, G, n):
-    """96 query rows per kv head and 32 tokens are where one kernel hands over to the other."""
+    """80 query rows per kv head and 32 tokens are where one kernel hands over to the other."""
     rng = np.random.default_rng(16)
     bt = Batch([(700, n), (31, max(1, n - 1)), (5, 1)], 1, 64, 800, rng)
     for kind in ("causal", "tree"):
