@@ -245,8 +245,9 @@ int   slate_hip_rope_frequencies(double* w, double* magnitude, const slate_hip_r
  * offsets may pass 32 bits).  A sequence may have no token in a call.  One whose
  * numbers do not fit (tok_off falling or outside 0 .. T, more than max_new
  * tokens where the call has that bound, pos0 < 0, pos0 + tokens > max_seq,
- * kv_base < 0) is left out: nothing of it is read or written.  Rows of the
- * outputs that no sequence owns stay as they were.
+ * kv_base < 0) is left out: nothing of it is read or written.  Behind a fall
+ * of tok_off sequences may be left out too.  Rows of the outputs that no
+ * sequence owns stay as they were.
  * The 8-bit pools: int8 codes (device, 16-byte aligned), and the f16 steps
  * (uint16_t bits, 16-byte aligned) of each 32 codes, the step of element e
  * at index e / 32.  A value is step * code: the values of Q8_0, in two pools
@@ -275,7 +276,8 @@ int   slate_hip_kv_load_q8(float* k, float* v, int64_t ld, const int8_t* Kq, con
  * tokens that one sequence brings (1 for a decode step); head_dim is at most
  * 512; 32, 64 and 128 run on the matrix instructions, the others on a plain
  * kernel.  Queries must be finite and, like the cache's values, below 2^100
- * in size.  What the cache holds in rows a token does not see never matters.
+ * in size (f32 values are resolved to 2^-22 of their row's largest, and to
+ * 2^-114).  What the cache holds in rows a token does not see never matters.
  * ws: device scratch of slate_hip_attention_packed_bytes, 16-byte aligned,
  * its content of no matter, for calls that run beside each other or are
  * captured into graphs that do; NULL takes the backend's own, which calls on

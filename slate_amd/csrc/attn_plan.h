@@ -8,7 +8,9 @@
 // its neighbours': two slots of partial results per workgroup, whatever the
 // batch.  A block that lies inside one range is written straight out.
 // Every wave works the plan out by itself from the descriptors, which a lane
-// each loads once; N < 2^31 (the entries check it).
+// each loads once; N < 2^31: the entries check it for T tokens, and sequences
+// behind a fall of tok_off, which could have the same tokens over and over,
+// are left out.
 #pragma once
 #include "lanes.h"
 #include "packed.h"
@@ -50,11 +52,17 @@ template <class Count>
 class Plan {
   public:
     int total;
+    int end;                           // sequences from it on are left out
 
     __device__ __forceinline__ Plan(const PackedBatch& pb, const Count& count) : pb_(pb), count_(count) {
+        end = pb.B;
+        cut(0);
         first_ = load(0);
         total = __builtin_amdgcn_readlane(first_.upto, 63);
-        for (int b0 = 64; b0 < pb.B; b0 += 64) total += __builtin_amdgcn_readlane(load(b0).upto, 63);
+        for (int b0 = 64; b0 < end; b0 += 64) {
+            cut(b0);
+            total += __builtin_amdgcn_readlane(load(b0).upto, 63);
+        }
     }
     // The plan's first 64 sequences can wait in LDS instead of in registers.
     struct Lane {
@@ -62,8 +70,8 @@ class Plan {
         int64_t base;
         int own, upto;                 // granules of the lane's sequence, and with those of the lanes before it
     };
-    __device__ __forceinline__ Plan(const PackedBatch& pb, const Count& count, int total_, const Lane& first)
-        : total(total_), pb_(pb), count_(count), first_(first) {}
+    __device__ __forceinline__ Plan(const PackedBatch& pb, const Count& count, int total_, int end_, const Lane& first)
+        : total(total_), end(end_), pb_(pb), count_(count), first_(first) {}
     __device__ __forceinline__ const Lane& first() const { return first_; }
     // 0 <= x < total
     __device__ __forceinline__ Place find(int x) const {
@@ -96,10 +104,15 @@ class Plan {
     }
 
   private:
+    __device__ __forceinline__ void cut(int b0) {
+        const int b = b0 + (int)(threadIdx.x & 63);
+        const uint64_t falls = __builtin_amdgcn_ballot_w64(b < end && pb_.tok_off[b + 1] < pb_.tok_off[b]);
+        if (falls) end = b0 + __builtin_ctzll(falls);
+    }
     __device__ __forceinline__ Lane load(int b0) const {
         const int b = b0 + (int)(threadIdx.x & 63);
         Lane s{};
-        if (b < pb_.B) {
+        if (b < end) {
             s.seq = seq_view(pb_, b);
             s.base = pb_.kv_base[b];
             s.own = count_(s.seq);

@@ -109,7 +109,7 @@ struct AttnRows {
                 top = fmaxf(top, fabsf(v[t][e]));
             }
         top = cols_max(top);
-        const int e2 = top > 0.f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+        const int e2 = top > 0.f ? min(126, 14 - __builtin_amdgcn_frexp_expf(top)) : 0;   // unq is not 0
         unq = ldexpf(1.0f, -e2);
 #pragma unroll
         for (int t = 0; t < NB; ++t) {

@@ -421,10 +421,10 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
                      count.seen(pl.seq, pl.block) - 1,
                      TREE ? pl.seq.p0 : pl.seq.p0 + pl.block * ROWS / G + 1, base + pl.h * a.head_stride};
     };
-    const int total = plan.total;
+    const int total = plan.total, end = plan.end;
     auto piece_after = [&](const Piece& p) {
         const int x = p.x + p.g1 - p.g0;
-        return x < x1 ? piece_in(ManyPlan(pb, count, total, s_plan[lane]), x) : Piece{x1};
+        return x < x1 ? piece_in(ManyPlan(pb, count, total, end, s_plan[lane]), x) : Piece{x1};
     };
     // a stage's rows on their way: the thread's unit of K and of V, and steps
     // (rows past the last key repeat it: nobody sees them)
@@ -485,7 +485,11 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
 #pragma unroll
                         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
                         top = lanes_max<HD / 8>(top);
-                        const int e2 = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+                        // K: a step's inverse stays a normal number.  V: weights carry 2^(11 - 14 + e2) (AR_PEXP),
+                        // and their sum over the keys stays finite; rows below 2^-92 are kept to 2^-114.
+                        const int e2 = top > 0.f && top < INFINITY
+                                           ? min(kv ? 90 : 126, 14 - __builtin_amdgcn_frexp_expf(top))
+                                           : 0;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], e2);
                         half8_t hi, lo;

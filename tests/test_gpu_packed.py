@@ -367,6 +367,60 @@ def test_base_is_rounded_down_to_a_row(hip):
     r.check()
 
 
+@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("first", [2, 70])
+def test_token_offsets_that_fall(hip, q8, n, first):
+    """Offsets that go back over the same tokens again and again: the sequences before the first fall are computed,
+    the others may be left out, and no count of keys passes 32 bits."""
+    seqs = [(50 + b, n) for b in range(first)]
+    B = 1000
+    rng = np.random.default_rng(first)
+    bt = Batch(seqs, 1, 64, 4000, rng)
+    parent = random_parents(bt, rng, "chain")
+    r = Run(bt, 2, q8, 21, parent)
+    off = np.zeros(B + 1, np.int32)
+    off[:first + 1] = bt.off
+    off[first + 1::2] = 0
+    off[first + 2::2] = bt.T
+    pos0 = np.zeros(B, np.int32)
+    pos0[:first] = bt.pos0
+    base = np.zeros(B, np.int64)
+    base[:first] = bt.base
+    bt.d_off, bt.d_pos, bt.d_base = (DeviceBuffer.from_array(a) for a in (off, pos0, base))
+    bt.B = B
+    r.call(max_new=min(bt.T, 1024))
+    bt.B = first
+    r.check()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 96, 2.0 ** -60, 2.0 ** -85, 2.0 ** -105, 2.0 ** -130])
+def test_tree_values_far_from_one(hip, scale):
+    """f32 values up to 2^99, far below 1, and queries that are all but 0: nothing over- or underflows into NaN."""
+    rng = np.random.default_rng(3)
+    for name in ("K", "V", "q"):
+        bt = Batch([(40, 12), (0, 40), (300, 3)], 2, 64, 400, rng)
+        pools = fill_f32(bt, 5)
+        if name != "q":
+            pools[name] *= np.float32(scale)
+        r = Run(bt, 4, False, 5, random_parents(bt, rng, "random"), pools=pools)
+        if name == "q":
+            r.q *= np.float32(scale)
+            r.qd.upload(r.q)
+        r.call()
+        if name != "V" or scale >= 2.0 ** -85:
+            r.check()
+            continue
+        # below 2^-92 a value is kept to 2^-114: half a step of the lower half at the scale 2^90, and products add
+        # at most the weights' own rounding
+        out = r.result().astype(np.float64)
+        exact = Run(bt, 4, False, 5, r.parent, pools=dict(pools, V=pools["V"] / np.float32(scale)))
+        exact.call()
+        exact.check()
+        want = exact.result().astype(np.float64) * scale
+        assert np.abs(out - want).max() <= 2.0 ** -113 + 2.0 ** -20 * np.abs(want).max()
+
+
 @pytest.mark.parametrize("G,n", [(1, 32), (1, 33), (3, 26), (3, 27), (3, 32), (4, 20), (4, 21), (4, 24), (4, 25), (16, 5),
                                  (16, 6), (16, 7), (80, 1), (81, 1), (96, 1), (97, 1)])
 def test_rows_around_the_kernels_border(hip, G, n):
