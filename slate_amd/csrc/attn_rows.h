@@ -128,8 +128,10 @@ struct AttnRows {
     // The weights p of the lane's 4 H scores s (keys 16 hf + 4g + i of row j;
     // -inf: not seen).  big: the largest V step, in the lane's own keys
     // (EACH) or in any lane; exponent(big): e with that step in [2^(e-1), 2^e).
+    // shift: powers of two that the weights of each 32 keys get besides (none: nullptr).
     template <int H, bool EACH, class Exponent>
-    __device__ __forceinline__ void weights(const floatx4* s, int big, const Exponent& exponent, float* p) {
+    __device__ __forceinline__ void weights(const floatx4* s, int big, const Exponent& exponent, float* p,
+                                            const int* shift = nullptr) {
         float mx = s[0][0];
 #pragma unroll
         for (int e = 1; e < 4 * H; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
@@ -157,9 +159,15 @@ struct AttnRows {
         }
         const float mref = pexp - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-        for (int e = 0; e < 4 * H; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], unq, mref));
-            l += p[e];
+        for (int b = 0; b < H / 2; ++b) {
+            const float by = shift ? mref + (float)shift[b] : mref;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 8 * b; e < 8 * b + 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], unq, by));
+                (shift ? sum : l) += p[e];
+            }
+            if (shift) l += ldexpf(sum, -shift[b]);
         }
     }
 

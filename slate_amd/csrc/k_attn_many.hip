@@ -169,8 +169,8 @@ struct ManyRows : AttnRows<HD> {
     // keys (8-bit, all keys seen).  bad: keys whose V row has an element that
     // is not finite (it is 0 in the plane), vrow the first key's row (f32).
     template <int H, bool MASKED>
-    __device__ __forceinline__ void keys(const _Float16* planes, int at, const unsigned char* steps, int top,
-                                         uint32_t seen, uint32_t bad, const float* vrow) {
+    __device__ __forceinline__ void keys(const _Float16* planes, int at, const unsigned char* steps, int2 top,
+                                         const _Float16* vnorm, uint32_t seen, uint32_t bad, const float* vrow) {
         constexpr int PLANE = AM_KEYS * HD;
         const int lane = threadIdx.x & 63, g = lane >> 4;
         const _Float16 *k = planes + at * HD, *v = k + (F32 ? 2 : 1) * PLANE;
@@ -301,7 +301,8 @@ struct ManyRows : AttnRows<HD> {
                         }
                 }
         } else {
-            int big = top;
+            int big = max(top.x, top.y);
+            const int shift[2] = {step_exponent(top.x), step_exponent(top.y)};
             if (MASKED) {
                 big = 0;
 #pragma unroll
@@ -315,45 +316,68 @@ struct ManyRows : AttnRows<HD> {
                     }
                 }
             }
-            this->template weights<H, true>(s, big, step_exponent, p);
-            // The weights by group q's steps, as halves, while group q - 1 is multiplied.
-            Steps dv[2][8];
-            auto read_dv = [&](int b) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) dv[b & 1][e] = vs[32 * b + 16 * (e >> 2) + 4 * g + (e & 3)];
-            };
+            // Group q's weights are p times its steps as halves, hi + lo to 22
+            // bits, made while group q - 1 is multiplied.
             half8_t wh[2], wl[2];
-            auto split = [&](int q) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = times(p[8 * (q / NB) + e], dv[q / NB & 1][e].s[q % NB]);
-                    if (MASKED) x[e] = sees(e) ? x[e] : 0.f;   // a step that the row does not see may be anything
-                }
-                halves(x, wh[q & 1], wl[q & 1]);
+            auto multiply = [&](int q, int k) {            // k: the tile in bit 0, hi in bit 1
+                o[2 * (q % NB) + (k & 1)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    vr[q & 1][k & 1], k & 2 ? wh[q & 1] : wl[q & 1], o[2 * (q % NB) + (k & 1)], 0, 0, 0);
             };
-            read_dv(0);
-            split(0);
+            if constexpr (MASKED) {
+                this->template weights<H, true>(s, big, step_exponent, p);
+                Steps dv[8];
 #pragma unroll
-            for (int q = 0; q < GROUPS; ++q) {
-                const int t = q % NB;
-                if (q + 1 < GROUPS) read_v(q + 1);
-                if (t == (NB > 1 ? NB - 2 : 0) && q + NB < GROUPS + t) read_dv(q / NB + 1);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int e = 0; e < 8; ++e) dv[e] = vs[16 * (e >> 2) + 4 * g + (e & 3)];
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int q = 0; q < GROUPS; ++q) {
+                    if (q + 1 < GROUPS) read_v(q + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    float x[8];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        o[2 * t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vr[q & 1][u], k ? wh[q & 1] : wl[q & 1],
-                                                                              o[2 * t + u], 0, 0, 0);
-                if (q + 1 < GROUPS) {
-                    split(q + 1);
+                    for (int e = 0; e < 8; ++e) x[e] = sees(e) ? times(p[e], dv[e].s[q]) : 0.f;   // an unseen step may be anything
+                    halves(x, wh[q & 1], wl[q & 1]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);
+                    for (int k = 0; k < 4; ++k) multiply(q, k);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                // All keys are seen: their steps come as f16 d by the power of
+                // two of the largest of the 32, in (0, 1), and p = a + b, by
+                // the inverse power, is split but once.  hi = f16(a d), its
+                // remainder a d - hi is exact, lo = b d + that: packed f16
+                // operations, half of what f32 products and their halves take.
+                this->template weights<H, true>(s, big, step_exponent, p, shift);
+                half8_t ph[H / 2], pl[H / 2], d[2];
+#pragma unroll
+                for (int b = 0; b < H / 2; ++b) halves(p + 8 * b, ph[b], pl[b]);
+                auto read_d = [&](int q) {
+                    const _Float16* at = vnorm + q % NB * AM_KEYS + 32 * (q / NB) + 4 * g;
+                    const half4_t lo = *(const half4_t*)at, hi = *(const half4_t*)(at + 16);
+                    d[q & 1] = half8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                };
+                half8_t rest;
+                auto split = [&](int q, int k) {           // in three steps
+                    const half8_t a = ph[q / NB], dq = d[q & 1];
+                    if (k == 0) wh[q & 1] = a * dq;
+                    if (k == 1) rest = __builtin_elementwise_fma(a, dq, -wh[q & 1]);
+                    if (k == 2) wl[q & 1] = __builtin_elementwise_fma(pl[q / NB], dq, rest);
+                };
+                read_d(0);
+                if (GROUPS > 1) read_d(1);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) split(0, k);
+#pragma unroll
+                for (int q = 0; q < GROUPS; ++q) {
+                    if (q + 1 < GROUPS) read_v(q + 1);
+                    if (q + 2 < GROUPS) read_d(q + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        multiply(q, k);
+                        if (q + 1 < GROUPS) split(q + 1, k);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -384,6 +408,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
     __shared__ ManyPlan::Lane s_plan[64];
     __shared__ uint32_t s_bad[4][2];                  // f32: keys whose V row has an element that is not finite
     __shared__ int s_top[2][2];                       // 8-bit: the largest V step of each 32 keys
+    __shared__ __attribute__((aligned(16))) _Float16 s_vnorm[2][F32 ? 1 : NB * KEYS];   // [block][key]: V steps by 2^-shift
     // what the waves that share rows leave for each other: where the stage
     // that is worked through was, if it fits
     constexpr int OS = HD + 4;
@@ -514,6 +539,9 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) top = max(top, __shfl_xor(top, off));
                 if ((lane & 31) == 0) s_top[to][lane >> 5] = top;
+#pragma unroll
+                for (int t = 0; t < NB; ++t)
+                    s_vnorm[to][t * KEYS + lane] = (_Float16)ldexpf((float)st.s[t], -step_exponent(top));
             }
         }
     };
@@ -622,12 +650,13 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             const unsigned char* steps = s_step[now];
             const int top0 = F32 ? 0 : s_top[now][0], top1 = F32 ? 0 : s_top[now][1];
             const bool all = sh.parts == 1 && k0 + KEYS <= open && k0 < end;
-            if (all) R.template keys<4, false>(planes, 0, steps, max(top0, top1), 0, 0, nullptr);
+            if (all) R.template keys<4, false>(planes, 0, steps, make_int2(top0, top1), s_vnorm[now], 0, 0, nullptr);
 #pragma unroll 1
             for (int at = 0; !all && at < KEYS && k0 + at < end; at += AR_KEYS) {
                 if (((2 * gr + at / AR_KEYS) & (sh.parts - 1)) != sh.part) continue;
                 if (k0 + at + AR_KEYS <= open) {
-                    R.template keys<2, false>(planes, at, steps, at ? top1 : top0, 0, 0, nullptr);
+                    R.template keys<2, false>(planes, at, steps, make_int2(at ? top1 : top0, 0), s_vnorm[now] + (F32 ? 0 : at), 0, 0,
+                                                nullptr);
                     continue;
                 }
                 uint32_t seen = 0;
@@ -640,7 +669,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
                     const uint32_t hi = wd + 1 < 0 ? 0xffffffffu : wd + 1 < words ? s_seen[wd + 1][tok - tok0] : 0;
                     seen = (uint32_t)(((uint64_t)hi << 32 | lo) >> (d & 31));
                 }
-                R.template keys<2, true>(planes, at, steps, 0, seen, F32 ? s_bad[now_ring][at >> 5] : 0,
+                R.template keys<2, true>(planes, at, steps, make_int2(0, 0), nullptr, seen, F32 ? s_bad[now_ring][at >> 5] : 0,
                                          F32 ? a.vf + pc.at + (int64_t)(k0 + at) * HD : nullptr);
             }
             if (had && !early) bring();
