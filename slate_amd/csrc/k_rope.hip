@@ -13,21 +13,24 @@ namespace slate_hip {
 
 // A thread owns four neighbouring pairs (VEC = 4, rot % 8 == 0) or one (VEC = 1,
 // any even rot) and walks over heads with their cosines and sines: two
-// 16-byte loads and stores a head, two heads' loads at a time.  Where the rest
-// of the head is copied (y != x) and comes in groups of eight too, the
-// threads after the pairs' copy those the same way.  A workgroup takes one
+// 16-byte loads and stores a head, two heads' loads at a time (of single pairs
+// four heads').  Where the rest of the head is copied (y != x), the threads
+// after the pairs' copy it the same way.  A workgroup takes one
 // row, or a part of its heads where rows are few.
 // Memory bound: 4096 rows of 72 heads of 128 (302 MB) take 60.3 us, 5.0 TB/s
 // (a 4 GiB copy reaches 4.7); one pass over heads at a time and scalar copies
-// of the rest took 66.9.  16 rows of 40 heads: 3 us, the launch and two rounds
-// of load latency.
+// of the rest took 66.9.  Single pairs: 7438 rows of 40 heads of
+// 116, 42 of them turned (276 MB), 58.8 us, 4.7 TB/s (89.7 with the rest
+// copied after the pairs).  16 rows of 40 heads: 3 us, the launch and two
+// rounds of load latency.
 template <int VEC>
 __global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float* x, const int32_t* __restrict__ pos,
                                                           int n_heads, int hd, int64_t ld, int layout, int rot,
                                                           float magnitude, int units, int heads_per_wg,
                                                           const RopeTurns turns) {
-    constexpr int N = VEC == 4 ? 4 : 1;
+    constexpr int N = VEC == 4 ? 4 : 1, HEADS = VEC == 4 ? 2 : 4;   // loads at a time
     typedef float vec __attribute__((ext_vector_type(N), aligned(4)));
+    typedef float float4a __attribute__((ext_vector_type(4), aligned(4)));
     const int row = blockIdx.x;
     const int h0 = blockIdx.y * heads_per_wg, h1 = min(n_heads, h0 + heads_per_wg);
     const float* xr = x + (int64_t)row * ld;
@@ -51,16 +54,17 @@ __global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float*
                 s[e] *= magnitude;
             }
         }
-        for (int h = h0 + hh; h < h1; h += 2 * step) {
-            vec a[2], b[2];
+        for (int h = h0 + hh; h < h1; h += HEADS * step) {
+            vec a[HEADS], b[HEADS];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < HEADS; ++k) {
+                if (VEC == 1 && k > 0 && h + k * step >= h1) break;
                 const float* xh = xr + (int64_t)min(h + k * step, h1 - 1) * hd;
                 a[k] = *(const vec*)(xh + ja);
                 b[k] = *(const vec*)(xh + jb);
             }
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < HEADS; ++k) {
                 if (h + k * step >= h1) break;
                 vec ya = a[k], yb = b[k];
                 if (turn) {
@@ -91,9 +95,14 @@ __global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float*
     }
     const int done = 2 * VEC * units, tail = hd - done;   // what the units leave of a head
     if (tail > 0 && y != x) {
-        for (int e = threadIdx.x; e < (h1 - h0) * tail; e += blockDim.x) {
-            const int64_t at = (int64_t)(h0 + e / tail) * hd + done + e % tail;
-            yr[at] = xr[at];
+        const int each = (tail + 3) / 4;               // four floats a thread, the last of a head up to four
+        for (int e = threadIdx.x; e < (h1 - h0) * each; e += blockDim.x) {
+            const int c = 4 * (e % each);
+            const int64_t at = (int64_t)(h0 + e / each) * hd + done + c;
+            if (c + 4 <= tail)
+                *(float4a*)(yr + at) = *(const float4a*)(xr + at);
+            else
+                for (int k = 0; k < tail - c; ++k) yr[at + k] = xr[at + k];
         }
     }
 }
@@ -101,7 +110,8 @@ __global__ __launch_bounds__(256) void rope_scaled_kernel(float* y, const float*
 int launch_rope_scaled(float* y, const float* x, const int32_t* pos, int n_rows, int n_heads, int hd, int64_t ld,
                        int layout, int rot, float magnitude, const RopeTurns& turns, hipStream_t s) {
     const bool vec = rot % 8 == 0;
-    const int units = !vec ? rot / 2 : y != x && hd <= 2048 ? hd / 8 : rot / 8;
+    const int wide = vec ? 8 : 2;
+    const int units = y != x && hd <= 256 * wide ? hd / wide : rot / wide;
     const int step = 256 / units;
     // few rows: a workgroup takes as many heads as it has threads for
     const int per = n_rows < 512 ? max(step, n_heads / 32768) : n_heads;

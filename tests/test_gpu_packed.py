@@ -55,6 +55,10 @@ ROPES = [
     (515, 11, 96, 5, 1 << 17, dict(layout=1, rot_dim=96)),
     (3, 40000, 16, 0, 3000, dict(layout=0, rot_dim=16)),
     (4, 7, 2056, 0, 900, dict(layout=1, rot_dim=512)),
+    (9, 6, 116, 1, 900, dict(layout=1, rot_dim=42)),
+    (520, 3, 29, 0, 900, dict(layout=0, rot_dim=22)),
+    (520, 2, 25, 2, 900, dict(layout=1, rot_dim=22)),
+    (3, 2, 2083, 0, 900, dict(layout=0, rot_dim=64)),
 ]
 
 
