@@ -14,13 +14,13 @@
 //       largest element and split into halves hi + lo of 22 bits; three MFMAs
 //       a product (lo * lo is below what f32 sums keep).
 // What bounds it: over the 8-bit cache the vector unit (58 % of the cycles:
-// 64 x 4 products by steps, the weights and their halves, the conversion;
-// MFMA 28 %, LDS 37 %, the rest waits for the stage's barrier), over f32 pools
-// the bytes.  Head_dim 128, 8 kv heads: a mixed step of 13 decoding users and
-// three 1024-token chunks 360 us (242 TFLOP/s), one 4096-token prompt 340 us,
-// 4 users' 64-token trees over 9000 keys 241 us (304 TFLOP/s); 16 users'
-// 26-token trees over 645 MB of f32 caches 158 us (4.1 TB/s).  12 or 16
-// waves, or two tiles a wave, do not fit the registers.
+// products by steps, the weights and their halves, the conversion; MFMA 30 %,
+// LDS 44 %, a third of the waves' time waits, most for the stage's barrier),
+// over f32 pools the bytes.  Head_dim 128, 8 kv heads: a mixed step of 13
+// decoding users and three 1024-token chunks 351 us (248 TFLOP/s), one
+// 4096-token prompt 321 us, 4 users' 64-token trees over 9000 keys 227 us
+// (323 TFLOP/s); 16 users' 26-token trees over 645 MB of f32 caches 159 us
+// (4.1 TB/s).  12 or 16 waves, or two tiles a wave, do not fit the registers.
 // Rows stay as they are stored, [key][element]: V^T comes out of LDS by the
 // transposing read.  16-byte chunks of a row are permuted, chunk c of key k
 // at place c ^ turn(k), so that both kinds of reads spread over the banks.
@@ -165,8 +165,9 @@ struct ManyRows : AttnRows<HD> {
 
     // 16 H keys from key `at` of the stage on.  planes: K hi (lo), V hi (lo);
     // ks, vs: the keys' steps (Steps, or the power of two of a row as a
-    // float).  MASKED as in Q8Rows (H = 2).  top: the largest V step among the
-    // keys (8-bit, all keys seen).  bad: keys whose V row has an element that
+    // float).  MASKED as in Q8Rows (H = 2).  8-bit, all keys seen: top, the
+    // bits of the largest V step of each 32 keys, vnorm, the V steps by the
+    // inverse of its power of two, [block][key].  bad: keys whose V row has an element that
     // is not finite (it is 0 in the plane), vrow the first key's row (f32).
     template <int H, bool MASKED>
     __device__ __forceinline__ void keys(const _Float16* planes, int at, const unsigned char* steps, int2 top,
@@ -180,8 +181,9 @@ struct ManyRows : AttnRows<HD> {
         const floatx4 zero = zeros();
         // Operands come out of LDS one group of MFMAs ahead; the fences keep
         // the order, which the scheduler gives up where registers get scarce
-        // (mixed step 405 -> 368 us, trees over f32 172 -> 158 us).  8-bit: what a group leaves to
-        // the vector unit goes between the MFMAs of the next (368 -> 360 us).
+        // (mixed step 405 -> 368 us, trees over f32 172 -> 158 us).  8-bit: what
+        // a group leaves to the vector unit goes between the MFMAs of the next
+        // (368 -> 360 us).
         // A group of K: 16 keys, for f32 at most 64 elements of them.
         constexpr int KT = F32 && NB > 2 ? 2 : NB, KG = NB / KT, LO = F32 ? KT : 0;
         half8_t kr[2][KT + LO];
@@ -344,8 +346,10 @@ struct ManyRows : AttnRows<HD> {
                 // All keys are seen: their steps come as f16 d by the power of
                 // two of the largest of the 32, in (0, 1), and p = a + b, by
                 // the inverse power, is split but once.  hi = f16(a d), its
-                // remainder a d - hi is exact, lo = b d + that: packed f16
-                // operations, half of what f32 products and their halves take.
+                // remainder a d - hi is exact (or below 2^-25 where a weight of
+                // 1 stands for 2^10 or more), lo = b d + that: packed f16
+                // operations, half of what f32 products and their halves take
+                // (mixed step 373 -> 341 us).
                 this->template weights<H, true>(s, big, step_exponent, p, shift);
                 half8_t ph[H / 2], pl[H / 2], d[2];
 #pragma unroll
