@@ -115,7 +115,9 @@ __global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ 
             float4 v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float* sl = slot(min(k0 + k, en.pieces - 1));
+                ml[k] = make_float2(-INFINITY, 0.f);
+                if (k0 + k >= en.pieces) continue;     // the same for the whole workgroup
+                const float* sl = slot(k0 + k);
                 ml[k] = *(const float2*)(sl + slot_rows * HD + 2 * r);
                 v[k] = *(const float4*)(sl + r * HD + c);
             }
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ 
             o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float fk = k0 + k < en.pieces ? __builtin_amdgcn_exp2f(ml[k].x - mt) : 0.f;
+                const float fk = __builtin_amdgcn_exp2f(ml[k].x - mt);
                 if (fk == 0.f) continue;
                 l += fk * ml[k].y;
                 o.x += fk * v[k].x;
