@@ -398,6 +398,29 @@ def test_token_offsets_that_fall(hip, q8, n, first):
     r.check()
 
 
+@pytest.mark.parametrize("order", ["mixed", "rising", "falling"])
+@pytest.mark.parametrize("hd,G,n", [(128, 4, 1), (128, 4, 40), (64, 8, 33), (32, 2, 70)])
+def test_q8_steps_of_all_sizes(hip, hd, G, n, order):
+    """V steps that differ by up to 2^26 from block to block and key to key, some of them 0 or below f16's normal
+    range."""
+    rng = np.random.default_rng(n)
+    bt = Batch([(600, n), (0, n), (77, max(1, n - 3))], 2, hd, 700, rng)
+    pools = fill_q8(bt, 8)
+    q, st = pools["V"]
+    for b, (p, m) in enumerate(bt.seqs):
+        for h in range(bt.Hkv):
+            at, rows = bt.row(b, h, 0) // 32, p + m
+            by = rng.integers(-13, 14, (rows, hd // 32)).astype(np.float64)
+            if order != "mixed":
+                by = np.clip(np.sort(by[:, 0])[::-1 if order == "falling" else 1][:, None] + by / 8, -13, 13)
+            v = st[at:at + rows * (hd // 32)].reshape(rows, -1).astype(np.float64) * 2.0 ** np.rint(by)
+            v[rng.random(v.shape) < 0.05] = 0
+            st[at:at + v.size] = v.astype(np.float16).reshape(-1)
+    r = Run(bt, G, True, 8, pools=pools)
+    r.call()
+    r.check()
+
+
 @pytest.mark.parametrize("scale", [2.0 ** 96, 2.0 ** -60, 2.0 ** -85, 2.0 ** -105, 2.0 ** -130])
 def test_tree_values_far_from_one(hip, scale):
     """f32 values up to 2^99, far below 1, and queries that are all but 0: nothing over- or underflows into NaN."""
