@@ -17,9 +17,9 @@
 // products by steps, the weights and their halves, the conversion; MFMA 30 %,
 // LDS 44 %, a third of the waves' time waits, most for the stage's barrier),
 // over f32 pools the bytes.  Head_dim 128, 8 kv heads: a mixed step of 13
-// decoding users and three 1024-token chunks 351 us (248 TFLOP/s), one
-// 4096-token prompt 321 us, 4 users' 64-token trees over 9000 keys 227 us
-// (323 TFLOP/s); 16 users' 26-token trees over 645 MB of f32 caches 159 us
+// decoding users and three 1024-token chunks 345 us (252 TFLOP/s), one
+// 4096-token prompt 321 us, 4 users' 64-token trees over 9000 keys 225 us
+// (325 TFLOP/s); 16 users' 26-token trees over 645 MB of f32 caches 159 us
 // (4.1 TB/s).  12 or 16 waves, or two tiles a wave, do not fit the registers.
 // Rows stay as they are stored, [key][element]: V^T comes out of LDS by the
 // transposing read.  16-byte chunks of a row are permuted, chunk c of key k
