@@ -304,7 +304,9 @@ struct ManyRows : AttnRows<HD> {
                 }
         } else {
             int big = max(top.x, top.y);
-            const int shift[2] = {step_exponent(top.x), step_exponent(top.y)};
+            // V steps of 0 in all 32 keys: the smallest step's exponent, so that weights stay in f16's range
+            // whatever the largest step elsewhere is (their products are 0, infinity's would be NaN)
+            const int shift[2] = {step_exponent(max(top.x, 1)), step_exponent(max(top.y, 1))};
             if (MASKED) {
                 big = 0;
 #pragma unroll

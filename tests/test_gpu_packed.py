@@ -421,6 +421,63 @@ def test_q8_steps_of_all_sizes(hip, hd, G, n, order):
     r.check()
 
 
+# committed rows whose V is 0: the first 32 keys, a whole stage of 64, one half of a stage, both halves of two
+# stages that meet, a row alone, and drafts
+ZERO_ROWS = [(0, 32), (128, 192), (288, 320), (416, 480), (500, 501), (608, 610)]
+
+
+def zero_v_rows(bt, pools, drop, scale):
+    """V by `scale`, and 0 in the rows `drop` (first, past the last) of every sequence."""
+    v = pools["V"][1] if isinstance(pools["V"], tuple) else pools["V"]
+    v[:] = (v.astype(np.float64) * scale).astype(v.dtype)
+    per = 32 if isinstance(pools["V"], tuple) else 1
+    for b, (p, n) in enumerate(bt.seqs):
+        for h in range(bt.Hkv):
+            at = bt.row(b, h, 0)
+            for lo, hi in drop:
+                lo, hi = min(lo, p + n), min(hi, p + n)
+                v[(at + lo * bt.hd) // per:(at + hi * bt.hd) // per] = 0
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.1, 0.01])
+@pytest.mark.parametrize("kind", ["causal", "tree"])
+@pytest.mark.parametrize("hd,Hkv,G,n", [(32, 2, 2, 70), (64, 1, 8, 40), (128, 2, 4, 40), (128, 1, 4, 1)])
+def test_q8_rows_of_zero_steps(hip, hd, Hkv, G, n, kind, scale):
+    """V steps of 0 in all of 32 and of 64 neighbouring keys that every token sees, as zeroed cache rows have them and
+    as the store leaves where a step rounds to 0; blocks of 128 query rows and of fewer (which share the keys)."""
+    rng = np.random.default_rng(hd + n)
+    bt = Batch([(600, n), (64, max(1, n - 3)), (450, max(1, n // 8)), (0, n)], Hkv, hd, 700, rng)
+    pools = fill_q8(bt, 8)
+    zero_v_rows(bt, pools, ZERO_ROWS, scale)
+    r = Run(bt, G, True, 8, random_parents(bt, rng, "random") if kind == "tree" else None, pools=pools)
+    r.call()
+    check_beside_zero_rows(r)
+
+
+def check_beside_zero_rows(r):
+    """As Run.check; a sequence whose V is 0 in every row gets zeros (its error has no largest V to go by)."""
+    bt, out = r.bt, r.result()
+    for b, (p, n) in enumerate(bt.seqs):
+        if not any(host_rows(bt, r.pools["V"], b, h, p + n).any() for h in range(bt.Hkv)):
+            tk = list(bt.tokens(b))
+            assert np.all(out[tk] == 0)
+            out[tk] = SENTINEL
+            bt.bad.add(b)
+    check_attention(bt, r.pools, r.q, out, r.G, r.parent)
+
+
+def test_q8_all_steps_zero(hip):
+    """Nothing but zeros in V: the output is 0."""
+    rng = np.random.default_rng(1)
+    for n in (1, 40):
+        bt = Batch([(300, n), (0, 2)], 1, 64, 400, rng)
+        pools = fill_q8(bt, 8)
+        zero_v_rows(bt, pools, [(0, 400)], 1.0)
+        r = Run(bt, 4, True, 8, pools=pools)
+        r.call()
+        check_beside_zero_rows(r)
+
+
 @pytest.mark.parametrize("scale", [2.0 ** 96, 2.0 ** -60, 2.0 ** -85, 2.0 ** -105, 2.0 ** -130])
 def test_tree_values_far_from_one(hip, scale):
     """f32 values up to 2^99, far below 1, and queries that are all but 0: nothing over- or underflows into NaN."""
