@@ -270,8 +270,9 @@ struct ManyRows : AttnRows<HD> {
             for (int hf = 0; hf < H; ++hf) d[hf] = *(const floatx4*)(vf + 16 * hf + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4 * H; ++e) {
+                const float step = d[e >> 2][e & 3];   // (a bit cast of the element itself reads the vector's first)
                 if (!sees(e)) s[e >> 2][e & 3] = -INFINITY;
-                if (sees(e)) big = max(big, __builtin_bit_cast(int, d[e >> 2][e & 3]));
+                if (sees(e)) big = max(big, __builtin_bit_cast(int, step));
             }
             this->template weights<H, true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
 #pragma unroll

@@ -478,6 +478,28 @@ def test_q8_all_steps_zero(hip):
         check_beside_zero_rows(r)
 
 
+@pytest.mark.parametrize("order", ["mixed", "rising", "falling", "one"])
+@pytest.mark.parametrize("hd,G,n", [(128, 4, 5), (128, 4, 40), (64, 8, 33), (32, 2, 70)])
+def test_tree_rows_of_all_sizes(hip, hd, G, n, order):
+    """V rows of f32 pools that differ by up to 2^26 from key to key; one row in each ten far above the others, at
+    any place among its neighbours."""
+    rng = np.random.default_rng(n)
+    bt = Batch([(600, n), (0, n), (77, max(1, n - 3))], 2, hd, 700, rng)
+    pools = fill_f32(bt, 8)
+    for b, (p, m) in enumerate(bt.seqs):
+        for h in range(bt.Hkv):
+            at, rows = bt.row(b, h, 0), p + m
+            by = rng.integers(-13, 14, rows)
+            if order in ("rising", "falling"):
+                by = np.sort(by)[::-1 if order == "falling" else 1]
+            if order == "one":
+                by = np.where(rng.random(rows) < 0.1, 13, 0)
+            pools["V"][at:at + rows * hd] *= np.repeat(2.0 ** by, hd).astype(np.float32)
+    r = Run(bt, G, False, 8, random_parents(bt, rng, "random"), pools=pools)
+    r.call()
+    r.check()
+
+
 @pytest.mark.parametrize("scale", [2.0 ** 96, 2.0 ** -60, 2.0 ** -85, 2.0 ** -105, 2.0 ** -130])
 def test_tree_values_far_from_one(hip, scale):
     """f32 values up to 2^99, far below 1, and queries that are all but 0: nothing over- or underflows into NaN."""
