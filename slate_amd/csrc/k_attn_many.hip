@@ -528,7 +528,9 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
                         halves(x, hi, lo);
                         *(half8_t*)(at + place<HD>(key, elem / 8)) = hi;
                         *(half8_t*)(at + PLANE + place<HD>(key, elem / 8)) = lo;
-                        if (elem == 0) ((float*)s_step[to])[kv * KEYS + key] = ldexpf(1.0f, -e2);
+                        // a V row of zeros has a step of 0: it does not count among the largest steps
+                        if (elem == 0)
+                            ((float*)s_step[to])[kv * KEYS + key] = kv == 1 && top == 0.f ? 0.f : ldexpf(1.0f, -e2);
                     } else {
                         const uint4v r = raw[kv][u];
                         *(half8_t*)(at + place<HD>(key, elem / 8)) = codes_f16(uint2v{r[0], r[1]});

@@ -478,6 +478,30 @@ def test_q8_all_steps_zero(hip):
         check_beside_zero_rows(r)
 
 
+@pytest.mark.parametrize("scale", [1.0, 1e-2, 1e-4, 2.0 ** -20, 2.0 ** -60])
+@pytest.mark.parametrize("drop", [[(0, 1)], [(77, 78)], [(299, 300)], [(310, 312)], ZERO_ROWS, [(0, 64), (301, 340)]])
+def test_tree_rows_of_zeros(hip, drop, scale):
+    """V rows of zeros, committed and drafted, among small ones in f32 pools: the others keep their bits."""
+    rng = np.random.default_rng(3)
+    bt = Batch([(300, 40), (64, 3), (600, 12)], 2, 64, 640, rng)
+    pools = fill_f32(bt, 5)
+    zero_v_rows(bt, pools, drop, scale)
+    r = Run(bt, 4, False, 5, random_parents(bt, rng, "random"), pools=pools)
+    r.call()
+    check_beside_zero_rows(r)
+
+
+@pytest.mark.parametrize("hd,n", [(32, 33), (128, 5)])
+def test_tree_all_rows_zero(hip, hd, n):
+    rng = np.random.default_rng(4)
+    bt = Batch([(700, n), (0, 2)], 1, hd, 800, rng)
+    pools = fill_f32(bt, 5)
+    zero_v_rows(bt, pools, [(0, 800)], 1.0)
+    r = Run(bt, 4, False, 5, random_parents(bt, rng, "random"), pools=pools)
+    r.call()
+    check_beside_zero_rows(r)
+
+
 @pytest.mark.parametrize("order", ["mixed", "rising", "falling", "one"])
 @pytest.mark.parametrize("hd,G,n", [(128, 4, 5), (128, 4, 40), (64, 8, 33), (32, 2, 70)])
 def test_tree_rows_of_all_sizes(hip, hd, G, n, order):
