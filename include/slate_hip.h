@@ -245,7 +245,8 @@ int   slate_hip_rope_frequencies(double* w, double* magnitude, const slate_hip_r
  * offsets may pass 32 bits).  A sequence may have no token in a call.  One whose
  * numbers do not fit (tok_off falling or outside 0 .. T, more than max_new
  * tokens where the call has that bound, pos0 < 0, pos0 + tokens > max_seq,
- * kv_base < 0) is left out: nothing of it is read or written.  Behind a fall
+ * kv_base < 0) is left out: nothing of it is read or written.  (In attention
+ * a max_seq above 2^31 - 1024 counts as that.)  Behind a fall
  * of tok_off sequences may be left out too.  Rows of the outputs that no
  * sequence owns stay as they were.
  * The 8-bit pools: int8 codes (device, 16-byte aligned), and the f16 steps

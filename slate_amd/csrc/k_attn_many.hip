@@ -34,6 +34,7 @@ constexpr int AM_TH = 512;
 constexpr int AM_ROWS = 8 * AR_TILE;   // query rows of a block
 constexpr int AM_KEYS = 64;            // keys of a stage
 constexpr int AM_KEEP = 512;           // blocks of up to this many keys are not cut
+static_assert(AM_KEYS <= 128 && PK_MAX_KEYS + AM_KEYS > 0, "a count of keys passes 32 bits");
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 

@@ -22,7 +22,8 @@ constexpr int AF_WGS = 512;            // two workgroups per CU (LDS)
 constexpr int AF_GRAN = 4 * AR_KEYS;   // keys of a granule
 constexpr int AF_KEEP = 4;             // blocks of up to this many granules are not cut
 
-__host__ __device__ inline int few_granules(int keys) { return (keys + AF_GRAN - 1) / AF_GRAN; }
+__host__ __device__ constexpr int few_granules(int keys) { return (keys + AF_GRAN - 1) / AF_GRAN; }
+static_assert(few_granules(PK_MAX_KEYS) == (1 << 24) - 8 && AF_GRAN <= 128, "a count of keys passes 32 bits");
 
 // Granules of a sequence: blocks of 16 rows, of each kv head.
 struct FewCount {

@@ -70,7 +70,7 @@ int kv8_check(const char* what, const void* kq, const void* ks, const void* vq, 
     return 0;
 }
 
-int attention_packed(const char* what, const PackedAttn& a, const PackedBatch& pb, bool tree, size_t ws_bytes) {
+int attention_packed(const char* what, const PackedAttn& a, PackedBatch pb, bool tree, size_t ws_bytes) {
     const bool q8 = a.kf == nullptr && a.vf == nullptr;
     SH_REQUIRE(a.out && a.q && pb.tok_off && pb.pos0 && pb.kv_base && (!tree || a.parent) &&
                    (q8 ? a.kv8.kq && a.kv8.ks && a.kv8.vq && a.kv8.vs : a.kf && a.vf),
@@ -85,6 +85,7 @@ int attention_packed(const char* what, const PackedAttn& a, const PackedBatch& p
                "%s: head_dim=%d or head_stride=%lld", what, a.hd, (long long)a.head_stride);
     SH_REQUIRE(!q8 || (aligned16(a.kv8.kq) && aligned16(a.kv8.ks) && aligned16(a.kv8.vq) && aligned16(a.kv8.vs)),
                "%s: pools are not 16-byte aligned", what);
+    if (pb.max_seq > PK_MAX_KEYS) pb.max_seq = PK_MAX_KEYS;
     // the kernels count key granules of at least 32 per block of at least 16 query rows in 32 bits
     const double granules = (double)a.Hkv * ((double)pb.T * (a.Hq / a.Hkv) / 16 + pb.B) * (pb.max_seq / 32 + 1.0);
     SH_REQUIRE(granules < 2147483648.0 && (int64_t)pb.T * a.Hq <= INT32_MAX, "%s: %d tokens over max_seq=%d are too much for one call", what, pb.T,

@@ -9,6 +9,9 @@ namespace slate_hip {
 constexpr int PK_MAX_SEQ = 1024;       // sequences of a batch
 constexpr int PK_MAX_DRAFT = 1024;     // drafted tokens of a sequence
 constexpr int PK_MAX_HD = 512;
+// Keys that a sequence can have in the attention kernels, which round counts of
+// them up to 128 and step past the last ones in 32 bits.
+constexpr int PK_MAX_KEYS = INT32_MAX - 1023;
 constexpr int KV8_BLOCK = 32;          // elements that share a step
 
 struct PackedBatch {

@@ -270,6 +270,19 @@ def test_ragged_q8(hip, hd, Hkv, G, kind):
     r.check()
 
 
+@pytest.mark.parametrize("hd", [64, 96])
+@pytest.mark.parametrize("n", [1, 25])
+@pytest.mark.parametrize("kind", ["ragged", "tree_q8", "tree"])
+def test_no_limit_on_the_context(hip, kind, n, hd):
+    """max_seq = INT32_MAX, as a program without a limit passes it: blocks are cut and joined as with the true one."""
+    rng = np.random.default_rng(17)
+    bt = Batch([(5000, n), (700, 1)], 1, hd, 5100, rng)
+    r = Run(bt, 4, kind != "tree", 6, None if kind == "ragged" else random_parents(bt, rng, "random"))
+    bt.max_seq = 2 ** 31 - 1
+    r.call()
+    r.check()
+
+
 @pytest.mark.parametrize("B", [1, 65, 200])
 def test_ragged_q8_many_sequences(hip, B):
     rng = np.random.default_rng(B)
