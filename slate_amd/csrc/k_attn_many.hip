@@ -740,6 +740,9 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
 
 int64_t attention_many_bytes(int hd) { return plan_bytes(AM_WGS, AM_ROWS, hd); }
 bool attention_many_takes(const PackedAttn& a) { return a.hd == 32 || a.hd == 64 || a.hd == 128; }
+double attention_many_most(const PackedAttn& a, const PackedBatch& pb) {
+    return a.Hkv * ((double)pb.T * (a.Hq / a.Hkv) / AM_ROWS + pb.B) * ((pb.max_seq + AM_KEYS - 1) / AM_KEYS);
+}
 
 template <int HD>
 static void launch_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {

@@ -170,6 +170,13 @@ int64_t attention_packed_bytes(int Hq, int Hkv, int hd) {
     return max(attention_q8_few_bytes(hd), attention_many_bytes(hd));
 }
 
+bool attention_packed_fits(const PackedAttn& a, const PackedBatch& pb) {
+    const double most = attention_q8_few_takes(a, pb) ? attention_q8_few_most(a, pb)
+                        : attention_many_takes(a)     ? attention_many_most(a, pb)
+                                                      : 0;
+    return most < 2147483648.0;
+}
+
 int launch_attention_packed(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {
     if (attention_q8_few_takes(a, pb)) return launch_attention_q8_few(a, pb, s);
     if (attention_many_takes(a)) return launch_attention_many(a, pb, s);

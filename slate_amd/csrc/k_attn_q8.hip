@@ -236,6 +236,9 @@ bool attention_q8_few_takes(const PackedAttn& a, const PackedBatch& pb) {
     return !a.kf && (a.hd == 32 || a.hd == 64 || a.hd == 128) && pb.max_new <= AF_MAX_NEW &&
            pb.max_new * (int64_t)(a.Hq / a.Hkv) <= AF_MAX_ROWS;
 }
+double attention_q8_few_most(const PackedAttn& a, const PackedBatch& pb) {
+    return a.Hkv * ((double)pb.T * (a.Hq / a.Hkv) / AR_TILE + pb.B) * few_granules(pb.max_seq);
+}
 
 template <int HD>
 static void launch_few(const PackedAttn& a, const PackedBatch& pb, hipStream_t s) {

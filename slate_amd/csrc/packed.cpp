@@ -86,10 +86,8 @@ int attention_packed(const char* what, const PackedAttn& a, PackedBatch pb, bool
     SH_REQUIRE(!q8 || (aligned16(a.kv8.kq) && aligned16(a.kv8.ks) && aligned16(a.kv8.vq) && aligned16(a.kv8.vs)),
                "%s: pools are not 16-byte aligned", what);
     if (pb.max_seq > PK_MAX_KEYS) pb.max_seq = PK_MAX_KEYS;
-    // the kernels count key granules of at least 32 per block of at least 16 query rows in 32 bits
-    const double granules = (double)a.Hkv * ((double)pb.T * (a.Hq / a.Hkv) / 16 + pb.B) * (pb.max_seq / 32 + 1.0);
-    SH_REQUIRE(granules < 2147483648.0 && (int64_t)pb.T * a.Hq <= INT32_MAX, "%s: %d tokens over max_seq=%d are too much for one call", what, pb.T,
-               pb.max_seq);
+    SH_REQUIRE((int64_t)pb.T * a.Hq <= INT32_MAX - 127 && attention_packed_fits(a, pb),
+               "%s: %d tokens over max_seq=%d are too much for one call", what, pb.T, pb.max_seq);
     const size_t bytes = (size_t)pb.T * a.Hq * a.hd * sizeof(float);
     SH_REQUIRE(!overlap(a.out, bytes, a.q, bytes), "%s: out overlaps q", what);
     const size_t need = (size_t)attention_packed_bytes(a.Hq, a.Hkv, a.hd);

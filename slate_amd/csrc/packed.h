@@ -83,6 +83,11 @@ int launch_attention_q8_few(const PackedAttn& a, const PackedBatch& pb, hipStrea
 bool attention_many_takes(const PackedAttn& a);
 int64_t attention_many_bytes(int hd);
 int launch_attention_many(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
+// The most granules of keys that a call's blocks can have together; the kernels
+// count them in 32 bits.
+double attention_q8_few_most(const PackedAttn& a, const PackedBatch& pb);
+double attention_many_most(const PackedAttn& a, const PackedBatch& pb);
+bool attention_packed_fits(const PackedAttn& a, const PackedBatch& pb);
 int launch_attention_packed(const PackedAttn& a, const PackedBatch& pb, hipStream_t s);
 
 }  // namespace slate_hip

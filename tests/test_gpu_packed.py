@@ -311,6 +311,32 @@ def test_prompts_of_many_blocks(hip, G, seqs):
     r.check()
 
 
+def test_prompt_of_131072_tokens(hip):
+    """A whole long prompt in one call, 64 heads: a few of its rows against the reference.
+
+    With N(0, 1) values and weights of one size the sum over t keys is a random walk: its partial sums are at most
+    about as large as the result.  Each of the 2 t / 32 products that are added to it rounds it by up to 2^-24, with
+    independent signs sqrt(2 t / 32) 2^-24 in all (5.4e-6 for 131072 keys), besides what NORM_TOL stands for."""
+    n, hd, Hkv, G = 131072, 32, 8, 8
+    rng = np.random.default_rng(18)
+    bt = Batch([(0, n)], Hkv, hd, n, rng)
+    pools = fill_q8(bt, 6)
+    part = rng.normal(0, 1, (4096, Hkv * G, hd)).astype(np.float32)
+    q = np.concatenate([part] * (n // 4096))
+    flat = [DeviceBuffer.from_array(a) for name in "KV" for a in pools[name]]
+    qd, out = DeviceBuffer.from_array(q), DeviceBuffer(q.nbytes)
+    ok(lib().slate_hip_attention_ragged_q8(out.p, qd.p, *[d.p for d in flat], *bt.desc(), 1, n, n, Hkv * G, Hkv, hd,
+                                           bt.head_stride, n, None, 0))
+    got = out.to_array(np.float32, q.shape).astype(np.float64)
+    for h in range(Hkv):
+        K, V = (host_rows(bt, pools[name], 0, h, n) for name in "KV")
+        for t in (0, 1, 4095, 65536 + 17 * h, n - 1):
+            want, _, _ = pr.attend(q[t:t + 1, h * G:(h + 1) * G].astype(np.float64), K[:t + 1], V[:t + 1],
+                                   np.ones((1, t + 1), bool), hd)
+            err = np.linalg.norm(got[t, h * G:(h + 1) * G] - want) / np.linalg.norm(want)
+            assert err <= NORM_TOL + (2 * (t + 1) / 32) ** 0.5 * 2.0 ** -24, (h, t, err)
+
+
 def test_ragged_q8_bound_on_tokens(hip):
     """A sequence with more tokens than max_new is left out; the others are computed."""
     bt = Batch([(10, 1), (20, 5), (30, 2)], 1, 64, 64, np.random.default_rng(1))

@@ -154,6 +154,17 @@ def test_attention_accepts(no_device, kind):
         good(no_device, attn_call(no_device, kind, **kw))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_accepts_long_prompts(no_device, kind):
+    """Whole prompts and wide steps of long contexts stay far inside the 32 bits that the kernels count in."""
+    far = dict(q=A + (1 << 45))
+    for kw in (dict(T=131072, Hq=64, Hkv=8, max_seq=131072, max_new=131072 if kind == "ragged_q8" else 1024, **far),
+               dict(T=131072, Hq=64, Hkv=8, max_seq=1 << 20, max_new=1024, **far),
+               dict(T=16384, B=1024, Hq=64, Hkv=8, max_seq=1 << 17, max_new=16, **far)):
+        good(no_device, attn_call(no_device, kind, **kw))
+    assert attn_call(no_device, kind, T=131072, Hq=64, Hkv=8, max_seq=1 << 22, max_new=1024, **far) == -1
+
+
 def test_workspace_bytes(lib):
     f = lib.slate_hip_attention_packed_bytes
     assert f(32, 8, 128) >= 0 and f(7, 1, 16) >= 0
