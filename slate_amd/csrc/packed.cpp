@@ -27,7 +27,9 @@ bool rope_ok(const slate_hip_rope_t* r) {
     return r->scaling != 3 || r->theta_base > 1;
 }
 
-void rope_frequencies(double* w, double* magnitude, const slate_hip_rope_t* r) {
+// False where a frequency or the magnitude is too large for its type (an angle
+// of any position has to be a finite double).
+bool rope_frequencies(double* w, double* magnitude, const slate_hip_rope_t* r) {
     const int n = r->rot_dim / 2;
     double a = 0, b = 0;
     if (r->scaling == 3) {
@@ -35,6 +37,7 @@ void rope_frequencies(double* w, double* magnitude, const slate_hip_rope_t* r) {
         a = fmax(0.0, floor(per * log(r->orig_ctx / (r->high * TWO_PI))));
         b = fmin(r->rot_dim - 1.0, ceil(per * log(r->orig_ctx / (r->low * TWO_PI))));
     }
+    bool fine = true;
     const double per_pair = -2.0 * log(r->theta_base) / r->rot_dim;   // exp: a tenth of pow's time, within 2^-48
     for (int i = 0; i < n; ++i) {
         const double f = exp(per_pair * i);
@@ -43,9 +46,11 @@ void rope_frequencies(double* w, double* magnitude, const slate_hip_rope_t* r) {
         if (r->scaling == 2) slow = 1 - fmin(1.0, fmax(0.0, (r->orig_ctx * f / TWO_PI - r->low) / (r->high - r->low)));
         if (r->scaling == 3) slow = fmin(1.0, fmax(0.0, (i - a) / (b > a ? b - a : 0.001)));
         w[i] = slow == 0 ? f : slow * (f / r->factor) + (1 - slow) * f;
+        fine &= isfinite(w[i] * 2147483648.0) != 0;
     }
     *magnitude = r->magnitude != 0 ? r->magnitude
                                    : (r->scaling == 3 && r->factor > 1 ? 0.1 * log(r->factor) + 1 : 1.0);
+    return fine && isfinite((float)*magnitude);
 }
 
 // Whether the byte ranges [a, a + n) and [b, b + m) share a byte.
@@ -114,7 +119,7 @@ extern "C" {
 
 int slate_hip_rope_frequencies(double* w, double* magnitude, const slate_hip_rope_t* rope) {
     SH_REQUIRE(w && magnitude && rope_ok(rope), "rope_frequencies: bad arguments");
-    rope_frequencies(w, magnitude, rope);
+    SH_REQUIRE(rope_frequencies(w, magnitude, rope), "rope_frequencies: out of range");
     return 0;
 }
 
@@ -126,10 +131,10 @@ int slate_hip_rope_scaled(float* y, const float* x, const int32_t* pos, int n_ro
                (long long)ld);
     const size_t bytes = ((size_t)(n_rows - 1) * ld + (size_t)n_heads * head_dim) * sizeof(float);
     SH_REQUIRE(y == x || !overlap(y, bytes, x, bytes), "rope_scaled: y overlaps x");
-    if (!device_ok()) return -7;
     RopeTurns turns = {};
     double magnitude = 1;
-    rope_frequencies(turns.w, &magnitude, rope);
+    SH_REQUIRE(rope_frequencies(turns.w, &magnitude, rope), "rope_scaled: frequencies out of range");
+    if (!device_ok()) return -7;
     for (int i = 0; i < rope->rot_dim / 2; ++i) turns.w[i] /= TWO_PI;
     std::lock_guard<std::mutex> lk(g_enqueue_mu);
     return launch_rope_scaled(y, x, pos, n_rows, n_heads, head_dim, ld, rope->layout, rope->rot_dim, (float)magnitude,

@@ -61,6 +61,18 @@ def test_rope_refuses_configurations(lib, kw):
     assert "rope" in slate_amd.last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(scaling=1, factor=5e-324), dict(theta_base=1e-322, rot_dim=512),
+                                dict(scaling=3, factor=1e-320), dict(scaling=1, factor=1e-300), dict(magnitude=1e39),
+                                dict(magnitude=-1e300)])
+def test_rope_refuses_what_overflows(lib, kw):
+    """Frequencies whose angles, or a magnitude that, would be infinite."""
+    c = rope_cfg(**kw)
+    w, m = (C.c_double * 512)(), C.c_double()
+    assert lib.slate_hip_rope_frequencies(w, C.byref(m), C.byref(c)) == -1
+    assert lib.slate_hip_rope_scaled(A, A, A, 4, 2, 512, 1024, C.byref(c)) == -1
+    assert "out of range" in slate_amd.last_error()
+
+
 def good(lib, rc):
     """A call with these arguments passes the checks (it must not be made where it would run)."""
     assert rc == -7, slate_amd.last_error()
