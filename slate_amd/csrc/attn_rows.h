@@ -86,19 +86,9 @@ struct AttnRows {
     float pexp;                    // the weights are 2^(score - m + pexp)
     int lim;                       // the largest V step seen, as the caller orders them (0: none)
 
-    // Rows from q (row j at qp, or nothing there), scaled by `scale`
-    // and then to [2^13, 2^14) at the row's largest element: lo keeps its 11
-    // bits for any element within 2^-14 of that one.
-    __device__ __forceinline__ void start(const float* qp, bool live, float scale) {
-        const int g = (threadIdx.x & 63) >> 4;
-        float4u raw[NB][2];
-#pragma unroll
-        for (int t = 0; t < NB; ++t) {
-            raw[t][0] = *(const float4u*)(qp + 32 * t + 8 * g);
-            raw[t][1] = *(const float4u*)(qp + 32 * t + 8 * g + 4);
-        }
-        start(raw, live, scale);
-    }
+    // Rows from q (raw: elements 32t + 8g .. +7 of row j; not live: no row),
+    // scaled by `scale` and then to [2^13, 2^14) at the row's largest element:
+    // lo keeps its 11 bits for any element within 2^-14 of that one.
     __device__ __forceinline__ void start(const float4u (*raw)[2], bool live, float scale) {
         float v[NB][8], top = 0.f;
 #pragma unroll

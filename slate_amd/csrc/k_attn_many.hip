@@ -63,7 +63,6 @@ template <int HD, bool F32>
 struct ManyGeom {
     static constexpr int PLANE = AM_KEYS * HD;         // halves
     static constexpr int PLANES = F32 ? 4 : 2;         // K hi (lo), V hi (lo)
-    static constexpr int CH = HD / 8;                  // 8-element chunks of a row
     // what a thread brings in: 16 codes of a row, or 8 f32
     static constexpr int UNIT = F32 ? 8 : 16;
     static constexpr int UNITS = AM_KEYS * HD / UNIT;  // of K, and of V
