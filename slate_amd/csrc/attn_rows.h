@@ -83,7 +83,7 @@ struct AttnRows {
     floatx4 o[ND];                 // O^T: columns 16n + 4g .. +3 of row j
     float unq;                     // what undoes Q's scale
     float m, l;                // running maximum (log2), the lane's part of the sum
-    float pexp;                    // the weights are 2^(score - m + pexp)
+    float pexp;                    // the weights are 2^(score - m + pexp), or 2^(score - m) where it is kept APART
     int lim;                       // the largest V step seen, as the caller orders them (0: none)
 
     // Rows from q (raw: elements 32t + 8g .. +7 of row j; not live: no row),
@@ -119,7 +119,9 @@ struct AttnRows {
     // -inf: not seen).  big: the largest V step, in the lane's own keys
     // (EACH) or in any lane; exponent(big): e with that step in [2^(e-1), 2^e).
     // shift: powers of two that the weights of each 32 keys get besides (none: nullptr).
-    template <int H, bool EACH, class Exponent>
+    // APART: the caller's steps take 2^pexp.  f32 rows may be of any size, pexp
+    // up to 100, and an exponent of 64 or more keeps but 17 bits behind its point.
+    template <int H, bool EACH, bool APART = false, class Exponent>
     __device__ __forceinline__ void weights(const floatx4* s, int big, const Exponent& exponent, float* p,
                                             const int* shift = nullptr) {
         float mx = s[0][0];
@@ -130,6 +132,7 @@ struct AttnRows {
             const float mn = fmaxf(m, cols_max(mx));
             float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
+            if (APART) l *= f;
             if (__builtin_amdgcn_ballot_w64(big > lim)) {
                 if (!EACH)
 #pragma unroll
@@ -143,11 +146,11 @@ struct AttnRows {
                     pexp = pe;
                 }
             }
-            l *= f;
+            if (!APART) l *= f;
 #pragma unroll
             for (int n = 0; n < ND; ++n) o[n] *= f;
         }
-        const float mref = pexp - (m == -INFINITY ? 0.f : m);
+        const float mref = (APART ? 0.f : pexp) - (m == -INFINITY ? 0.f : m);
 #pragma unroll
         for (int b = 0; b < H / 2; ++b) {
             const float by = shift ? mref + (float)shift[b] : mref;
@@ -161,9 +164,10 @@ struct AttnRows {
         }
     }
 
-    // What undoes the weights' scale, and its sum over the keys without it.
+    // What undoes the weights' scale, and their sum over the keys without it.
     __device__ __forceinline__ float back() const { return __builtin_amdgcn_exp2f(-pexp); }
-    __device__ __forceinline__ float sum() const { return cols_sum(l) * back(); }
+    template <bool APART = false>
+    __device__ __forceinline__ float sum() const { return cols_sum(l) * (APART ? 1.0f : back()); }
 };
 
 }  // namespace slate_hip

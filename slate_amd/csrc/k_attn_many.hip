@@ -274,11 +274,12 @@ struct ManyRows : AttnRows<HD> {
                 if (!sees(e)) s[e >> 2][e & 3] = -INFINITY;
                 if (sees(e)) big = max(big, __builtin_bit_cast(int, step));
             }
-            this->template weights<H, true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
+            this->template weights<H, true, true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
+            const float by = __builtin_amdgcn_exp2f(this->pexp);
 #pragma unroll
             for (int b = 0; b < H / 2; ++b) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = p[8 * b + e] * (sees(e) ? d[2 * b + (e >> 2)][e & 3] : 0.f);
+                for (int e = 0; e < 8; ++e) x[e] = p[8 * b + e] * (sees(e) ? d[2 * b + (e >> 2)][e & 3] * by : 0.f);
                 halves(x, ph, pl);
 #pragma unroll
                 for (int n = 0; n < ND; ++n) {
@@ -685,7 +686,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
         }
         const bool whole = pc.g0 == 0 && pc.g1 == pc.gran;
         const float back = R.back();
-        float l = R.sum();
+        float l = R.template sum<F32>();
 #pragma unroll
         for (int n = 0; n < ND; ++n) R.o[n] *= back;
         if (sh.parts > 1) {                            // the parts of the keys joined

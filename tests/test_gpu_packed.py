@@ -541,6 +541,20 @@ def test_tree_all_rows_zero(hip, hd, n):
     check_beside_zero_rows(r)
 
 
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -20, 2.0 ** -41, 2.0 ** -70, 2.0 ** 80])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_tree_weights_do_not_go_by_the_size_of_v(hip, hd, scale):
+    """Few keys of small scores, where the bound on a weight is a few 2^-22: it holds at any size of V."""
+    rng = np.random.default_rng(hd)
+    bt = Batch([(2, 6), (0, 3), (5, 1), (0, 12), (1, 4), (3, 2)] * 8, 2, hd, 16, rng)
+    pools = fill_f32(bt, 5)
+    pools["K"] *= np.float32(2.0 ** -8)
+    pools["V"] *= np.float32(scale)
+    r = Run(bt, 3, False, 5, random_parents(bt, rng, "random"), pools=pools)
+    r.call()
+    r.check()
+
+
 @pytest.mark.parametrize("order", ["mixed", "rising", "falling", "one"])
 @pytest.mark.parametrize("hd,G,n", [(128, 4, 5), (128, 4, 40), (64, 8, 33), (32, 2, 70)])
 def test_tree_rows_of_all_sizes(hip, hd, G, n, order):
