@@ -121,6 +121,9 @@ struct Q8Rows : AttnRows<HD> {
         }
         float p[8];
         this->template weights<2, MASKED>(s, big, step_exponent, p);
+        const float by = __builtin_amdgcn_exp2f(this->pexp);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] *= by;
         // the transposing read: lane j of a group names half (j & 1) of the 16
         // columns of the key of slot 8g + j / 2 (slot 8g + e is the lane's e-th key)
         const int tkey = 16 * (j >> 3) + 4 * g + ((j >> 1) & 3);

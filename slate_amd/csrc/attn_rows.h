@@ -83,7 +83,7 @@ struct AttnRows {
     floatx4 o[ND];                 // O^T: columns 16n + 4g .. +3 of row j
     float unq;                     // what undoes Q's scale
     float m, l;                // running maximum (log2), the lane's part of the sum
-    float pexp;                    // the weights are 2^(score - m + pexp), or 2^(score - m) where it is kept APART
+    float pexp;                    // o is 2^pexp times what l and m say
     int lim;                       // the largest V step seen, as the caller orders them (0: none)
 
     // Rows from q (raw: elements 32t + 8g .. +7 of row j; not live: no row),
@@ -115,13 +115,14 @@ struct AttnRows {
         lim = 0;
     }
 
-    // The weights p of the lane's 4 H scores s (keys 16 hf + 4g + i of row j;
+    // The weights p = 2^(score - m) of the lane's 4 H scores s (keys 16 hf + 4g + i of row j;
     // -inf: not seen).  big: the largest V step, in the lane's own keys
     // (EACH) or in any lane; exponent(big): e with that step in [2^(e-1), 2^e).
-    // shift: powers of two that the weights of each 32 keys get besides (none: nullptr).
-    // APART: the caller's steps take 2^pexp.  f32 rows may be of any size, pexp
-    // up to 100, and an exponent of 64 or more keeps but 17 bits behind its point.
-    template <int H, bool EACH, bool APART = false, class Exponent>
+    // The caller multiplies them, or the steps, by 2^pexp: an exponent of 64 or
+    // more (V may be of any size, pexp is up to 100) would keep but 17 bits behind
+    // its point.  Or p has the powers of two pexp + shift[i] in it, 11 at most,
+    // for each 32 keys.
+    template <int H, bool EACH, class Exponent>
     __device__ __forceinline__ void weights(const floatx4* s, int big, const Exponent& exponent, float* p,
                                             const int* shift = nullptr) {
         float mx = s[0][0];
@@ -132,7 +133,7 @@ struct AttnRows {
             const float mn = fmaxf(m, cols_max(mx));
             float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
-            if (APART) l *= f;
+            l *= f;
             if (__builtin_amdgcn_ballot_w64(big > lim)) {
                 if (!EACH)
 #pragma unroll
@@ -146,28 +147,27 @@ struct AttnRows {
                     pexp = pe;
                 }
             }
-            if (!APART) l *= f;
 #pragma unroll
             for (int n = 0; n < ND; ++n) o[n] *= f;
         }
-        const float mref = (APART ? 0.f : pexp) - (m == -INFINITY ? 0.f : m);
+        const float mref = m == -INFINITY ? 0.f : -m;
 #pragma unroll
         for (int b = 0; b < H / 2; ++b) {
-            const float by = shift ? mref + (float)shift[b] : mref;
+            const float k = shift ? pexp + (float)shift[b] : 0.f;
+            const float by = mref + k;
             float sum = 0.f;
 #pragma unroll
             for (int e = 8 * b; e < 8 * b + 8; ++e) {
                 p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], unq, by));
                 (shift ? sum : l) += p[e];
             }
-            if (shift) l += ldexpf(sum, -shift[b]);
+            if (shift) l += ldexpf(sum, -(int)k);
         }
     }
 
-    // What undoes the weights' scale, and their sum over the keys without it.
+    // What undoes o's scale, and the sum of the weights over the keys.
     __device__ __forceinline__ float back() const { return __builtin_amdgcn_exp2f(-pexp); }
-    template <bool APART = false>
-    __device__ __forceinline__ float sum() const { return cols_sum(l) * (APART ? 1.0f : back()); }
+    __device__ __forceinline__ float sum() const { return cols_sum(l); }
 };
 
 }  // namespace slate_hip

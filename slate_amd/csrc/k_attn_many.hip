@@ -274,7 +274,7 @@ struct ManyRows : AttnRows<HD> {
                 if (!sees(e)) s[e >> 2][e & 3] = -INFINITY;
                 if (sees(e)) big = max(big, __builtin_bit_cast(int, step));
             }
-            this->template weights<H, true, true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
+            this->template weights<H, true>(s, big, [](int b) { return (b >> 23) - 126; }, p);
             const float by = __builtin_amdgcn_exp2f(this->pexp);
 #pragma unroll
             for (int b = 0; b < H / 2; ++b) {
@@ -331,6 +331,9 @@ struct ManyRows : AttnRows<HD> {
             };
             if constexpr (MASKED) {
                 this->template weights<H, true>(s, big, step_exponent, p);
+                const float by = __builtin_amdgcn_exp2f(this->pexp);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] *= by;
                 Steps dv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dv[e] = vs[16 * (e >> 2) + 4 * g + (e & 3)];
@@ -686,7 +689,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
         }
         const bool whole = pc.g0 == 0 && pc.g1 == pc.gran;
         const float back = R.back();
-        float l = R.template sum<F32>();
+        float l = R.sum();
 #pragma unroll
         for (int n = 0; n < ND; ++n) R.o[n] *= back;
         if (sh.parts > 1) {                            // the parts of the keys joined

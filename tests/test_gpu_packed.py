@@ -555,6 +555,24 @@ def test_tree_weights_do_not_go_by_the_size_of_v(hip, hd, scale):
     r.check()
 
 
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -6, 2.0 ** -14, 2.0 ** -17, 2.0 ** 10])
+@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_q8_weights_do_not_go_by_the_size_of_v(hip, hd, n, scale):
+    """The same over the 8-bit cache, whose steps end at 2^-24."""
+    rng = np.random.default_rng(hd)
+    few = [(1, 1), (1, 1), (2, 1), (3, 1)] * 8
+    bt = Batch(few + [(2, min(n, 5)), (0, min(n, 3)), (5, 1), (70, 1), (1, min(n, 4)), (35, n)] * 4, 2, hd, 80, rng)
+    pools = fill_q8(bt, 5)
+    for name, by in (("K", 2.0 ** -8), ("V", scale)):
+        st = pools[name][1]
+        st[:] = (st.astype(np.float64) * by).astype(np.float16)
+    for parent in (None, random_parents(bt, rng, "random")):
+        r = Run(bt, 3, True, 5, parent, pools=pools)
+        r.call()
+        r.check()
+
+
 @pytest.mark.parametrize("order", ["mixed", "rising", "falling", "one"])
 @pytest.mark.parametrize("hd,G,n", [(128, 4, 5), (128, 4, 40), (64, 8, 33), (32, 2, 70)])
 def test_tree_rows_of_all_sizes(hip, hd, G, n, order):
