@@ -276,9 +276,14 @@ int   slate_hip_kv_load_q8(float* k, float* v, int64_t ld, const int8_t* Kq, con
  * Scores are q.k / sqrt(head_dim), as attention_ragged's.  max_new bounds the
  * tokens that one sequence brings (1 for a decode step); head_dim is at most
  * 512; 32, 64 and 128 run on the matrix instructions, the others on a plain
- * kernel.  Queries must be finite and, like the cache's values, below 2^100
- * in size (f32 values are resolved to 2^-22 of their row's largest, and to
- * 2^-114).  What the cache holds in rows a token does not see never matters.
+ * kernel in f32.  Queries must be finite and, like the cache's values, below
+ * 2^100 in size.  On the matrix instructions queries, weights and f32 values
+ * have 22 bits, sums are f32, and V counts by what is largest in it: an f32
+ * value is resolved to 2^-22 of its row's largest (and to 2^-114), an 8-bit one
+ * to 2^-24 of the largest in the 32 cache rows around it, and what a key adds to
+ * the sum to 2^-33 of the largest weight times the largest V of all keys seen,
+ * also where that V has no weight.  What the cache holds in rows a token does
+ * not see never matters.
  * T * n_q_heads <= 2^31 - 128, and the kernels count blocks of query rows times pieces
  * of keys in 32 bits: where n_kv_heads * (T * n_q_heads / n_kv_heads / 128 + B)
  * * max_seq / 64 (or, for max_new * n_q_heads / n_kv_heads <= 80 and max_new

@@ -573,6 +573,43 @@ def test_q8_weights_do_not_go_by_the_size_of_v(hip, hd, n, scale):
         r.check()
 
 
+@pytest.mark.parametrize("ratio", [2.0 ** 6, 2.0 ** 10])
+@pytest.mark.parametrize("hd,G,n", [(128, 4, 1), (128, 4, 40), (64, 8, 33), (32, 2, 12)])
+def test_large_v_rows_without_weight(hip, hd, G, n, ratio):
+    """One key in ten has V `ratio` times as large and, by its K, a weight below 2^-60: what the others give is still
+    held to 2^-18 of itself.  Each weight is resolved to 2^-33 of the largest weight times the largest V seen: 2^-23 of
+    the others here, and their errors are independent."""
+    rng = np.random.default_rng(n)
+    bt = Batch([(600, n), (0, n), (77, max(1, n - 3))], 2, hd, 700, rng)
+    for kind in ("ragged", "tree_q8", "tree"):
+        q8 = kind != "tree"
+        pools = fill_f32(bt, 8)
+        for b, (p, m) in enumerate(bt.seqs):
+            for h in range(bt.Hkv):
+                at, rows = bt.row(b, h, 0), p + m
+                K, V = (pools[x][at:at + rows * hd].reshape(rows, hd) for x in "KV")
+                big = rng.random(rows) < 0.1
+                big[:max(1, p)][0] = False             # a root sees a key with weight
+                big[p:] = False
+                K[:, 0] = np.where(big, -6 * np.sqrt(hd), 0.0)
+                V[big] *= np.float32(ratio)
+        if q8:
+            full = fill_q8(bt, 8)
+            for x in "KV":
+                for b, (p, m) in enumerate(bt.seqs):
+                    for h in range(bt.Hkv):
+                        at, size = bt.row(b, h, 0), (p + m) * hd
+                        cq, cs = pr.quantise(pools[x][at:at + size].reshape(-1, hd))
+                        full[x][0][at:at + size] = cq.reshape(-1)
+                        full[x][1][at // 32:(at + size) // 32] = cs.reshape(-1)
+            pools = full
+        r = Run(bt, G, q8, 8, None if kind == "ragged" else random_parents(bt, rng, "random"), pools=pools)
+        r.q[:, :, 0] = 9.0
+        r.qd.upload(r.q)
+        r.call()
+        r.check()
+
+
 @pytest.mark.parametrize("order", ["mixed", "rising", "falling", "one"])
 @pytest.mark.parametrize("hd,G,n", [(128, 4, 5), (128, 4, 40), (64, 8, 33), (32, 2, 70)])
 def test_tree_rows_of_all_sizes(hip, hd, G, n, order):
