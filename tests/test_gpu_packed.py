@@ -865,6 +865,39 @@ def test_kv_codes_at_every_tie(hip):
     assert np.array_equal(host["K"][1][at // 32:at // 32 + 2 * n].view(np.uint16), cs.reshape(-1).view(np.uint16))
 
 
+def test_kv_steps_next_to_ties(hip):
+    """The step is f16(max / 127) with one rounding: maxima at and next to 127 times each kind of f16 tie (a quotient
+    taken as a product with 1 / 127 lands on the wrong side of some, 1.9853441 among them)."""
+    rng = np.random.default_rng(6)
+    bits = np.concatenate([np.arange(1, 64), rng.integers(64, 0x7bfe, 1500), [0x7bfe]]).astype(np.uint16)
+    low, high = (b.view(np.float16).astype(np.float64) for b in (bits, bits + np.uint16(1)))
+    tie = 127.0 * (low + high) / 2                     # exact: 12 bits times 7
+    tops, want = [], []
+    for by in (-2, -1, 0, 1, 2):
+        t = tie.astype(np.float32)
+        for _ in range(abs(by)):
+            t = np.nextafter(t, np.float32(np.inf) if by > 0 else np.float32(0))
+        up = (t > tie) | ((t == tie) & (bits % 2 == 1))
+        tops.append(t)
+        want.append(bits + up.astype(np.uint16))
+    more = np.array([1.9853441, 1.9892198, 3.9706881, 3.9939425], np.float32)
+    tops = np.concatenate(tops + [more])
+    want = np.concatenate(want + [(more.astype(np.float64) / 127).astype(np.float16).view(np.uint16)])
+    n = -(-len(tops) // 2)
+    k = np.zeros((n, 64), np.float32)
+    k.reshape(-1, 32)[:len(tops), 7] = tops * rng.choice([-1, 1], len(tops)).astype(np.float32)
+    k.reshape(-1, 32)[:len(tops), 20] = tops / np.float32(3)
+    bt = Batch([(0, n)], 1, 64, n, rng)
+    host, back = store_load(bt, k, k, 64)
+    at = bt.row(0, 0, 0)
+    for name in "KV":
+        got = host[name][1][at // 32:at // 32 + len(tops)].view(np.uint16)
+        assert np.array_equal(got, want), (tops[got != want][:5], got[got != want][:5], want[got != want][:5])
+    cq, cs = pr.quantise(k)
+    assert np.array_equal(host["K"][0][at:at + n * 64], cq.reshape(-1))
+    assert np.array_equal(back[0], pr.values(cq, cs).astype(np.float32))
+
+
 # -- offsets, streams, graphs, threads ----------------------------------------------
 @pytest.mark.parametrize("q8", [False, True])
 def test_offsets_past_32_bits(hip, q8):
