@@ -494,8 +494,8 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             st = *(const Steps*)((tid < KEYS ? a.kv8.ks : a.kv8.vs) + r);
         }
     };
-    // and into LDS; `masked`: some row may not see some key of it
-    auto put = [&](int to, int ring, bool masked) {
+    // and into LDS; some row may not see its keys from `all` on
+    auto put = [&](int to, int ring, int all) {
         _Float16* rows = s_rows[to];
         if (mine) {
 #pragma unroll
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
                         float x[8], top = 0.f;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x[e] = f32[kv][u][e >> 2][e & 3];
-                        if (kv == 1 && masked) {
+                        if (kv == 1 && key >= all) {
                             bool bad = false;
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
             }
         }
     };
-    auto put_piece = [&](const Piece& p, int gr, int to, int ring) { put(to, ring, (gr + 1) * KEYS > p.open); };
+    auto put_piece = [&](const Piece& p, int gr, int to, int ring) { put(to, ring, p.open - gr * KEYS); };
 
     // How a block's rows go to the waves: tiles of 16 rows, each taken by
     // W / tiles waves, which share the keys 32 by 32.

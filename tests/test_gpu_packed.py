@@ -752,6 +752,23 @@ def test_tree_values_a_token_does_not_see(hip, q8):
         assert err <= NORM_TOL
 
 
+@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("row", [0, 31, 35, 39])
+def test_tree_committed_values_that_are_not_finite(hip, n, row):
+    """A committed V row that is not finite reaches every token of its sequence and kv head, and no other, wherever
+    it lies among the drafts' keys."""
+    rng = np.random.default_rng(row)
+    bt = Batch([(40, n), (50, 2)], 2, 64, 100, rng)
+    pools = fill_f32(bt, 3)
+    at = bt.row(0, 1, row)
+    pools["V"][at:at + 64] = np.nan
+    r = Run(bt, 2, False, 3, random_parents(bt, rng, "random"), pools=pools)
+    r.call()
+    out = r.result()
+    assert np.isnan(out[:n, 2:]).all()
+    assert np.isfinite(out[:n, :2]).all() and np.isfinite(out[n:]).all()
+
+
 def test_attention_large_scores(hip):
     """Scores of thousands (a channel of K far above the others) and queries and keys far from 1."""
     rng = np.random.default_rng(9)
