@@ -286,7 +286,7 @@ int   slate_hip_kv_load_q8(float* k, float* v, int64_t ld, const int8_t* Kq, con
  * not see never matters.
  * T * n_q_heads <= 2^31 - 128, and the kernels count blocks of query rows times pieces
  * of keys in 32 bits: where n_kv_heads * (T * n_q_heads / n_kv_heads / 128 + B)
- * * max_seq / 64 (or, for max_new * n_q_heads / n_kv_heads <= 80 and max_new
+ * * max_seq / 64 (or, for max_new * n_q_heads / n_kv_heads <= 48 and max_new
  * <= 32, / 16 and / 128) reaches 2^31 the call is refused.
  * ws: device scratch of slate_hip_attention_packed_bytes, 16-byte aligned,
  * its content of no matter, for calls that run beside each other or are

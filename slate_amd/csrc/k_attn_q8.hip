@@ -1,6 +1,6 @@
 // k_attn_q8.hip -- attention over the 8-bit cache for few query rows per
 // (sequence, kv head): a decode step's tokens times the query heads of a kv
-// head, trees of up to 80 rows.  The arithmetic: attn_q8.h, how the keys are
+// head, trees of up to 48 rows.  The arithmetic: attn_q8.h, how the keys are
 // shared out: attn_plan.h.
 //
 // A workgroup takes a block of 16 rows over a range of keys, each of its four
@@ -226,12 +226,16 @@ __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(PackedAttn a, Packe
 // ---------------------------------------------------------------------------
 int64_t attention_q8_few_bytes(int hd) { return plan_bytes(AF_WGS, AR_TILE, hd); }
 // Blocks of 16 rows read the keys again for every block, but without a
-// barrier: 48 rows (12 drafts, 4 heads a kv head, 16 sequences of up to 4096)
-// 56 us here and 64 in the many-row kernel, 80 rows 77 and 80, 96 rows 87 and
-// 81; 64 sequences of up to 2000 107 and 123, 144 and 144, 173 and 152; of
-// head_dim 64 36 and 44, 49 and 50, 55 and 51; one sequence of 16384 39 and 35,
-// 47 and 43, 47 and 43.  A row's drafts are kept in 32 bits.
-constexpr int AF_MAX_ROWS = 80, AF_MAX_NEW = 32;
+// barrier.  us here and in the many-row kernel (head_dim 128, 4 query heads a kv
+// head, trees of max_new drafts each, in brackets of half as many to max_new):
+// 16 sequences of up to 4096: 32 rows 49 and 58, 48 rows 64 and 64 (55 and 62),
+// 64 rows 81 and 72 (69 and 69), 80 rows 93 and 77 (78 and 76); 64 sequences of up
+// to 2000: 32 rows 84 and 111, 48 rows 128 and 126 (108 and 121), 64 rows 148 and
+// 127 (121 and 123); head_dim 64: 48 rows 42 and 45, 64 rows 51 and 49.  One
+// sequence of 16384 goes faster there at any number of rows but 64 (20 rows 32
+// and 31, 48 rows 40 and 34): the rule, which knows a bound on the rows and no
+// lengths, leaves that.  A row's drafts are kept in 32 bits.
+constexpr int AF_MAX_ROWS = 48, AF_MAX_NEW = 32;
 bool attention_q8_few_takes(const PackedAttn& a, const PackedBatch& pb) {
     return !a.kf && (a.hd == 32 || a.hd == 64 || a.hd == 128) && pb.max_new <= AF_MAX_NEW &&
            pb.max_new * (int64_t)(a.Hq / a.Hkv) <= AF_MAX_ROWS;

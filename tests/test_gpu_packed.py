@@ -671,6 +671,19 @@ def test_rows_around_the_kernels_border(hip, G, n):
         r.check()
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("G,n", [(3, 16), (3, 17), (4, 12), (4, 13), (12, 4), (7, 6), (7, 7), (16, 3), (16, 4), (48, 1),
+                                 (49, 1), (1, 31), (2, 24), (2, 25)])
+def test_rows_around_48(hip, G, n, hd):
+    """Up to 48 query rows per kv head (and 32 tokens) one kernel takes a batch, from there on another."""
+    rng = np.random.default_rng(19)
+    bt = Batch([(700, n), (31, max(1, n - 1)), (5, 1)], 1, hd, 800, rng)
+    for kind in ("causal", "tree"):
+        r = Run(bt, G, True, 6, random_parents(bt, rng, "random") if kind == "tree" else None)
+        r.call()
+        r.check()
+
+
 def random_parents(bt, rng, kind):
     out = np.full(bt.T, -1, np.int32)
     for b in range(bt.B):
