@@ -5,11 +5,12 @@
 //
 // K and V come as f16 numbers times a power of two or a step each (per key, or
 // per key and 32 elements).  Q and P are split into two halves, hi = f16(x)
-// and lo = f16(x - hi), 22 bits in all, so nothing is rounded to fewer bits
-// than that.  Softmax, sums and steps are f32.  A row's running maximum moves
-// only when a score passes it by 2^4, so weights reach 2^4; they carry a
-// power of two by the largest V step seen, so that weight times step stays
-// inside f16's range whatever V's size is.
+// and lo = f16(x - hi), 22 bits in all.  Softmax, sums and steps are f32 (but
+// V's steps of 32 keys that all rows see, f16 relative to the largest of them: 11
+// bits like the steps themselves down to 2^-14 of it, and 2^-25 of it below).
+// A row's running maximum moves only when a score passes it by 2^4, so weights
+// reach 2^4; weight times step carries a power of two by the largest V step seen,
+// so that it stays inside f16's range whatever V's size is.
 #pragma once
 #include "lanes.h"
 #include "mfma.h"

@@ -13,14 +13,17 @@
 //   f32: a row of K or V is scaled by a power of two to [2^13, 2^14) at its
 //       largest element and split into halves hi + lo of 22 bits; three MFMAs
 //       a product (lo * lo is below what f32 sums keep).
-// What bounds it: over the 8-bit cache the vector unit (58 % of the cycles:
-// products by steps, the weights and their halves, the conversion; MFMA 30 %,
-// LDS 44 %, a third of the waves' time waits, most for the stage's barrier),
-// over f32 pools the bytes.  Head_dim 128, 8 kv heads: a mixed step of 13
-// decoding users and three 1024-token chunks 345 us (252 TFLOP/s), one
-// 4096-token prompt 321 us, 4 users' 64-token trees over 9000 keys 225 us
-// (325 TFLOP/s); 16 users' 26-token trees over 645 MB of f32 caches 159 us
-// (4.1 TB/s).  12 or 16 waves, or two tiles a wave, do not fit the registers.
+// What bounds it: over the 8-bit cache no unit by itself.  The vector unit is
+// busy in 57 % of the cycles (products by steps, the weights and their halves,
+// the conversion), the matrix unit in 27 % (causal) and 30 % (trees), LDS in 41
+// and 43 %, and a wave waits in 36 % of its cycles, most for the stage's barrier.
+// Over f32 pools it is the bytes.  Head_dim 128, 8 kv heads: a mixed step of 13
+// decoding users and three chunks of 714 to 839 tokens 347 us (251 TFLOP/s), a
+// whole prompt of 4096 tokens 478 us (287 TFLOP/s), 4 users' trees of 32 to 61
+// drafts over 48000 keys 230 us (319 TFLOP/s); 16 users' trees of 14 to 24
+// drafts over 645 MB of f32 caches 164 us (3.9 TB/s; 158 on the fastest of the
+// machines it was timed on).  12 or 16 waves, or two tiles a wave, do not fit
+// the registers.
 // Rows stay as they are stored, [key][element]: V^T comes out of LDS by the
 // transposing read.  16-byte chunks of a row are permuted, chunk c of key k
 // at place c ^ turn(k), so that both kinds of reads spread over the banks.

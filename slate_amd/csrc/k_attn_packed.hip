@@ -13,7 +13,7 @@ namespace slate_hip {
 // wave, joined at the end.  It serves the head_dims that the matrix kernels do
 // not take (other than 32, 64, 128).  Every query row reads its keys for
 // itself, out of L2: a decode step of 16 users at head_dim 128 took it 1155 us
-// where the few-row kernel takes 27.
+// where the few-row kernel takes 27.5.
 __global__ __launch_bounds__(256) void attn_packed_rows_kernel(PackedAttn a, PackedBatch pb) {
     __shared__ uint32_t s_seen[PK_MAX_DRAFT / 32];
     __shared__ float s_o[4][PK_MAX_HD], s_m[4], s_l[4];

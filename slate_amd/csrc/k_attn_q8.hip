@@ -10,9 +10,10 @@
 // each wave copies its next 32 keys' rows straight into LDS (16 bytes per
 // lane, no registers) while it works on the last 32, with no barrier until
 // its range ends; 70 KB are on their way per CU.  Head_dim 128, 8 kv heads of
-// 4 query heads: decode of 64 users over 1.33 GB in 243 us (5.4 TB/s), of 16
-// users over 79 MB in 27 us (its loads alone take 22, plan and join the
-// rest), trees of 8 tokens (two blocks, the keys read twice) of 16 users 44 us.
+// 4 query heads: decode of 64 users over 1.33 GB in 245 us (5.4 TB/s), of 16
+// users over 79 MB in 27.5 us (its loads alone take 22, plan and join the
+// rest), trees of 4 to 8 drafts (up to two blocks, the keys read again for the
+// second) of 16 users 43.4 us.
 #include "attn_plan.h"
 #include "attn_q8.h"
 

@@ -5,9 +5,9 @@
 //
 // Eight lanes share a block of 32 elements, four of them each: the maximum
 // stays inside a DPP row, loads and stores are whole lines.  Memory bound: K
-// and V rows of about 5000 tokens (8 heads of 128) are stored in 16 us (52 MB
-// read and written, 3.3 TB/s; a store per token and exact divisions took 21)
-// and loaded in 13.5 us (3.9 TB/s); rows of 16 tokens in 3 us each, launch and
+// and V rows of 5592 tokens (8 heads of 128) are stored in 16.4 us (58 MB
+// read and written, 3.5 TB/s; a store per token and exact divisions took 21)
+// and loaded in 13.3 us (4.4 TB/s); rows of 16 tokens in 3 us each, launch and
 // two rounds of load latency.
 #include "lanes.h"
 #include "packed.h"
@@ -17,10 +17,13 @@ namespace slate_hip {
 constexpr int KV8_THREADS = 256;
 
 // x / step rounded to nearest even within -127 .. 127 (step > 0 an f16 number,
-// inv its reciprocal within 2^-23, |x| at most about 178 step).  x inv is off
-// the quotient by less than 2^-14, so it rounds the same way unless it lies
+// inv its reciprocal within 2^-23).  |x| is at most 190.5 steps (max / 127 just
+// below 1.5 * 2^-24 becomes a step of 2^-24), so x inv is off the quotient by
+// less than 2^-14 and rounds the same way unless it lies
 // that close to a tie; there the remainder x - n step, which fma gives without
-// error (n has 8 bits, step 11), says on which side of the tie x is.
+// error (n has 8 bits, step 11), says on which side of the tie x is.  Where the
+// step was limited to 65504, or x is infinite, |x| can be anything above: what
+// is 127 steps or more ends at the clamp either way.
 __device__ __forceinline__ int code_of(float x, float step, float inv) {
     const float t = x * inv;
     float n = rintf(t);
@@ -160,7 +163,8 @@ __global__ __launch_bounds__(KV8_THREADS) void kv_load_q8_kernel(float* __restri
 }
 
 // Tokens of a workgroup: few tokens are spread over workgroups, many share the
-// descriptors' latency.
+// descriptors' latency.  Storing and loading 5592 tokens takes 39.4 us with one a
+// workgroup, 32.9 with 2, 33.2 with 4 and 38.1 with 8.
 constexpr int KV8_TOK = 4;
 static bool kv8_one(const PackedBatch& pb) { return pb.T < 1024; }
 
