@@ -610,6 +610,39 @@ def test_large_v_rows_without_weight(hip, hd, G, n, ratio):
         r.check()
 
 
+@pytest.mark.parametrize("kind", ["ragged", "tree_q8", "tree"])
+@pytest.mark.parametrize("hd,G,n", [(64, 8, 1), (128, 4, 40), (64, 8, 33)])
+def test_small_columns_beside_large_ones(hip, hd, G, n, kind):
+    """32 columns of V 2^16 times as large as the others.  A value is resolved to 2^-24 of the largest around it (f32:
+    2^-22 of itself or far less), what a key adds to 2^-33 of the largest V; the weights' own errors count against the
+    column.  So a small column is off by at most 2^-23 of the largest V and the usual bound times its own values."""
+    rng = np.random.default_rng(n)
+    bt = Batch([(300, n), (64, max(1, n - 3))], 1, hd, 400, rng)
+    q8 = kind != "tree"
+    pools = (fill_q8 if q8 else fill_f32)(bt, 8)
+    x = pools["V"][1] if q8 else pools["V"]
+    for b, (p, m) in enumerate(bt.seqs):
+        at, per = bt.row(b, 0, 0) // (32 if q8 else 1), hd // 32 if q8 else hd
+        v = x[at:at + (p + m) * per].reshape(p + m, per)
+        large = slice(0, 1) if q8 else slice(0, 32)
+        v[:] = (v.astype(np.float64) * 2.0 ** -6).astype(x.dtype)
+        v[:, large] = (v[:, large].astype(np.float64) * 2.0 ** 16).astype(x.dtype)
+    parent = None if kind == "ragged" else random_parents(bt, rng, "random")
+    r = Run(bt, G, q8, 8, parent, pools=pools)
+    r.call()
+    r.check()
+    out = r.result().astype(np.float64)
+    for b, (p, m) in enumerate(bt.seqs):
+        tk = list(bt.tokens(b))
+        sees = np.ones((m, p + m), bool)
+        sees[:, p:] = np.tril(np.ones((m, m), bool)) if parent is None else pr.ancestors(parent[tk])
+        K, V = (host_rows(bt, pools[name], b, 0, p + m) for name in "KV")
+        want, A, top = pr.attend(r.q[tk].astype(np.float64), K, V, sees, hd)
+        tol = 2 * ((2.0 ** -21 + hd * 2.0 ** -24) * A + 2.0 ** -22 * top) + 2.0 ** -22 + (p + m) * 2.0 ** -24
+        err = np.abs(out[tk] - want)[:, :, 32:].max()
+        assert err <= 2.0 ** -23 * np.abs(V).max() + tol * np.abs(V[:, 32:]).max(), (b, err)
+
+
 @pytest.mark.parametrize("order", ["mixed", "rising", "falling", "one"])
 @pytest.mark.parametrize("hd,G,n", [(128, 4, 5), (128, 4, 40), (64, 8, 33), (32, 2, 70)])
 def test_tree_rows_of_all_sizes(hip, hd, G, n, order):
