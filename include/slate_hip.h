@@ -320,6 +320,119 @@ int   slate_hip_attention_tree_q8(float* out, const float* q, const int8_t* Kq, 
  * heads they refuse. */
 int64_t slate_hip_attention_packed_bytes(int n_q_heads, int n_kv_heads, int head_dim);
 
+/* ---- a K/V cache in pages, and verification of drafted tokens --------------
+ * The cache's rows are given out in pages of page_size rows to n_slots slots (a
+ * sequence has one).  All arrays are the caller's (device); pages_reset fills
+ * them.  Page table[s * max_pages + i] holds the rows i * page_size .. of slot s,
+ * for i < held[s]; entries behind are -1.  free_pages[0 .. n_free[0]-1] are the
+ * pages that no slot has, the last is taken first.  n_pages * page_size and
+ * max_pages * page_size are at most 2^31 - 1024. */
+typedef struct slate_hip_pages {
+    int32_t *table, *held, *free_pages, *n_free;   /* [n_slots * max_pages], [n_slots], [n_pages], [1] */
+    int n_slots, max_pages, n_pages, page_size;
+} slate_hip_pages_t;
+/* The pools of K and V (device, 16-byte aligned) and where in them row r (0 ..
+ * page_size-1) of page p of head h is: its head_dim elements start at element p *
+ * page_stride + h * head_stride + r * row_stride.  Strides are multiples of 8, row_stride
+ * at least head_dim and at most 2^26, so any order of page, head and row will do;
+ * head_dim is a multiple of 8, at most 256. */
+typedef struct slate_hip_paged_kv {
+    void *K, *V;
+    int dtype;                                     /* 0: f32, 1: f16, 2: bf16 */
+    int n_kv_heads, head_dim;
+    int64_t page_stride, head_stride, row_stride;
+} slate_hip_paged_kv_t;
+
+/* All pages free (page 0 is taken first), no slot has any. */
+int   slate_hip_pages_reset(const slate_hip_pages_t* pages);
+/* Take the pages that a step's new tokens need, and lay its batch out as
+ * pack_batch does.  Sequence b (of B, 1 .. 1024) has slot[b], pos0[b] rows cached
+ * and brings n_new[b] >= 0 tokens (device int32[B] each): its slot gets the pages
+ * that hold pos0 + n_new rows, if it has fewer, sequence after sequence.  Outputs
+ * (device): tok_off[B+1]; of every token its sequence tok2seq[T], position
+ * tok_pos[T] and cache row tok_row[T] (page * page_size + row within it, where
+ * kv_store_paged puts it; -1 where the table names no page); last_tok[B] (-1 for
+ * a sequence without tokens).  status[0] says 0, or, with nothing else written:
+ * -1 bad descriptor (a negative number, a slot outside 0 .. n_slots-1 or in two
+ * sequences, held or n_free outside their ranges), -2 more rows than a slot can
+ * have, more tokens than T_cap or more pages than are free. */
+int   slate_hip_pages_extend(const slate_hip_pages_t* pages, const int32_t* slot, const int32_t* pos0,
+                             const int32_t* n_new, int B, int T_cap, int32_t* tok_off, int32_t* tok2seq,
+                             int32_t* tok_pos, int32_t* tok_row, int32_t* last_tok, int32_t* status);
+/* Give back the pages behind the first length[b] rows (device int32[B]; 0: all)
+ * of slot[b]: of requests that end, of drafts that did not stand.  The pages
+ * that pages_extend just took come back in the order in which they lay there.
+ * status as above (-1 also where the stack would hold more than n_pages). */
+int   slate_hip_pages_trim(const slate_hip_pages_t* pages, const int32_t* slot, const int32_t* length, int B,
+                           int32_t* status);
+/* New K and V rows into their pages: k, v [T, n_kv_heads * head_dim] f32 (16-byte
+ * aligned), rows ld floats apart (ld % 4 == 0), rounded to the pools' type to
+ * nearest, ties to even.  A row whose tok_row is outside 0 .. n_pages * page_size - 1
+ * is stored nowhere; of two rows with the same tok_row either may stay. */
+int   slate_hip_kv_store_paged(const slate_hip_paged_kv_t* kv, const slate_hip_pages_t* pages, const float* k,
+                               const float* v, int64_t ld, const int32_t* tok_row, int T);
+/* Causal GQA attention of new tokens over the pages: q, out [T, n_q_heads *
+ * head_dim] f32 (out is not q).  Sequence b's tokens are the rows tok_off[b] ..
+ * tok_off[b+1]-1, at most max_new of them, and token i attends to rows 0 .. pos0[b]
+ * + i of slot[b] (its own is stored before the call).  Scores are q.k /
+ * sqrt(head_dim); query head g belongs to kv head g / (n_q_heads / n_kv_heads).
+ * A sequence whose numbers do not fit (as for the packed batches above; slot
+ * outside 0 .. n_slots-1, more than max_pages * page_size rows) is left out; rows
+ * of out that no sequence owns stay as they were.  Keys in pages outside 0 ..
+ * n_pages-1 count as not seen, and a token that sees none gets zeros.  What the
+ * cache holds in rows that a token does not see never matters, not even
+ * infinities and NaN; one in a row that it sees makes its output not finite.
+ * Queries must be finite and below 2^100 in size, bf16 and f32 K and V too.  Sums are
+ * f32.  f32 caches are multiplied in f32, for bf16 ones queries and weights are split
+ * into 24 bits, for f16 ones into 22.
+ * Made for few tokens a sequence (decode steps, drafts): K and V are read once for
+ * every 16 query rows of a kv head, or 32 where there are more.  T * n_q_heads <=
+ * 2^31 - 128, and n_kv_heads * (T * n_q_heads / n_kv_heads / 16 + B) * max_pages *
+ * page_size / 128 stays below 2^31.  ws as for attention_ragged_q8, of
+ * slate_hip_attention_paged_bytes. */
+int   slate_hip_attention_paged(float* out, const float* q, const slate_hip_paged_kv_t* kv,
+                                const slate_hip_pages_t* pages, const int32_t* slot, const int32_t* tok_off,
+                                const int32_t* pos0, int B, int T, int max_new, int n_q_heads, void* ws,
+                                size_t ws_bytes);
+/* Bytes of ws for these heads, whatever the batch; -1 for heads it refuses. */
+int64_t slate_hip_attention_paged_bytes(int n_q_heads, int n_kv_heads, int head_dim);
+
+/* Which drafted tokens stand, and the token after them.  Sequence b has the rows
+ * tok_off[b] .. tok_off[b+1]-1 (device int32[B+1]): the first is its last
+ * committed token, the others are drafts; row i continues row parent[i] (device
+ * int32[T], counted within the sequence, below i; another value: no row), or row i - 1
+ * where parent is NULL.  Row t of logits (f32, rows ld floats apart, V of them
+ * count) is the target's distribution after row t, p = softmax(logits /
+ * temperature[b]) (device float[B]; NULL: 1; 0, negative or NaN: all of it on the
+ * largest logit, the lowest of equal ones).  NaN counts as -infinity, +infinity
+ * shares all of p with its like; a row that is all -infinity has no p.  From the first
+ * row on, the drafts x that continue the row are tried in order, the first one
+ * accepted is the next row:
+ *  - with draft_probs (rows draft_ld floats apart; row t is the distribution q that
+ *    token[t] was drawn from; chains only, parent NULL): where u[t] q(x) < p(x).  If it is
+ *    turned down the next token comes from max(p - q, 0), or from p where that is 0;
+ *  - without: where u[t] (1 - the sum of p of those turned down before) < p(x), a
+ *    token that was turned down before having p 0.  The next token comes from p
+ *    without those turned down (from p where nothing else has any);
+ *  - at temperature 0: where x has the largest logit, whatever u and q are.
+ * Where none stands the next token is the lowest i with p(i) > 0 and a sum of p up to i above
+ * u_next[b] times the whole sum (the last with p > 0 where no sum is).  u (device
+ * float[T], at the drafts) and u_next (float[B]) are uniform in [0, 1).  Tokens
+ * outside 0 .. V-1 never stand.  q is not negative.
+ * Outputs (device): n_accepted[b] (-1 for a sequence without rows or whose
+ * tok_off does not fit); out_tok[T]: in a sequence's rows the accepted tokens, the next
+ * one (-1: no p), then -1; out_row[T] (or NULL): the rows that were accepted,
+ * counted within the sequence, then -1.  Rows that no sequence owns stay as they were.
+ * Acceptance is decided in 64 bits from sums of f32 exponentials (p within 2^-20 of
+ * itself), the next token's sums are 64-bit throughout.
+ * ws: device scratch of slate_hip_verify_drafts_bytes, as for attention_ragged_q8. */
+int   slate_hip_verify_drafts(int32_t* n_accepted, int32_t* out_tok, int32_t* out_row, const float* logits, int64_t ld,
+                              const int32_t* token, const int32_t* parent, const float* draft_probs, int64_t draft_ld,
+                              const float* temperature, const float* u, const float* u_next, const int32_t* tok_off,
+                              int B, int T, int V, void* ws, size_t ws_bytes);
+/* Bytes of ws for a batch of that size; -1 for one it refuses. */
+int64_t slate_hip_verify_drafts_bytes(int B, int T, int V);
+
 /* Synthetic weights generated on the device (seeded, ~N(0, std)):
  * f32 values, or rows x cols quantised to Q4_K. */
 int   slate_hip_synth_f32(float* dst, int64_t n, uint64_t seed, float std);

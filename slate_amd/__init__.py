@@ -61,6 +61,16 @@ class RopeConfig(C.Structure):          # slate_hip_rope_t
                 ("magnitude", C.c_double)]
 
 
+class Pages(C.Structure):               # slate_hip_pages_t
+    _fields_ = [("table", vp), ("held", vp), ("free_pages", vp), ("n_free", vp), ("n_slots", C.c_int),
+                ("max_pages", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int)]
+
+
+class PagedKv(C.Structure):             # slate_hip_paged_kv_t
+    _fields_ = [("K", vp), ("V", vp), ("dtype", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("row_stride", C.c_int64)]
+
+
 # name -> (restype, argtypes) for every exported entry point
 SIGNATURES = {
     "slate_backend_hip": (C.POINTER(BackendStruct), []),
@@ -110,6 +120,16 @@ SIGNATURES = {
     "slate_hip_attention_tree": (C.c_int, [vp] * 8 + [C.c_int] * 6 + [C.c_int64, C.c_int, vp, C.c_size_t]),
     "slate_hip_attention_tree_q8": (C.c_int, [vp] * 10 + [C.c_int] * 6 + [C.c_int64, C.c_int, vp, C.c_size_t]),
     "slate_hip_attention_packed_bytes": (C.c_int64, [C.c_int] * 3),
+    "slate_hip_pages_reset": (C.c_int, [C.POINTER(Pages)]),
+    "slate_hip_pages_extend": (C.c_int, [C.POINTER(Pages)] + [vp] * 3 + [C.c_int] * 2 + [vp] * 6),
+    "slate_hip_pages_trim": (C.c_int, [C.POINTER(Pages), vp, vp, C.c_int, vp]),
+    "slate_hip_kv_store_paged": (C.c_int, [C.POINTER(PagedKv), C.POINTER(Pages), vp, vp, C.c_int64, vp, C.c_int]),
+    "slate_hip_attention_paged": (C.c_int, [vp, vp, C.POINTER(PagedKv), C.POINTER(Pages)] + [vp] * 3 +
+                                  [C.c_int] * 4 + [vp, C.c_size_t]),
+    "slate_hip_attention_paged_bytes": (C.c_int64, [C.c_int] * 3),
+    "slate_hip_verify_drafts": (C.c_int, [vp] * 4 + [C.c_int64] + [vp] * 3 + [C.c_int64] + [vp] * 4 +
+                                [C.c_int] * 3 + [vp, C.c_size_t]),
+    "slate_hip_verify_drafts_bytes": (C.c_int64, [C.c_int] * 3),
     "slate_hip_synth_f32": (C.c_int, [vp, C.c_int64, C.c_uint64, C.c_float]),
     "slate_hip_synth_q4k": (C.c_int, [vp, C.c_int64, C.c_int64, C.c_uint64, C.c_float]),
     "slate_hip_llama_new": (vp, [C.POINTER(LlamaConfig), vp, vp, vp, C.c_int,

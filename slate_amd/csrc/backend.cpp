@@ -152,7 +152,7 @@ KnobScope::~KnobScope() { t_knobs = prev_; }
 std::mutex g_enqueue_mu;
 
 struct ScratchBuf { void* p = nullptr; size_t n = 0; };
-static ScratchBuf g_scratch[8];
+static ScratchBuf g_scratch[10];
 
 void* scratch(int slot, size_t bytes) {
     ScratchBuf& b = g_scratch[slot];

@@ -1,0 +1,256 @@
+// k_pages.hip -- pages of a K/V cache taken and given back, the slot map of a
+// step's tokens, and new K/V rows stored by it.
+#include "attn_plan.h"
+#include "paged.h"
+
+namespace slate_hip {
+
+constexpr int PGS_TH = 1024;           // threads of the one workgroup: a sequence each
+constexpr int PGS_HASH = 2048;
+
+// Sums over the workgroup, each thread bringing a count below 2^31: the
+// inclusive one up to the thread (below 2^31 if the whole is), and the whole.
+struct Scan {
+    int upto;
+    int64_t total;
+};
+__device__ __forceinline__ Scan block_scan(int v, int64_t* s_part) {
+    const int w = threadIdx.x >> 6;
+    const int upto = wave_scan(v);
+    // halves of 16 bits: their sums over a wave pass no 32 bits
+    const int64_t whole = ((int64_t)wave_sum_int(v >> 16) << 16) + wave_sum_int(v & 0xffff);
+    if ((threadIdx.x & 63) == 0) s_part[w] = whole;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int i = 0; i < PGS_TH / 64; ++i) {
+        before += i < w ? s_part[i] : 0;
+        total += s_part[i];
+    }
+    __syncthreads();
+    return Scan{(int)before + upto, total};
+}
+
+// Whether another sequence brought the same slot: an open hash of the slots
+// seen.
+__device__ __forceinline__ bool seen_before(int* s_hash, int slot) {
+    uint32_t at = (uint32_t)slot * 2654435761u >> 21;
+    for (;;) {                         // twice as many places as slots: ends
+        const int was = atomicCAS(&s_hash[at], -1, slot);
+        if (was == -1) return false;
+        if (was == slot) return true;
+        at = (at + 1) & (PGS_HASH - 1);
+    }
+}
+static_assert(PGS_HASH == 1 << 11 && PGS_HASH >= 2 * PK_MAX_SEQ, "the hash's shift");
+
+// The first sequence whose inclusive sum is above x (which is below the last one's).
+__device__ __forceinline__ int find_above(const int* s_upto, int B, int x) {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_upto[mid] > x)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    return lo;
+}
+
+__global__ __launch_bounds__(256) void pages_reset_kernel(Pages pg) {
+    const int64_t step = (int64_t)gridDim.x * 256, cells = (int64_t)pg.n_slots * pg.max_pages;
+    const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (int64_t i = i0; i < cells; i += step) pg.table[i] = -1;
+    for (int64_t i = i0; i < pg.n_slots; i += step) pg.held[i] = 0;
+    for (int64_t i = i0; i < pg.n_pages; i += step) pg.free_pages[i] = pg.n_pages - 1 - (int)i;
+    if (i0 == 0) pg.n_free[0] = pg.n_pages;
+}
+
+// Two sums over the sequences (tokens, new pages); then a thread per new page
+// and per token finds its sequence in them.
+__global__ __launch_bounds__(PGS_TH) void pages_extend_kernel(Pages pg, const int32_t* __restrict__ slot,
+                                                              const int32_t* __restrict__ pos0,
+                                                              const int32_t* __restrict__ n_new, int B, int T_cap,
+                                                              int32_t* __restrict__ tok_off,
+                                                              int32_t* __restrict__ tok2seq,
+                                                              int32_t* __restrict__ tok_pos,
+                                                              int32_t* __restrict__ tok_row,
+                                                              int32_t* __restrict__ last_tok,
+                                                              int32_t* __restrict__ status) {
+    __shared__ int s_hash[PGS_HASH], s_slot[PGS_TH], s_pos0[PGS_TH], s_held[PGS_TH], s_tok[PGS_TH], s_page[PGS_TH];
+    __shared__ int64_t s_part[PGS_TH / 64];
+    __shared__ int s_err;
+    const int b = threadIdx.x;
+    for (int i = b; i < PGS_HASH; i += PGS_TH) s_hash[i] = -1;
+    if (b == 0) s_err = 0;
+    __syncthreads();
+    const int n_free = pg.n_free[0];
+    int sl = 0, p0 = 0, n = 0, held = 0, fresh = 0;
+    if (b < B) {
+        sl = slot[b];
+        p0 = pos0[b];
+        n = n_new[b];
+        bool bad = sl < 0 || sl >= pg.n_slots || p0 < 0 || n < 0 || n_free < 0 || n_free > pg.n_pages;
+        if (!bad) {
+            held = pg.held[sl];
+            bad = seen_before(s_hash, sl) || held < 0 || held > pg.max_pages;
+        }
+        const int64_t rows = (int64_t)p0 + n;
+        if (bad)
+            atomicOr(&s_err, 1);
+        else if (rows > (int64_t)pg.max_pages * pg.page_size)
+            atomicOr(&s_err, 2);
+        else
+            fresh = max(0, (int)((rows + pg.page_size - 1) / pg.page_size) - held);
+        n = max(n, 0);
+    }
+    const Scan tok = block_scan(n, s_part), page = block_scan(fresh, s_part);
+    s_slot[b] = sl;
+    s_pos0[b] = p0;
+    s_held[b] = held;
+    s_tok[b] = tok.upto;
+    s_page[b] = page.upto;
+    __syncthreads();
+    int err = s_err & 1 ? -1 : s_err ? -2 : 0;
+    if (err == 0 && (tok.total > T_cap || page.total > n_free)) err = -2;
+    if (b == 0) status[0] = err;
+    if (err != 0) return;
+    const int T = (int)tok.total, new_pages = (int)page.total;
+    if (b < B) {
+        tok_off[b] = tok.upto - n;
+        if (b == B - 1) tok_off[B] = tok.upto;
+        last_tok[b] = n > 0 ? tok.upto - 1 : -1;
+        if (fresh > 0) pg.held[sl] = held + fresh;
+    }
+    if (b == 0) pg.n_free[0] = n_free - new_pages;
+    for (int k = threadIdx.x; k < new_pages; k += PGS_TH) {
+        const int s = find_above(s_page, B, k), first = s > 0 ? s_page[s - 1] : 0;
+        pg.table[(int64_t)s_slot[s] * pg.max_pages + s_held[s] + (k - first)] = pg.free_pages[n_free - 1 - k];
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < T; t += PGS_TH) {
+        const int s = find_above(s_tok, B, t), first = s > 0 ? s_tok[s - 1] : 0;
+        const int pos = s_pos0[s] + (t - first), i = pos / pg.page_size;
+        const int pno = pg.table[(int64_t)s_slot[s] * pg.max_pages + i];
+        tok2seq[t] = s;
+        tok_pos[t] = pos;
+        tok_row[t] = (unsigned)pno < (unsigned)pg.n_pages ? pno * pg.page_size + (pos - i * pg.page_size) : -1;
+    }
+}
+
+__global__ __launch_bounds__(PGS_TH) void pages_trim_kernel(Pages pg, const int32_t* __restrict__ slot,
+                                                            const int32_t* __restrict__ length, int B,
+                                                            int32_t* __restrict__ status) {
+    __shared__ int s_hash[PGS_HASH], s_slot[PGS_TH], s_keep[PGS_TH], s_page[PGS_TH];
+    __shared__ int64_t s_part[PGS_TH / 64];
+    __shared__ int s_err;
+    const int b = threadIdx.x;
+    for (int i = b; i < PGS_HASH; i += PGS_TH) s_hash[i] = -1;
+    if (b == 0) s_err = 0;
+    __syncthreads();
+    const int n_free = pg.n_free[0];
+    int sl = 0, keep = 0, back = 0;
+    if (b < B) {
+        sl = slot[b];
+        const int len = length[b];
+        bool bad = sl < 0 || sl >= pg.n_slots || len < 0 || n_free < 0 || n_free > pg.n_pages;
+        if (!bad) {
+            const int held = pg.held[sl];
+            bad = seen_before(s_hash, sl) || held < 0 || held > pg.max_pages;
+            keep = min(held, (int)(((int64_t)len + pg.page_size - 1) / pg.page_size));
+            back = held - keep;
+        }
+        if (bad) {
+            atomicOr(&s_err, 1);
+            back = 0;
+        }
+    }
+    const Scan page = block_scan(back, s_part);
+    s_slot[b] = sl;
+    s_keep[b] = keep;
+    s_page[b] = page.upto;
+    __syncthreads();
+    int err = s_err ? -1 : 0;
+    if (err == 0 && n_free + page.total > pg.n_pages) err = -1;
+    if (b == 0) status[0] = err;
+    if (err != 0) return;
+    const int total = (int)page.total;
+    if (b < B && back > 0) pg.held[sl] = keep;
+    if (b == 0) pg.n_free[0] = n_free + total;
+    for (int k = threadIdx.x; k < total; k += PGS_TH) {
+        const int s = find_above(s_page, B, k), first = s > 0 ? s_page[s - 1] : 0;
+        int32_t* cell = pg.table + (int64_t)s_slot[s] * pg.max_pages + s_keep[s] + (k - first);
+        pg.free_pages[n_free + total - 1 - k] = *cell;
+        *cell = -1;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rows rounded to the pools' type: 8 elements a thread, so that heads and rows
+// of any stride are written 16 (f32: 32) bytes at a time.
+template <class E>
+struct Eight {
+    E e[8];
+};
+
+template <class E>
+__global__ __launch_bounds__(256) void kv_store_paged_kernel(slate_hip_paged_kv_t kv, int page_size, int n_rows,
+                                                             const float* __restrict__ k, const float* __restrict__ v,
+                                                             int64_t ld, const int32_t* __restrict__ tok_row) {
+    const int t = blockIdx.x, row = tok_row[t];
+    if ((unsigned)row >= (unsigned)n_rows) return;
+    const float* src = (blockIdx.y ? v : k) + (int64_t)t * ld;
+    const int page = row / page_size;
+    E* dst = (E*)(blockIdx.y ? kv.V : kv.K) + page * kv.page_stride + (row - page * page_size) * kv.row_stride;
+    const int c8 = kv.head_dim / 8;
+    for (int c = threadIdx.x; c < kv.n_kv_heads * c8; c += 256) {
+        const float4 a = *(const float4*)(src + 8 * c), b = *(const float4*)(src + 8 * c + 4);
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const int h = c / c8;
+        Eight<E> o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o.e[e] = (E)x[e];
+        *(Eight<E>*)__builtin_assume_aligned(dst + h * kv.head_stride + 8 * (c - h * c8), 16) = o;
+    }
+}
+
+int launch_pages_reset(const Pages& pg, hipStream_t s) {
+    const int64_t cells = max((int64_t)pg.n_slots * pg.max_pages, (int64_t)pg.n_pages);
+    hipLaunchKernelGGL(pages_reset_kernel, dim3((unsigned)min((int64_t)1024, (cells + 255) / 256)), dim3(256), 0, s, pg);
+    SH_CHECK_LAUNCH();
+    return 0;
+}
+
+int launch_pages_extend(const Pages& pg, const int32_t* slot, const int32_t* pos0, const int32_t* n_new, int B,
+                        int T_cap, int32_t* tok_off, int32_t* tok2seq, int32_t* tok_pos, int32_t* tok_row,
+                        int32_t* last_tok, int32_t* status, hipStream_t s) {
+    hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(PGS_TH), 0, s, pg, slot, pos0, n_new, B, T_cap, tok_off,
+                       tok2seq, tok_pos, tok_row, last_tok, status);
+    SH_CHECK_LAUNCH();
+    return 0;
+}
+
+int launch_pages_trim(const Pages& pg, const int32_t* slot, const int32_t* length, int B, int32_t* status,
+                      hipStream_t s) {
+    hipLaunchKernelGGL(pages_trim_kernel, dim3(1), dim3(PGS_TH), 0, s, pg, slot, length, B, status);
+    SH_CHECK_LAUNCH();
+    return 0;
+}
+
+int launch_kv_store_paged(const slate_hip_paged_kv_t& kv, const Pages& pg, const float* k, const float* v, int64_t ld,
+                          const int32_t* tok_row, int T, hipStream_t s) {
+    const dim3 grid(T, 2);
+    const int rows = pg.n_pages * pg.page_size;
+    if (kv.dtype == KV_F32)
+        hipLaunchKernelGGL(kv_store_paged_kernel<float>, grid, dim3(256), 0, s, kv, pg.page_size, rows, k, v, ld,
+                           tok_row);
+    else if (kv.dtype == KV_F16)
+        hipLaunchKernelGGL(kv_store_paged_kernel<_Float16>, grid, dim3(256), 0, s, kv, pg.page_size, rows, k, v, ld,
+                           tok_row);
+    else
+        hipLaunchKernelGGL(kv_store_paged_kernel<__bf16>, grid, dim3(256), 0, s, kv, pg.page_size, rows, k, v, ld,
+                           tok_row);
+    SH_CHECK_LAUNCH();
+    return 0;
+}
+
+}  // namespace slate_hip
