@@ -43,18 +43,22 @@ __device__ __forceinline__ T* uniform(T* p) {
 // A place on the line: granule `at` of the sequence's `own`.
 struct Place {
     SeqView seq;
-    int64_t base;                      // kv_base
+    int64_t base;                      // seq_base
     int at;
 };
 
-// Count(SeqView) -> granules of a sequence (all its heads and blocks).
-template <class Count>
+// Where a sequence's cache is: kv_base.
+__device__ __forceinline__ int64_t seq_base(const PackedBatch& pb, int b) { return pb.kv_base[b]; }
+
+// Count(SeqView) -> granules of a sequence (all its heads and blocks).  Batch
+// has tok_off and B, seq_view and seq_base.
+template <class Count, class Batch = PackedBatch>
 class Plan {
   public:
     int total;
     int end;                           // sequences from it on are left out
 
-    __device__ __forceinline__ Plan(const PackedBatch& pb, const Count& count) : pb_(pb), count_(count) {
+    __device__ __forceinline__ Plan(const Batch& pb, const Count& count) : pb_(pb), count_(count) {
         end = pb.B;
         cut(0);
         first_ = load(0);
@@ -70,7 +74,7 @@ class Plan {
         int64_t base;
         int own, upto;                 // granules of the lane's sequence, and with those of the lanes before it
     };
-    __device__ __forceinline__ Plan(const PackedBatch& pb, const Count& count, int total_, int end_, const Lane& first)
+    __device__ __forceinline__ Plan(const Batch& pb, const Count& count, int total_, int end_, const Lane& first)
         : total(total_), end(end_), pb_(pb), count_(count), first_(first) {}
     __device__ __forceinline__ const Lane& first() const { return first_; }
     // 0 <= x < total
@@ -114,13 +118,13 @@ class Plan {
         Lane s{};
         if (b < end) {
             s.seq = seq_view(pb_, b);
-            s.base = pb_.kv_base[b];
+            s.base = seq_base(pb_, b);
             s.own = count_(s.seq);
         }
         s.upto = wave_scan(s.own);
         return s;
     }
-    const PackedBatch& pb_;
+    const Batch& pb_;
     const Count count_;
     Lane first_;
 };
@@ -146,6 +150,10 @@ inline int64_t plan_bytes(int P, int rows, int hd) {
 }
 // hd 32, 64 or 128.
 void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, int P, hipStream_t s);
+// The same for slots of `slot_hd` (64, 128, 256) columns of which the first hd are
+// real, and rows that may have seen no key (their outputs are zeros).
+void launch_attn_join_paged(float* out, void* ws, int Hq, int Hkv, int hd, int slot_hd, int slot_rows, int P,
+                            hipStream_t s);
 
 // The entry of workgroup w, whose range begins at x0 in granule `in` of a
 // block of `gran`; begin(w) are the ranges' beginnings.  Called by a whole

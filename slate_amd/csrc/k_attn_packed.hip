@@ -98,10 +98,11 @@ __global__ __launch_bounds__(256) void attn_packed_rows_kernel(PackedAttn a, Pac
 // Joins the parts of a block that lies in several workgroups' ranges:
 // workgroup b takes the block that is first cut before workgroup b + 1 of the
 // attention kernel, HD / 4 lanes a row, eight parts' loads at a time.
+// PAGED: rows of hd <= HD columns, which may have seen no key.
 constexpr int JOIN_TH = 512;
-template <int HD>
+template <int HD, bool PAGED>
 __global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ out, void* ws, int Hq, int G,
-                                                       int slot_rows, int P) {
+                                                       int slot_rows, int P, int hd) {
     const JoinEntry en = *entry_of(ws, blockIdx.x + 1);
     const int c = 4 * (threadIdx.x % (HD / 4));
     // the first part's slot, then the first slot of each workgroup after it
@@ -140,8 +141,9 @@ __global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ 
                 o.w += fk * v[k].w;
             }
         }
-        const float inv = 1.0f / l;
-        float* op = out + ((int64_t)(en.t0 + (en.r0 + r) / G) * Hq + en.h * G + (en.r0 + r) % G) * HD + c;
+        if (PAGED && c >= hd) return;
+        const float inv = PAGED && l == 0.f ? 0.f : 1.0f / l;
+        float* op = out + ((int64_t)(en.t0 + (en.r0 + r) / G) * Hq + en.h * G + (en.r0 + r) % G) * (PAGED ? hd : HD) + c;
         op[0] = o.x * inv;
         op[1] = o.y * inv;
         op[2] = o.z * inv;
@@ -149,11 +151,11 @@ __global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ 
     }
 }
 
-template <int HD>
-static void launch_join_hd(float* out, void* ws, int Hq, int Hkv, int slot_rows, int P, hipStream_t s) {
+template <int HD, bool PAGED = false>
+static void launch_join_hd(float* out, void* ws, int Hq, int Hkv, int slot_rows, int P, hipStream_t s, int hd = HD) {
     constexpr int AT_ONCE = JOIN_TH / (HD / 4);        // rows of a workgroup
-    hipLaunchKernelGGL(attn_join_kernel<HD>, dim3(P - 1, (slot_rows + AT_ONCE - 1) / AT_ONCE), dim3(JOIN_TH), 0, s, out,
-                       ws, Hq, Hq / Hkv, slot_rows, P);
+    hipLaunchKernelGGL((attn_join_kernel<HD, PAGED>), dim3(P - 1, (slot_rows + AT_ONCE - 1) / AT_ONCE), dim3(JOIN_TH), 0,
+                       s, out, ws, Hq, Hq / Hkv, slot_rows, P, hd);
 }
 
 void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_rows, int P, hipStream_t s) {
@@ -163,6 +165,16 @@ void launch_attn_join(float* out, void* ws, int Hq, int Hkv, int hd, int slot_ro
         launch_join_hd<64>(out, ws, Hq, Hkv, slot_rows, P, s);
     else
         launch_join_hd<32>(out, ws, Hq, Hkv, slot_rows, P, s);
+}
+
+void launch_attn_join_paged(float* out, void* ws, int Hq, int Hkv, int hd, int slot_hd, int slot_rows, int P,
+                            hipStream_t s) {
+    if (slot_hd == 256)
+        launch_join_hd<256, true>(out, ws, Hq, Hkv, slot_rows, P, s, hd);
+    else if (slot_hd == 128)
+        launch_join_hd<128, true>(out, ws, Hq, Hkv, slot_rows, P, s, hd);
+    else
+        launch_join_hd<64, true>(out, ws, Hq, Hkv, slot_rows, P, s, hd);
 }
 
 int64_t attention_packed_bytes(int Hq, int Hkv, int hd) {

@@ -37,6 +37,13 @@ struct PagedBatch {
     int B, T, max_new, n_slots;
     int max_seq;                       // rows that a slot can have
 };
+__device__ __forceinline__ SeqView seq_view(const PagedBatch& pb, int b) {
+    const int t0 = pb.tok_off[b], t1 = pb.tok_off[b + 1], p0 = pb.pos0[b], slot = pb.slot[b];
+    const bool fits = t0 >= 0 && t1 >= t0 && t1 <= pb.T && t1 - t0 <= pb.max_new && p0 >= 0 &&
+                      p0 <= pb.max_seq - (t1 - t0) && slot >= 0 && slot < pb.n_slots;
+    return SeqView{t0, fits ? t1 - t0 : 0, p0};
+}
+__device__ __forceinline__ int64_t seq_base(const PagedBatch& pb, int b) { return pb.slot[b]; }
 int64_t attention_paged_bytes(int hd);
 int launch_attention_paged(const PagedAttn& a, const PagedBatch& pb, hipStream_t s);
 
