@@ -419,12 +419,12 @@ int64_t slate_hip_attention_paged_bytes(int n_q_heads, int n_kv_heads, int head_
  * u_next[b] times the whole sum (the last with p > 0 where no sum is).  u (device
  * float[T], at the drafts) and u_next (float[B]) are uniform in [0, 1).  Tokens
  * outside 0 .. V-1 never stand.  q is not negative.
- * Outputs (device): n_accepted[b] (-1 for a sequence without rows or whose
- * tok_off does not fit); out_tok[T]: in a sequence's rows the accepted tokens, the next
+ * Outputs (device): n_accepted[b] (-1 for a sequence that is left out: without rows, with
+ * more than 1024 drafts, outside 0 .. T, or behind a fall of tok_off); out_tok[T]: in a sequence's rows the accepted tokens, the next
  * one (-1: no p), then -1; out_row[T] (or NULL): the rows that were accepted,
  * counted within the sequence, then -1.  Rows that no sequence owns stay as they were.
- * Acceptance is decided in 64 bits from sums of f32 exponentials (p within 2^-20 of
- * itself), the next token's sums are 64-bit throughout.
+ * Probabilities, sums and comparisons are in 64 bits, exponentials good to 2^-42.  V is at
+ * most 2^31 - 1024.
  * ws: device scratch of slate_hip_verify_drafts_bytes, as for attention_ragged_q8. */
 int   slate_hip_verify_drafts(int32_t* n_accepted, int32_t* out_tok, int32_t* out_row, const float* logits, int64_t ld,
                               const int32_t* token, const int32_t* parent, const float* draft_probs, int64_t draft_ld,
