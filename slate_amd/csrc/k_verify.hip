@@ -19,11 +19,12 @@ namespace slate_hip {
 
 constexpr int VF_CHUNK = 1024;         // logits of a wave: 16 a lane
 constexpr int VF_TH = 512;             // threads that walk a sequence
+constexpr int VF_SUM_WGS = 1024;       // workgroups of the sums
 constexpr int VF_ROWS = PK_MAX_DRAFT + 1;
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// 2^t for t <= 0, to 2^-42 of itself: e^(f ln 2) for the part f of t behind the
+// 2^t for t < 1000, to 2^-42 of itself: e^(f ln 2) for the part f of t behind the
 // point, |f ln 2| <= 0.347, by its series up to the tenth power.
 __device__ __forceinline__ double pow2(double t) {
     t = fmax(t, -1100.0);
@@ -42,18 +43,61 @@ __device__ __forceinline__ double pow2(double t) {
     return ldexp(e, (int)n);
 }
 
-// Weight of logit x beside the largest one: e^((x - top) / temperature), by =
-// log2(e) / temperature.  0 for -infinity; infinite logits share all.
+// Weight of logit x beside `top`, the largest one or (where all weights fit beside
+// it) 0: e^((x - top) / temperature), by = log2(e) / temperature.  0 for -infinity;
+// infinite logits share all.
 __device__ __forceinline__ double weight(float x, float top, double by) {
     if (!(x > -INFINITY)) return 0;
     if (x == top) return 1;
     return top == INFINITY ? 0 : pow2(((double)x - (double)top) * by);
 }
 
+// The same beside 0 instead of the largest logit, for sums over whole rows: 64 bits hold
+// 2^512 as they hold 1.  2^(k / 64 + r / 64), |r| <= 1/2, is 2^(k / 64) from a table (entry
+// k % 64 in lane k % 64) times the series of e^(r ln 2 / 64) up to the fourth power, to
+// 2^-44 of itself; 13 operations.
+class Weights {
+  public:
+    __device__ __forceinline__ Weights() {
+        const int lane = threadIdx.x & 63;
+        const uint64_t u = __builtin_bit_cast(uint64_t, exp2(lane * (1.0 / 64)));
+        lo_ = (uint32_t)u;
+        hi_ = (uint32_t)(u >> 32) - ((uint32_t)lane << 14);    // k << 14 is k / 64 in the exponent, and this
+    }
+    __device__ __forceinline__ void start(double by) {
+        by_ = 64 * by;
+        low_ = (float)(-900 / by);
+        most_ = (float)(512 / by);
+    }
+    // Whether a wave's values can be taken so, `top` being the largest that the lane
+    // has: none above 2^512 and one above 2^-512, so that what counts as 2^-900
+    // below shows in no sum (infinities, NaN, temperatures without an end: no).
+    __device__ __forceinline__ bool takes(float top) const {
+        return most_ < 1e38f && !__builtin_amdgcn_ballot_w64(top > most_) && __builtin_amdgcn_ballot_w64(top > -most_);
+    }
+    __device__ __forceinline__ double operator()(float x) const {
+        constexpr double WHOLE = 6755399441055744.0;   // 1.5 2^52: a sum with it is a whole number in its low bits
+        constexpr double L = 0.69314718055994530942 / 64;
+        const double d = (double)fmaxf(x, low_);       // NaN counts as the least
+        const double kd = fma(d, by_, WHOLE), r = fma(d, by_, WHOLE - kd);
+        const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, kd);
+        const uint32_t lo = __builtin_amdgcn_ds_bpermute((int)(4 * k), (int)lo_);
+        const uint32_t hi = __builtin_amdgcn_ds_bpermute((int)(4 * k), (int)hi_) + (k << 14);
+        const double t = __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+        const double e = r * fma(r, fma(r, fma(r, L * L * L * L / 24, L * L * L / 6), L * L / 2), L);
+        return fma(t, e, t);
+    }
+
+  private:
+    uint32_t lo_, hi_;
+    double by_ = 0;
+    float low_ = 0, most_ = INFINITY;
+};
+
 struct alignas(16) Part {
-    float top;                         // -infinity: none
+    float top;                         // the largest logit, or 0 (Weights); -infinity: no p
     int best;                          // its first place (greedy rows)
-    double sum;                        // of the weights beside it
+    double sum;                        // of the weights beside top
 };
 
 // The temperature's inverse times log2(e); 0 stands for greedy here.
@@ -66,37 +110,64 @@ __device__ __forceinline__ Heat heat_of(const float* temperature, int b) {
     return Heat{!(t > 0), t > 0 ? 1.4426950408889634074 / (double)t : 0.0};
 }
 
-__device__ __forceinline__ int place(int c, int k, int lane) { return c * VF_CHUNK + 256 * k + 4 * lane; }
-
 // A wave's 16 values a lane of chunk c: x[4k + e] is element 256 k + 4 lane + e of
-// it; `none` behind V.
+// it, whole lines at a time; `none` behind V.
+__device__ __forceinline__ int place(int c, int i) {
+    return c * VF_CHUNK + 256 * (i / 4) + 4 * (int)(threadIdx.x & 63) + i % 4;
+}
 __device__ __forceinline__ void load16(const float* z, int c, int V, float none, float* x) {
-    const int lane = threadIdx.x & 63;
     if (V - c * VF_CHUNK >= VF_CHUNK) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float4u v = *(const float4u*)(z + place(c, k, lane));
+            const float4u v = *(const float4u*)(z + place(c, 4 * k));
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 * k + e] = v[e];
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int at = place(c, i / 4, lane) + i % 4;
+            const int at = place(c, i);
             x[i] = at < V ? z[at] : none;
         }
     }
 }
-
-__device__ __forceinline__ double wave_sum_f64(double v) {
+// Four elements in a row.
+__device__ __forceinline__ void load4(const float* z, int at, int V, float none, float* x) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    for (int i = 0; i < 4; ++i) x[i] = at < V - i ? z[at + i] : none;
+}
+
+// Inclusive sum over the wave's lanes (DPP: within rows of 16, then across).
+__device__ __forceinline__ double wave_scan_f64(double v) {
+#define VF_SCAN_STEP(ctrl, rows)                                                                               \
+    {                                                                                                          \
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);                                                    \
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, ctrl, rows, 0xF, false);          \
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), ctrl, rows, 0xF, false);            \
+        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                              \
+    }
+    VF_SCAN_STEP(0x111, 0xF)           // row_shr:1, 2, 4, 8
+    VF_SCAN_STEP(0x112, 0xF)
+    VF_SCAN_STEP(0x114, 0xF)
+    VF_SCAN_STEP(0x118, 0xF)
+    VF_SCAN_STEP(0x142, 0xA)           // row_bcast:15 into rows 1 and 3
+    VF_SCAN_STEP(0x143, 0xC)           // row_bcast:31 into rows 2 and 3
+#undef VF_SCAN_STEP
     return v;
 }
+__device__ __forceinline__ double last_lane(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, 63), hi = __builtin_amdgcn_readlane((int)(u >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) { return last_lane(wave_scan_f64(v)); }
 __device__ __forceinline__ int wave_min_int(int v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = min(v, __shfl_xor(v, o));
-    return v;
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR1, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR2, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, DPP_ROW_HALF_MIRROR, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, DPP_ROW_MIRROR, 0xF, 0xF, false));
+    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
 __host__ __device__ constexpr int chunks_of(int V) { return (V - 1) / VF_CHUNK + 1; }
@@ -106,6 +177,7 @@ struct Next {
     int row, turned, at;               // the row whose p it is, the draft's row (-1: nothing to do), where it goes
     float top;
     double sum;                        // of the row's weights
+    int done, pad;                     // workgroups that have left their chunks' masses
 };
 struct Space {
     Part* part;
@@ -123,46 +195,69 @@ int64_t verify_drafts_bytes(int B, int T, int V) {
     return T * nch * (int64_t)sizeof(Part) + B * nch * (int64_t)sizeof(double) + B * (int64_t)sizeof(Next);
 }
 
-// Softmax sums (greedy rows: the largest logit) of all rows, a wave per chunk.
-__global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a) {
+// Softmax sums (greedy rows: the largest logit) of all rows, a wave per chunk of a
+// stretch of rows, the next row's logits under way while it works on the last.
+__global__ __launch_bounds__(256, 4) void verify_sums_kernel(VerifyArgs a) {
     const int lane = threadIdx.x & 63, nch = chunks_of(a.V);
     const int c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (c >= nch) return;
+    const int r0 = (int)((int64_t)a.T * blockIdx.y / gridDim.y), r1 = (int)((int64_t)a.T * (blockIdx.y + 1) / gridDim.y);
     const Space sp = space_of(a);
-    for (int t = blockIdx.y; t < a.T; t += gridDim.y) {
-        float x[16];
-        load16(a.logits + (int64_t)t * a.ld, c, a.V, -INFINITY, x);
-        // the sequence, for its temperature (a row that belongs to none has some)
-        int b = 0;
-        if (a.temperature)
-            for (int b0 = 0; b0 < a.B; b0 += 64) {
-                const int i = b0 + lane;
-                uint64_t begun = __builtin_amdgcn_ballot_w64(i < a.B && a.tok_off[i] <= t);
-                const uint64_t falls = __builtin_amdgcn_ballot_w64(i < a.B && a.tok_off[i + 1] < a.tok_off[i]);
-                if (falls) begun &= (falls & -falls) - 1;
-                b += __popcll(begun);
-                if (falls) break;
-            }
-        const Heat heat = heat_of(a.temperature, max(0, b - 1));
-        float top = -INFINITY;
+    float next[16];
+    load16(a.logits + (int64_t)r0 * a.ld, c, a.V, -INFINITY, next);
+    // the first row's sequence, for its temperature (a row that belongs to none has some)
+    int b = 0;
+    if (a.temperature)
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+            const int i = b0 + lane;
+            uint64_t begun = __builtin_amdgcn_ballot_w64(i < a.B && a.tok_off[i] <= r0);
+            const uint64_t falls = __builtin_amdgcn_ballot_w64(i < a.B && a.tok_off[i + 1] < a.tok_off[i]);
+            if (falls) begun &= (falls & -falls) - 1;
+            b += __popcll(begun);
+            if (falls) break;
+        }
+    b = max(0, b - 1);
+    Heat heat = heat_of(a.temperature, b);
+    Weights weights;
+    if (!heat.greedy) weights.start(heat.by);
+    for (int t = r0; t < r1; ++t) {
+        float x[16], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;        // NaN too
-            top = fmaxf(top, x[i]);
+            x[i] = next[i];
+            top = fmaxf(top, x[i]);                    // (not NaN)
         }
-        top = wave_max(top);
-        Part p{top, -1, 0};
-        if (heat.greedy) {
-            int at = INT32_MAX;
-#pragma unroll
-            for (int i = 15; i >= 0; --i)
-                if (x[i] == top) at = place(c, i / 4, lane) + i % 4;
-            p.best = wave_min_int(at);
-        } else {
+        if (t + 1 < r1) load16(a.logits + (int64_t)(t + 1) * a.ld, c, a.V, -INFINITY, next);
+        // (behind a fall of tok_off no row's sums are looked at)
+        if (a.temperature && b + 1 < a.B && a.tok_off[b + 1] <= t) {
+            while (b + 1 < a.B && a.tok_off[b + 1] <= t) ++b;
+            heat = heat_of(a.temperature, b);
+            if (!heat.greedy) weights.start(heat.by);
+        }
+        Part p{0.f, -1, 0};
+        if (!heat.greedy && weights.takes(top)) {
             double s = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s += weight(x[i], top, heat.by);
+            for (int i = 0; i < 16; ++i) s += weights(x[i]);
             p.sum = wave_sum_f64(s);
+        } else {
+            p.top = top = wave_max(top);
+            if (heat.greedy) {
+                int at = INT32_MAX;
+#pragma unroll
+                for (int i = 15; i >= 0; --i)
+                    if (x[i] == top) at = place(c, i);
+                p.best = wave_min_int(at);
+            } else {
+                double s = 0;
+#pragma unroll 1
+                for (int i = 0; i < 16; ++i) {
+                    s += weight(x[0], top, heat.by);
+#pragma unroll
+                    for (int k = 0; k < 15; ++k) x[k] = x[k + 1];
+                }
+                p.sum = wave_sum_f64(s);
+            }
         }
         if (lane == 0) sp.part[(int64_t)t * nch + c] = p;
     }
@@ -194,101 +289,106 @@ __device__ __forceinline__ Part row_part(const Part* part, int nch, const Heat& 
 struct Sums {
     double upto, total;
 };
+template <int TH>
 __device__ __forceinline__ Sums block_sums(double v, double* s_part) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(v, o);
-        if (lane >= o) v += up;
-    }
+    const int w = threadIdx.x >> 6;
+    v = wave_scan_f64(v);
     __syncthreads();
-    if (lane == 63) s_part[w] = v;
+    if ((threadIdx.x & 63) == 63) s_part[w] = v;
     __syncthreads();
     double before = 0, total = 0;
 #pragma unroll
-    for (int i = 0; i < VF_TH / 64; ++i) {
+    for (int i = 0; i < TH / 64; ++i) {
         before += i < w ? s_part[i] : 0;
         total += s_part[i];
     }
     return Sums{before + v, total};
 }
 
+// The first thread of the workgroup that says `is`, or (none) the last that says
+// `some`; -1 if none does.  By ballots: that many atomics on one place of LDS take
+// 4 us.
+template <int TH>
+__device__ __forceinline__ int first_or_last(bool is, bool some, int* s_first, int* s_last) {
+    const int w = threadIdx.x >> 6;
+    const uint64_t a = __builtin_amdgcn_ballot_w64(is), b = __builtin_amdgcn_ballot_w64(some);
+    if ((threadIdx.x & 63) == 0) {
+        s_first[w] = a ? 64 * w + __builtin_ctzll(a) : -1;
+        s_last[w] = b ? 64 * w + 63 - __builtin_clzll(b) : -1;
+    }
+    __syncthreads();
+    int first = -1, last = -1;
+#pragma unroll
+    for (int i = 0; i < TH / 64; ++i) {
+        first = first < 0 ? s_first[i] : first;
+        last = max(last, s_last[i]);
+    }
+    return first >= 0 ? first : last < 0 ? -1 : last + TH;     // TH and more: of the last kind
+}
+
 // The token at which the sums of the chunks' masses pass u times the whole: mass(c)
-// is a chunk's, values(c, m) a wave's 16 elements of it a lane, in load16's places.
-// -1 where there is no mass.  Called by the workgroup; thread 0's answer counts.
-template <class Mass, class Values>
+// is a chunk's, values(at, m) are those of the tokens at .. at + 3.  -1 where there is
+// no mass.  Called by a workgroup of TH threads.
+template <int TH, class Mass, class Values>
 __device__ int pick_token(int nch, float u, const Mass& mass, const Values& values, double* s_part) {
-    __shared__ int s_chunk, s_last, s_pick;
+    static_assert(TH >= VF_CHUNK / 4, "four tokens a thread");
+    __shared__ int s_first[TH / 64], s_last[TH / 64], s_pick;
     __shared__ double s_before;
-    double total = 0;
-    for (int c0 = 0; c0 < nch; c0 += VF_TH) {
+    // up to a chunk a thread: one round of sums
+    const bool one = nch <= TH;
+    double own = (int)threadIdx.x < nch ? mass(threadIdx.x) : 0;
+    Sums s = block_sums<TH>(own, s_part);
+    double total = s.total;
+    for (int c0 = TH; c0 < nch; c0 += TH) {
         const int c = c0 + threadIdx.x;
-        total += block_sums(c < nch ? mass(c) : 0, s_part).total;
+        total += block_sums<TH>(c < nch ? mass(c) : 0, s_part).total;
     }
     const double at = total * (double)u;
-    if (threadIdx.x == 0) {
-        s_chunk = INT32_MAX;
-        s_last = -1;
-        s_pick = -1;
-    }
     double before = 0;
-    for (int c0 = 0; c0 < nch; c0 += VF_TH) {
-        const int c = c0 + threadIdx.x;
-        const double m = c < nch ? mass(c) : 0;
-        const Sums s = block_sums(m, s_part);          // its barriers order the writes above
-        if (m > 0) {
-            if (before + s.upto > at) atomicMin(&s_chunk, c);
-            atomicMax(&s_last, c);
+    int chunk = -1;
+    for (int c0 = 0; c0 < nch; c0 += TH) {
+        if (!one) {
+            own = c0 + (int)threadIdx.x < nch ? mass(c0 + threadIdx.x) : 0;
+            s = block_sums<TH>(own, s_part);
         }
-        __syncthreads();
-        const bool found = s_chunk != INT32_MAX;       // none at all: the last one with any mass
-        if ((found ? s_chunk : s_last) == c) s_before = before + (s.upto - m);
-        if (found) break;
+        const int who = first_or_last<TH>(own > 0 && before + s.upto > at, own > 0, s_first, s_last);
+        if (who >= 0) {                                // of the last kind: while none of the first follows
+            chunk = c0 + who % TH;
+            if ((int)threadIdx.x == who % TH) s_before = before + (s.upto - own);
+            if (who < TH) break;
+        }
         before += s.total;
+        __syncthreads();                               // before the next round's numbers
     }
-    __syncthreads();
-    const int lane = threadIdx.x & 63, chunk = s_chunk != INT32_MAX ? s_chunk : s_last;
-    if (threadIdx.x < 64 && chunk >= 0) {
-        double m[16], sum = s_before;
-        values(chunk, m);
-        int pick = -1, last = -1;
+    if (chunk < 0) return -1;
+    const int first = chunk * VF_CHUNK + 4 * (int)threadIdx.x;
+    double m[4] = {0, 0, 0, 0};
+    if (threadIdx.x < VF_CHUNK / 4) values(first, m);
+    own = (m[0] + m[1]) + (m[2] + m[3]);
+    s = block_sums<TH>(own, s_part);                   // its barriers: s_before is there, s_first is read
+    double run = s_before + (s.upto - own);
+    int here = -1, last = -1;                          // the thread's first that passes `at`, its last one
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            double v = (m[4 * k] + m[4 * k + 1]) + (m[4 * k + 2] + m[4 * k + 3]);
-            const double own = v;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double up = __shfl_up(v, o);
-                if (lane >= o) v += up;
-            }
-            double run = sum + (v - own);
-            int here = INT32_MAX, some = -1;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                run += m[4 * k + e];
-                if (m[4 * k + e] > 0) {
-                    some = place(chunk, k, lane) + e;
-                    if (run > at && here == INT32_MAX) here = some;
-                }
-            }
-            here = wave_min_int(here);
-            last = max(last, -wave_min_int(-some));
-            if (pick < 0 && here != INT32_MAX) pick = here;
-            sum += __shfl(v, 63);
+    for (int i = 0; i < 4; ++i) {
+        run += m[i];
+        if (m[i] > 0) {
+            last = first + i;
+            if (here < 0 && run > at) here = last;
         }
-        if (lane == 0) s_pick = pick >= 0 ? pick : last;
     }
+    const int who = first_or_last<TH>(here >= 0, last >= 0, s_first, s_last);
+    if (who >= 0 && (int)threadIdx.x == who % TH) s_pick = who < TH ? here : last;
     __syncthreads();
-    return s_pick;
+    return who < 0 ? -1 : s_pick;
 }
 
 // One workgroup per sequence: its rows' sums joined, its drafts' chances, the walk,
 // and the next token where no draft's probability has to be taken off.
 __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     __shared__ double s_sum[VF_ROWS], s_p[VF_ROWS], s_u[VF_ROWS];
-    __shared__ float s_top[VF_ROWS];
+    __shared__ float s_top[VF_ROWS], s_z[VF_ROWS];
     __shared__ int s_best[VF_ROWS], s_parent[VF_ROWS], s_tok[VF_ROWS];
-    __shared__ double s_part[VF_TH / 64];
+    __shared__ double s_part[VF_TH / 64], s_mass[VF_TH];
     __shared__ int s_node, s_acc, s_turned;
     const int b = blockIdx.x, lane = threadIdx.x & 63, V = a.V, nch = chunks_of(V);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -305,12 +405,19 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     }
     const int n = t1 - t0;
     const Heat heat = heat_of(a.temperature, b);
+    const float u_next = a.u_next[b];
+    // the drafts' numbers by the first waves, the rows' sums from the last wave on: side by side for few rows
     for (int i = threadIdx.x; i < n; i += VF_TH) {
-        s_tok[i] = a.token[t0 + i];
-        const int up = a.parent ? a.parent[t0 + i] : i - 1;
-        s_parent[i] = up >= 0 && up < i ? up : -1;
+        const int x = a.token[t0 + i];
+        int up = a.parent ? a.parent[t0 + i] : i - 1;
+        up = up >= 0 && up < i ? up : -1;
+        s_tok[i] = x;
+        s_parent[i] = up;
+        const bool in = up >= 0 && x >= 0 && x < V;
+        s_z[i] = in ? a.logits[(int64_t)(t0 + up) * a.ld + x] : -INFINITY;
+        s_u[i] = in ? a.u[t0 + i] * (a.q ? (double)a.q[(int64_t)(t0 + i) * a.q_ld + x] : 1.0) : INFINITY;   // infinite: never
     }
-    for (int i = w; i < n; i += VF_TH / 64) {
+    for (int i = VF_TH / 64 - 1 - w; i < n; i += VF_TH / 64) {
         const Part p = row_part(sp.part + (int64_t)(t0 + i) * nch, nch, heat);
         if (lane == 0) {
             s_sum[i] = p.sum;
@@ -322,7 +429,7 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     for (int i = threadIdx.x; i < n; i += VF_TH) {
         const int up = s_parent[i], x = s_tok[i];
         const bool in = x >= 0 && x < V;
-        double p = 0, u = INFINITY;                    // u infinite: never
+        double p = 0;
         if (up >= 0 && in) {
             // a token that an earlier child of the same row has was turned down before this one is tried
             bool again = false;
@@ -331,11 +438,10 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
             if (heat.greedy)
                 p = s_best[up] == x;
             else if (!again && s_sum[up] > 0)
-                p = weight(a.logits[(int64_t)(t0 + up) * a.ld + x], s_top[up], heat.by) / s_sum[up];
-            u = heat.greedy ? 0.5 : a.u[t0 + i] * (a.q ? (double)a.q[(int64_t)(t0 + i) * a.q_ld + x] : 1.0);
+                p = weight(s_z[i], s_top[up], heat.by) / s_sum[up];
+            if (heat.greedy) s_u[i] = 0.5;
         }
         s_p[i] = p;
-        s_u[i] = u;
     }
     __syncthreads();
     if (w == 0) {
@@ -380,7 +486,7 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     }
     const bool less = a.q && turned >= 0 && !heat.greedy && s_sum[node] > 0;
     if (threadIdx.x == 0)
-        sp.next[b] = Next{t0 + node, less ? t0 + turned : -1, t0 + acc, s_top[node], s_sum[node]};
+        sp.next[b] = Next{t0 + node, less ? t0 + turned : -1, t0 + acc, s_top[node], s_sum[node], 0, 0};
     if (less) return;                                  // the next kernels'
     if (heat.greedy || !(s_top[node] > -INFINITY)) {
         if (threadIdx.x == 0) a.out_tok[t0 + acc] = s_best[node];     // -1 where the row has no p
@@ -390,102 +496,131 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     const float* z = a.logits + (int64_t)(t0 + node) * a.ld;
     const Part* part = sp.part + (int64_t)(t0 + node) * nch;
     const float top = s_top[node];
-    const bool without = !a.q && turned >= 0;
-    auto values = [&](int c, double* m) {
-        float x[16];
-        load16(z, c, V, -INFINITY, x);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m[i] = weight(x[i], top, heat.by);
-    };
-    auto values_without = [&](int c, double* m) {
-        values(c, m);
-        for (int j = node + 1; j <= turned; ++j) {
-            if (s_parent[j] != node || s_tok[j] < 0 || s_tok[j] >= V || s_tok[j] / VF_CHUNK != c) continue;
-            const int x = s_tok[j] % VF_CHUNK;
-            if (lane == (x >> 2 & 63))
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (i == (x >> 8) * 4 + (x & 3)) m[i] = 0;
-        }
-    };
-    auto mass = [&](int c) { return part[c].sum * weight(part[c].top, top, heat.by); };
+    double* own = nch <= VF_TH ? s_mass : sp.mass + (int64_t)b * nch;
     int pick = -1;
-    if (without) {
-        double* own = sp.mass + (int64_t)b * nch;
-        for (int c = threadIdx.x; c < nch; c += VF_TH) own[c] = mass(c);
-        __syncthreads();
-        for (int j = node + 1 + w; j <= turned; j += VF_TH / 64) {
-            if (s_parent[j] != node || s_tok[j] < 0 || s_tok[j] >= V) continue;
-            const int c = s_tok[j] / VF_CHUNK;
-            double m[16], s = 0;
-            values_without(c, m);                      // of two tokens in a chunk either writes the same
+    // the second pass, where nothing was left, is from p itself
+    for (int without = !a.q && turned >= 0; without >= 0 && pick < 0; --without) {
+        auto taken = [&](int j) { return s_parent[j] == node && s_tok[j] >= 0 && s_tok[j] < V; };
+        auto values = [&](int at, double* m) {
+            float x[4];
+            load4(z, at, V, -INFINITY, x);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s += m[i];
-            s = wave_sum_f64(s);
-            if (lane == 0) own[c] = s;
-        }
+            for (int i = 0; i < 4; ++i) m[i] = weight(x[i], top, heat.by);
+            if (without)
+                for (int j = node + 1; j <= turned; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (taken(j) && s_tok[j] == at + i) m[i] = 0;
+        };
+        for (int c = threadIdx.x; c < nch; c += VF_TH) own[c] = part[c].sum * weight(part[c].top, top, heat.by);
         __syncthreads();
-        pick = pick_token(nch, a.u_next[b], [&](int c) { return own[c]; }, values_without, s_part);
+        if (without) {
+            for (int j = node + 1 + w; j <= turned; j += VF_TH / 64) {
+                if (!taken(j)) continue;
+                const int c = s_tok[j] / VF_CHUNK;
+                double s = 0;
+#pragma unroll 1
+                for (int k = 0; k < 4; ++k) {          // of two tokens in a chunk either writes the same
+                    double m[4];
+                    values(place(c, 4 * k), m);
+                    s += (m[0] + m[1]) + (m[2] + m[3]);
+                }
+                s = wave_sum_f64(s);
+                if (lane == 0) own[c] = s;
+            }
+            __syncthreads();
+        }
+        pick = pick_token<VF_TH>(nch, u_next, [&](int c) { return own[c]; }, values, s_part);
         __syncthreads();
     }
-    if (pick < 0) pick = pick_token(nch, a.u_next[b], mass, values, s_part);
     if (threadIdx.x == 0) a.out_tok[t0 + acc] = pick;
 }
-// What p has more than q, a wave per chunk: the sums.
-__device__ __forceinline__ void more_than(const VerifyArgs& a, const Next& nx, double by, int c, double* m) {
-    float x[16], y[16];
-    load16(a.logits + (int64_t)nx.row * a.ld, c, a.V, -INFINITY, x);
-    load16(a.q + (int64_t)nx.turned * a.q_ld, c, a.V, 0.f, y);
-    const double share = 1.0 / nx.sum;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m[i] = fmax(fma(weight(x[i], nx.top, by), share, -(double)y[i]), 0.0);
-}
-__global__ __launch_bounds__(256) void verify_less_kernel(VerifyArgs a) {
+
+// What p has more than q: the chunks' masses, a wave each, and by the last workgroup
+// of a sequence the token.  The masses pass between workgroups of other XCDs, so they
+// and the count of workgroups are written and read past the L2 (relaxed atomics of the
+// device's scope; a workgroup's count follows its masses by the wait between them).
+constexpr int VL_TH = 256;
+__global__ __launch_bounds__(VL_TH) void verify_less_kernel(VerifyArgs a) {
+    __shared__ double s_part[VL_TH / 64];
+    __shared__ int s_done;
     const int nch = chunks_of(a.V), b = blockIdx.y;
-    const int c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    const Space sp = space_of(a);
-    const Next nx = sp.next[b];
-    if (c >= nch || nx.turned < 0) return;
-    double m[16], s = 0;
-    more_than(a, nx, heat_of(a.temperature, b).by, c, m);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += m[i];
-    s = wave_sum_f64(s);
-    if ((threadIdx.x & 63) == 0) sp.mass[(int64_t)b * nch + c] = s;
-}
-__global__ __launch_bounds__(VF_TH) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ double s_part[VF_TH / 64];
-    const int nch = chunks_of(a.V), b = blockIdx.x;
+    const int c = __builtin_amdgcn_readfirstlane(blockIdx.x * (VL_TH / 64) + (threadIdx.x >> 6));
     const Space sp = space_of(a);
     const Next nx = sp.next[b];
     if (nx.turned < 0) return;
-    const double by = heat_of(a.temperature, b).by;
-    const double* own = sp.mass + (int64_t)b * nch;
-    int pick = pick_token(nch, a.u_next[b], [&](int c) { return own[c]; },
-                          [&](int c, double* m) { more_than(a, nx, by, c, m); }, s_part);
-    if (pick < 0) {                                    // p has nothing more than q: from p
-        __syncthreads();
-        const Part* part = sp.part + (int64_t)nx.row * nch;
-        pick = pick_token(nch, a.u_next[b], [&](int c) { return part[c].sum * weight(part[c].top, nx.top, by); },
-                          [&](int c, double* m) {
-                              float x[16];
-                              load16(a.logits + (int64_t)nx.row * a.ld, c, a.V, -INFINITY, x);
+    const double by = heat_of(a.temperature, b).by, share = 1.0 / nx.sum;
+    const float *z = a.logits + (int64_t)nx.row * a.ld, *q = a.q + (int64_t)nx.turned * a.q_ld;
+    double* own = sp.mass + (int64_t)b * nch;
+    auto more = [&](double w, float y) { return fmax(fma(w, share, -(double)y), 0.0); };
+    if (c < nch) {
+        float x[16], y[16], top = -INFINITY;
+        load16(z, c, a.V, -INFINITY, x);
+        load16(q, c, a.V, INFINITY, y);
+        double s = 0;
+        Weights weights;
+        weights.start(by);
 #pragma unroll
-                              for (int i = 0; i < 16; ++i) m[i] = weight(x[i], nx.top, by);
-                          },
-                          s_part);
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+        if (nx.top == 0.f && weights.takes(top)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const double wt = weights(x[i]);       // by all lanes
+                s += more(x[i] > -INFINITY ? wt : 0.0, y[i]);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+                s += more(weight(x[0], nx.top, by), y[0]);
+#pragma unroll
+                for (int k = 0; k < 15; ++k) {
+                    x[k] = x[k + 1];
+                    y[k] = y[k + 1];
+                }
+            }
+        }
+        s = wave_sum_f64(s);
+        if ((threadIdx.x & 63) == 0) __hip_atomic_store(own + c, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        s_done = __hip_atomic_fetch_add(&sp.next[b].done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (s_done != (int)gridDim.x - 1) return;
+    const Part* part = sp.part + (int64_t)nx.row * nch;
+    int pick = -1;
+    for (int less = 1; less >= 0 && pick < 0; --less) {        // where p has nothing more than q: from p
+        __syncthreads();
+        pick = pick_token<VL_TH>(
+            nch, a.u_next[b],
+            [&](int i) {
+                return less ? __hip_atomic_load(own + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                            : part[i].sum * weight(part[i].top, nx.top, by);
+            },
+            [&](int at, double* m) {
+                float x[4], y[4];
+                load4(z, at, a.V, -INFINITY, x);
+                load4(q, at, a.V, INFINITY, y);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    m[i] = weight(x[i], nx.top, by);
+                    if (less) m[i] = more(m[i], y[i]);
+                }
+            },
+            s_part);
     }
     if (threadIdx.x == 0) a.out_tok[nx.at] = pick;
 }
 
 int launch_verify_drafts(const VerifyArgs& a, hipStream_t s) {
     const int groups = (chunks_of(a.V) + 3) / 4;
-    hipLaunchKernelGGL(verify_sums_kernel, dim3(groups, min(a.T, 65535)), dim3(256), 0, s, a);
+    // about four waves a SIMD; a wave's rows follow each other
+    const int stretches = max(1, min(min(a.T, 65535), VF_SUM_WGS / groups));
+    hipLaunchKernelGGL(verify_sums_kernel, dim3(groups, stretches), dim3(256), 0, s, a);
     hipLaunchKernelGGL(verify_walk_kernel, dim3(a.B), dim3(VF_TH), 0, s, a);
-    if (a.q) {
-        hipLaunchKernelGGL(verify_less_kernel, dim3(groups, a.B), dim3(256), 0, s, a);
-        hipLaunchKernelGGL(verify_pick_kernel, dim3(a.B), dim3(VF_TH), 0, s, a);
-    }
+    if (a.q) hipLaunchKernelGGL(verify_less_kernel, dim3(groups, a.B), dim3(VL_TH), 0, s, a);
     SH_CHECK_LAUNCH();
     return 0;
 }
