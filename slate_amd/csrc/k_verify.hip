@@ -19,7 +19,10 @@ namespace slate_hip {
 
 constexpr int VF_CHUNK = 1024;         // logits of a wave: 16 a lane
 constexpr int VF_TH = 512;             // threads that walk a sequence
-constexpr int VF_SUM_WGS = 1024;       // workgroups of the sums
+// Workgroups of the sums: five waves a SIMD.  256 rows of 128256 logits take 34.4 us (3.8
+// TB/s; 27.5 with no exponentials), 35.8 with four, 38 with six, 47 with eight, which
+// leave the compiler fewer registers.
+constexpr int VF_SUM_WGS = 1280;
 constexpr int VF_ROWS = PK_MAX_DRAFT + 1;
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -195,9 +198,22 @@ int64_t verify_drafts_bytes(int B, int T, int V) {
     return T * nch * (int64_t)sizeof(Part) + B * nch * (int64_t)sizeof(double) + B * (int64_t)sizeof(Next);
 }
 
+// The weights of a lane's 16 logits, one after the other (in few instructions: what
+// runs once is as long as it is fetched).
+__device__ __forceinline__ double weights_of(float* x, float top, double by) {
+    double s = 0;
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+        s += weight(x[0], top, by);
+#pragma unroll
+        for (int k = 0; k < 15; ++k) x[k] = x[k + 1];
+    }
+    return s;
+}
+
 // Softmax sums (greedy rows: the largest logit) of all rows, a wave per chunk of a
 // stretch of rows, the next row's logits under way while it works on the last.
-__global__ __launch_bounds__(256, 4) void verify_sums_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(256, 5) void verify_sums_kernel(VerifyArgs a) {
     const int lane = threadIdx.x & 63, nch = chunks_of(a.V);
     const int c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (c >= nch) return;
@@ -249,14 +265,7 @@ __global__ __launch_bounds__(256, 4) void verify_sums_kernel(VerifyArgs a) {
                     if (x[i] == top) at = place(c, i);
                 p.best = wave_min_int(at);
             } else {
-                double s = 0;
-#pragma unroll 1
-                for (int i = 0; i < 16; ++i) {
-                    s += weight(x[0], top, heat.by);
-#pragma unroll
-                    for (int k = 0; k < 15; ++k) x[k] = x[k + 1];
-                }
-                p.sum = wave_sum_f64(s);
+                p.sum = wave_sum_f64(weights_of(x, top, heat.by));
             }
         }
         if (lane == 0) sp.part[(int64_t)t * nch + c] = p;
@@ -504,27 +513,27 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
         auto values = [&](int at, double* m) {
             float x[4];
             load4(z, at, V, -INFINITY, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m[i] = weight(x[i], top, heat.by);
             if (without)
                 for (int j = node + 1; j <= turned; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (taken(j) && s_tok[j] == at + i) m[i] = 0;
+                        if (taken(j) && s_tok[j] == at + i) x[i] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = weight(x[i], top, heat.by);
         };
         for (int c = threadIdx.x; c < nch; c += VF_TH) own[c] = part[c].sum * weight(part[c].top, top, heat.by);
         __syncthreads();
         if (without) {
             for (int j = node + 1 + w; j <= turned; j += VF_TH / 64) {
                 if (!taken(j)) continue;
-                const int c = s_tok[j] / VF_CHUNK;
-                double s = 0;
-#pragma unroll 1
-                for (int k = 0; k < 4; ++k) {          // of two tokens in a chunk either writes the same
-                    double m[4];
-                    values(place(c, 4 * k), m);
-                    s += (m[0] + m[1]) + (m[2] + m[3]);
-                }
+                const int c = s_tok[j] / VF_CHUNK;     // of two tokens in a chunk either writes the same
+                float x[16];
+                load16(z, c, V, -INFINITY, x);
+                for (int k = node + 1; k <= turned; ++k)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (taken(k) && s_tok[k] == place(c, i)) x[i] = -INFINITY;
+                double s = weights_of(x, top, heat.by);
                 s = wave_sum_f64(s);
                 if (lane == 0) own[c] = s;
             }
@@ -616,7 +625,7 @@ __global__ __launch_bounds__(VL_TH) void verify_less_kernel(VerifyArgs a) {
 
 int launch_verify_drafts(const VerifyArgs& a, hipStream_t s) {
     const int groups = (chunks_of(a.V) + 3) / 4;
-    // about four waves a SIMD; a wave's rows follow each other
+    // a wave's rows follow each other
     const int stretches = max(1, min(min(a.T, 65535), VF_SUM_WGS / groups));
     hipLaunchKernelGGL(verify_sums_kernel, dim3(groups, stretches), dim3(256), 0, s, a);
     hipLaunchKernelGGL(verify_walk_kernel, dim3(a.B), dim3(VF_TH), 0, s, a);
