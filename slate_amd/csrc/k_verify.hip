@@ -50,9 +50,9 @@ __device__ __forceinline__ double pow2(double t) {
 // it) 0: e^((x - top) / temperature), by = log2(e) / temperature.  0 for -infinity;
 // infinite logits share all.
 __device__ __forceinline__ double weight(float x, float top, double by) {
-    if (!(x > -INFINITY)) return 0;
-    if (x == top) return 1;
-    return top == INFINITY ? 0 : pow2(((double)x - (double)top) * by);
+    double w = pow2(((double)x - (double)top) * by);   // selects: branches would keep several from overlapping
+    w = top == INFINITY || !(x > -INFINITY) ? 0.0 : w;
+    return x == top && top > -INFINITY ? 1.0 : w;
 }
 
 // The same beside 0 instead of the largest logit, for sums over whole rows: 64 bits hold
@@ -198,15 +198,15 @@ int64_t verify_drafts_bytes(int B, int T, int V) {
     return T * nch * (int64_t)sizeof(Part) + B * nch * (int64_t)sizeof(double) + B * (int64_t)sizeof(Next);
 }
 
-// The weights of a lane's 16 logits, one after the other (in few instructions: what
-// runs once is as long as it is fetched).
+// The weights of a lane's 16 logits, four at a time (in few instructions: what runs
+// once takes as long as it is fetched).
 __device__ __forceinline__ double weights_of(float* x, float top, double by) {
     double s = 0;
 #pragma unroll 1
-    for (int i = 0; i < 16; ++i) {
-        s += weight(x[0], top, by);
+    for (int i = 0; i < 4; ++i) {
+        s += (weight(x[0], top, by) + weight(x[1], top, by)) + (weight(x[2], top, by) + weight(x[3], top, by));
 #pragma unroll
-        for (int k = 0; k < 15; ++k) x[k] = x[k + 1];
+        for (int k = 0; k < 12; ++k) x[k] = x[k + 4];
     }
     return s;
 }
