@@ -5,8 +5,12 @@
 
 namespace slate_hip {
 
-constexpr int PGS_TH = 1024;           // threads of the one workgroup: a sequence each
+constexpr int PGS_MAX_TH = 1024;       // threads of the one workgroup: a sequence each
+constexpr int PGS_FEW = 256;           // up to as many sequences in a workgroup of as many threads
 constexpr int PGS_HASH = 2048;
+// Tokens whose rows the workgroup that takes the pages finds itself; more are left to
+// workgroups of their own, as many as T_cap could need.
+constexpr int PGS_OWN_TOKENS = 2048;
 
 // Sums over the workgroup, each thread bringing a count below 2^31: the
 // inclusive one up to the thread (below 2^31 if the whole is), and the whole.
@@ -14,6 +18,7 @@ struct Scan {
     int upto;
     int64_t total;
 };
+template <int TH>
 __device__ __forceinline__ Scan block_scan(int v, int64_t* s_part) {
     const int w = threadIdx.x >> 6;
     const int upto = wave_scan(v);
@@ -22,11 +27,11 @@ __device__ __forceinline__ Scan block_scan(int v, int64_t* s_part) {
     if ((threadIdx.x & 63) == 0) s_part[w] = whole;
     __syncthreads();
     int64_t before = 0, total = 0;
-    for (int i = 0; i < PGS_TH / 64; ++i) {
+#pragma unroll
+    for (int i = 0; i < TH / 64; ++i) {
         before += i < w ? s_part[i] : 0;
         total += s_part[i];
     }
-    __syncthreads();
     return Scan{(int)before + upto, total};
 }
 
@@ -65,45 +70,53 @@ __global__ __launch_bounds__(256) void pages_reset_kernel(Pages pg) {
     if (i0 == 0) pg.n_free[0] = pg.n_pages;
 }
 
-// Two sums over the sequences (tokens, new pages); then a thread per new page
-// and per token finds its sequence in them.
-__global__ __launch_bounds__(PGS_TH) void pages_extend_kernel(Pages pg, const int32_t* __restrict__ slot,
-                                                              const int32_t* __restrict__ pos0,
-                                                              const int32_t* __restrict__ n_new, int B, int T_cap,
-                                                              int32_t* __restrict__ tok_off,
-                                                              int32_t* __restrict__ tok2seq,
-                                                              int32_t* __restrict__ tok_pos,
-                                                              int32_t* __restrict__ tok_row,
-                                                              int32_t* __restrict__ last_tok,
-                                                              int32_t* __restrict__ status) {
-    __shared__ int s_hash[PGS_HASH], s_slot[PGS_TH], s_pos0[PGS_TH], s_held[PGS_TH], s_tok[PGS_TH], s_page[PGS_TH];
-    __shared__ int64_t s_part[PGS_TH / 64];
+// The cache row of position pos of a slot, -1 where its page is none.
+__device__ __forceinline__ int row_at(const Pages& pg, int page, int in) {
+    return (unsigned)page < (unsigned)pg.n_pages ? page * pg.page_size + in : -1;
+}
+
+// Two sums over the sequences (tokens, new pages); then a thread per new page and per
+// token finds its sequence in them.  Latency: three rounds of loads one after the other
+// (descriptors, held, pages: a token's page comes from the table or from the stack that
+// the table is filled from, so nothing waits for what was written) in 4 us for 64
+// sequences.
+template <int TH>
+__global__ __launch_bounds__(TH) void pages_extend_kernel(Pages pg, const int32_t* __restrict__ slot,
+                                                          const int32_t* __restrict__ pos0,
+                                                          const int32_t* __restrict__ n_new, int B, int T_cap,
+                                                          int32_t* __restrict__ tok_off, int32_t* __restrict__ tok2seq,
+                                                          int32_t* __restrict__ tok_pos, int32_t* __restrict__ tok_row,
+                                                          int32_t* __restrict__ last_tok,
+                                                          int32_t* __restrict__ status) {
+    __shared__ int s_hash[PGS_HASH], s_slot[TH], s_pos0[TH], s_held[TH], s_tok[TH], s_page[TH];
+    __shared__ int64_t s_part[2][TH / 64];
     __shared__ int s_err;
     const int b = threadIdx.x;
-    for (int i = b; i < PGS_HASH; i += PGS_TH) s_hash[i] = -1;
-    if (b == 0) s_err = 0;
-    __syncthreads();
     const int n_free = pg.n_free[0];
     int sl = 0, p0 = 0, n = 0, held = 0, fresh = 0;
     if (b < B) {
         sl = slot[b];
         p0 = pos0[b];
         n = n_new[b];
-        bool bad = sl < 0 || sl >= pg.n_slots || p0 < 0 || n < 0 || n_free < 0 || n_free > pg.n_pages;
-        if (!bad) {
-            held = pg.held[sl];
-            bad = seen_before(s_hash, sl) || held < 0 || held > pg.max_pages;
-        }
+    }
+    const bool in = sl >= 0 && sl < pg.n_slots;
+    if (b < B && in) held = pg.held[sl];
+    for (int i = b; i < PGS_HASH; i += TH) s_hash[i] = -1;
+    if (b == 0) s_err = 0;
+    __syncthreads();
+    if (b < B) {
+        bool bad = !in || p0 < 0 || n < 0 || n_free < 0 || n_free > pg.n_pages || held < 0 || held > pg.max_pages;
+        if (in) bad |= seen_before(s_hash, sl);
         const int64_t rows = (int64_t)p0 + n;
         if (bad)
             atomicOr(&s_err, 1);
         else if (rows > (int64_t)pg.max_pages * pg.page_size)
             atomicOr(&s_err, 2);
         else
-            fresh = max(0, (int)((rows + pg.page_size - 1) / pg.page_size) - held);
+            fresh = max(0, (int)((unsigned)((int)rows + pg.page_size - 1) / (unsigned)pg.page_size) - held);
         n = max(n, 0);
     }
-    const Scan tok = block_scan(n, s_part), page = block_scan(fresh, s_part);
+    const Scan tok = block_scan<TH>(n, s_part[0]), page = block_scan<TH>(fresh, s_part[1]);
     s_slot[b] = sl;
     s_pos0[b] = p0;
     s_held[b] = held;
@@ -122,49 +135,79 @@ __global__ __launch_bounds__(PGS_TH) void pages_extend_kernel(Pages pg, const in
         if (fresh > 0) pg.held[sl] = held + fresh;
     }
     if (b == 0) pg.n_free[0] = n_free - new_pages;
-    for (int k = threadIdx.x; k < new_pages; k += PGS_TH) {
+    for (int k = threadIdx.x; k < new_pages; k += TH) {
         const int s = find_above(s_page, B, k), first = s > 0 ? s_page[s - 1] : 0;
         pg.table[(int64_t)s_slot[s] * pg.max_pages + s_held[s] + (k - first)] = pg.free_pages[n_free - 1 - k];
     }
-    __syncthreads();
-    for (int t = threadIdx.x; t < T; t += PGS_TH) {
+    if (T > PGS_OWN_TOKENS) return;
+    for (int t = threadIdx.x; t < T; t += TH) {
         const int s = find_above(s_tok, B, t), first = s > 0 ? s_tok[s - 1] : 0;
-        const int pos = s_pos0[s] + (t - first), i = pos / pg.page_size;
-        const int pno = pg.table[(int64_t)s_slot[s] * pg.max_pages + i];
+        const int pos = s_pos0[s] + (t - first), i = (int)((unsigned)pos / (unsigned)pg.page_size), own = i - s_held[s];
+        const int pno = own < 0 ? pg.table[(int64_t)s_slot[s] * pg.max_pages + i]
+                                : pg.free_pages[n_free - 1 - (s > 0 ? s_page[s - 1] : 0) - own];
         tok2seq[t] = s;
         tok_pos[t] = pos;
-        tok_row[t] = (unsigned)pno < (unsigned)pg.n_pages ? pno * pg.page_size + (pos - i * pg.page_size) : -1;
+        tok_row[t] = row_at(pg, pno, pos - i * pg.page_size);
     }
 }
 
-__global__ __launch_bounds__(PGS_TH) void pages_trim_kernel(Pages pg, const int32_t* __restrict__ slot,
-                                                            const int32_t* __restrict__ length, int B,
-                                                            int32_t* __restrict__ status) {
-    __shared__ int s_hash[PGS_HASH], s_slot[PGS_TH], s_keep[PGS_TH], s_page[PGS_TH];
-    __shared__ int64_t s_part[PGS_TH / 64];
+// The same for the tokens of a large batch: its offsets in LDS, a token a thread and round.
+constexpr int PGS_TOK_TH = 256, PGS_TOK = 4;
+__global__ __launch_bounds__(PGS_TOK_TH) void pages_tokens_kernel(Pages pg, const int32_t* __restrict__ slot,
+                                                                  const int32_t* __restrict__ pos0, int B,
+                                                                  const int32_t* __restrict__ tok_off,
+                                                                  int32_t* __restrict__ tok2seq,
+                                                                  int32_t* __restrict__ tok_pos,
+                                                                  int32_t* __restrict__ tok_row,
+                                                                  const int32_t* __restrict__ status) {
+    __shared__ int s_tok[PK_MAX_SEQ];                  // the sequences' ends
+    if (status[0] != 0) return;                        // tok_off is not this call's
+    const int T = tok_off[B], t0 = blockIdx.x * (PGS_TOK_TH * PGS_TOK);
+    if (T <= PGS_OWN_TOKENS || t0 >= T) return;
+    for (int b = threadIdx.x; b < B; b += PGS_TOK_TH) s_tok[b] = tok_off[b + 1];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PGS_TOK; ++k) {
+        const int t = t0 + PGS_TOK_TH * k + threadIdx.x;
+        if (t >= T) break;
+        const int s = find_above(s_tok, B, t), first = s > 0 ? s_tok[s - 1] : 0;
+        const int pos = pos0[s] + (t - first), i = (int)((unsigned)pos / (unsigned)pg.page_size);
+        tok2seq[t] = s;
+        tok_pos[t] = pos;
+        tok_row[t] = row_at(pg, pg.table[(int64_t)slot[s] * pg.max_pages + i], pos - i * pg.page_size);
+    }
+}
+
+template <int TH>
+__global__ __launch_bounds__(TH) void pages_trim_kernel(Pages pg, const int32_t* __restrict__ slot,
+                                                        const int32_t* __restrict__ length, int B,
+                                                        int32_t* __restrict__ status) {
+    __shared__ int s_hash[PGS_HASH], s_slot[TH], s_keep[TH], s_page[TH];
+    __shared__ int64_t s_part[TH / 64];
     __shared__ int s_err;
     const int b = threadIdx.x;
-    for (int i = b; i < PGS_HASH; i += PGS_TH) s_hash[i] = -1;
-    if (b == 0) s_err = 0;
-    __syncthreads();
     const int n_free = pg.n_free[0];
-    int sl = 0, keep = 0, back = 0;
+    int sl = 0, len = 0, held = 0, keep = 0, back = 0;
     if (b < B) {
         sl = slot[b];
-        const int len = length[b];
-        bool bad = sl < 0 || sl >= pg.n_slots || len < 0 || n_free < 0 || n_free > pg.n_pages;
-        if (!bad) {
-            const int held = pg.held[sl];
-            bad = seen_before(s_hash, sl) || held < 0 || held > pg.max_pages;
-            keep = min(held, (int)(((int64_t)len + pg.page_size - 1) / pg.page_size));
-            back = held - keep;
-        }
+        len = length[b];
+    }
+    const bool in = sl >= 0 && sl < pg.n_slots;
+    if (b < B && in) held = pg.held[sl];
+    for (int i = b; i < PGS_HASH; i += TH) s_hash[i] = -1;
+    if (b == 0) s_err = 0;
+    __syncthreads();
+    if (b < B) {
+        bool bad = !in || len < 0 || n_free < 0 || n_free > pg.n_pages || held < 0 || held > pg.max_pages;
+        if (in) bad |= seen_before(s_hash, sl);
+        keep = min(held, (int)(((unsigned)len + (unsigned)pg.page_size - 1) / (unsigned)pg.page_size));
+        back = held - keep;
         if (bad) {
             atomicOr(&s_err, 1);
             back = 0;
         }
     }
-    const Scan page = block_scan(back, s_part);
+    const Scan page = block_scan<TH>(back, s_part);
     s_slot[b] = sl;
     s_keep[b] = keep;
     s_page[b] = page.upto;
@@ -176,7 +219,7 @@ __global__ __launch_bounds__(PGS_TH) void pages_trim_kernel(Pages pg, const int3
     const int total = (int)page.total;
     if (b < B && back > 0) pg.held[sl] = keep;
     if (b == 0) pg.n_free[0] = n_free + total;
-    for (int k = threadIdx.x; k < total; k += PGS_TH) {
+    for (int k = threadIdx.x; k < total; k += TH) {
         const int s = find_above(s_page, B, k), first = s > 0 ? s_page[s - 1] : 0;
         int32_t* cell = pg.table + (int64_t)s_slot[s] * pg.max_pages + s_keep[s] + (k - first);
         pg.free_pages[n_free + total - 1 - k] = *cell;
@@ -223,15 +266,26 @@ int launch_pages_reset(const Pages& pg, hipStream_t s) {
 int launch_pages_extend(const Pages& pg, const int32_t* slot, const int32_t* pos0, const int32_t* n_new, int B,
                         int T_cap, int32_t* tok_off, int32_t* tok2seq, int32_t* tok_pos, int32_t* tok_row,
                         int32_t* last_tok, int32_t* status, hipStream_t s) {
-    hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(PGS_TH), 0, s, pg, slot, pos0, n_new, B, T_cap, tok_off,
-                       tok2seq, tok_pos, tok_row, last_tok, status);
+    if (B <= PGS_FEW)
+        hipLaunchKernelGGL(pages_extend_kernel<PGS_FEW>, dim3(1), dim3(PGS_FEW), 0, s, pg, slot, pos0, n_new, B, T_cap,
+                           tok_off, tok2seq, tok_pos, tok_row, last_tok, status);
+    else
+        hipLaunchKernelGGL(pages_extend_kernel<PGS_MAX_TH>, dim3(1), dim3(PGS_MAX_TH), 0, s, pg, slot, pos0, n_new, B,
+                           T_cap, tok_off, tok2seq, tok_pos, tok_row, last_tok, status);
+    constexpr int PER = PGS_TOK_TH * PGS_TOK;
+    if (T_cap > PGS_OWN_TOKENS)
+        hipLaunchKernelGGL(pages_tokens_kernel, dim3((unsigned)(((int64_t)T_cap + PER - 1) / PER)), dim3(PGS_TOK_TH), 0, s,
+                           pg, slot, pos0, B, tok_off, tok2seq, tok_pos, tok_row, status);
     SH_CHECK_LAUNCH();
     return 0;
 }
 
 int launch_pages_trim(const Pages& pg, const int32_t* slot, const int32_t* length, int B, int32_t* status,
                       hipStream_t s) {
-    hipLaunchKernelGGL(pages_trim_kernel, dim3(1), dim3(PGS_TH), 0, s, pg, slot, length, B, status);
+    if (B <= PGS_FEW)
+        hipLaunchKernelGGL(pages_trim_kernel<PGS_FEW>, dim3(1), dim3(PGS_FEW), 0, s, pg, slot, length, B, status);
+    else
+        hipLaunchKernelGGL(pages_trim_kernel<PGS_MAX_TH>, dim3(1), dim3(PGS_MAX_TH), 0, s, pg, slot, length, B, status);
     SH_CHECK_LAUNCH();
     return 0;
 }
