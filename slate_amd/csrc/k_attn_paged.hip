@@ -1,692 +1,25 @@
-// k_attn_paged.hip -- causal attention of new tokens over a K/V cache in pages.
-//
-// out = sum_k exp(s_k - m) V_k / sum_k exp(s_k - m), s_k = q.K_k / sqrt(hd),
-// over the rows 0 .. pos0 + i of the token's slot.
-//
-//   S^T [keys x 16 rows] = K Q^T,   O^T [hd x 16 rows] += V^T P^T
-//
-// Few query rows meet many keys, so the bytes of K and V bound it.  A workgroup
-// takes a block of 16 RT rows over a range of keys (attn_plan.h), each of its
-// four waves every fourth 32 of them.  K and V go from memory straight into the
-// registers that the MFMA takes them from, with no LDS and no barrier until the
-// range ends; the next keys' loads are under way while a wave works.  That needs
-// no transposition between lanes, as the order of a product's terms is free:
-//  - K: lane (g, j) = (lane / 16, lane % 16) reads 16 bytes g of each 64 of key j's
-//    row, and Q is laid out alike;
-//  - S^T leaves the keys 4g + i of row j in lane (g, j), so V's products take
-//    lane g's keys from there: its lanes read those keys' rows, CW columns each,
-//    whole rows of memory, and columns CW apart share an MFMA.
-// f16: Q (scaled by a power of two) and the weights (times 2^11) as two halves, 22
-// bits; bf16: as three, 24 bits; f32: f32 MFMAs.  Sums are f32.  A row's running
-// maximum moves only when a score passes it by 2^4.
-#include "attn_plan.h"
-#include "attn_rows.h"
-#include "paged.h"
+// k_attn_paged.hip -- attention over a K/V cache in pages: its workspace, the choice
+// of the type's kernels, and those of f32 caches.  How they work: attn_paged.h.
+#include "attn_paged.h"
 
 namespace slate_hip {
 
-// Workgroups: two per CU, one where K and V of a step fill half of the registers.
-__host__ __device__ constexpr int paged_wgs(int hd) { return hd > 128 ? 256 : 512; }
-constexpr int AP_SLICE = 32;           // keys of a wave within a granule
-constexpr int AP_GRAN = 4 * AP_SLICE;  // keys of a granule
-constexpr int AP_KEEP = 4;             // blocks of up to this many granules are not cut
-
-typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
-typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-
-__host__ __device__ constexpr int paged_granules(int keys) { return (keys + AP_GRAN - 1) / AP_GRAN; }
-
-template <int RT>
-struct PagedCount {
-    int G, Hkv;
-    __device__ __forceinline__ int blocks(const SeqView& s) const { return (s.n * G + 16 * RT - 1) / (16 * RT); }
-    __device__ __forceinline__ int operator()(const SeqView& s) const {
-        return s.n < 1 ? 0 : Hkv * blocks(s) * paged_granules(s.p0 + s.n);
-    }
-};
-
-// Where workgroup w's range begins: N w / P, or the start of the block there
-// if it is short.
-template <int WGS, class PlanT>
-__device__ __forceinline__ int paged_begin(const PlanT& plan, int w) {
-    const int x = plan.begin(w, WGS);
-    if (x >= plan.total) return plan.total;
-    const Place pl = plan.find(x);
-    const int gran = paged_granules(pl.seq.p0 + pl.seq.n), in = pl.at % gran;
-    return gran <= AP_KEEP ? x - in : x;
+int64_t attention_paged_bytes(int hd) {
+    return plan_bytes(paged_wgs(hd), hd <= 128 ? 64 : 32, hd <= 64 ? 64 : hd <= 128 ? 128 : 256);
 }
 
-// How a type's numbers are multiplied: NP operands stand for one f32.
-template <class E>
-struct Mul;
 template <>
-struct Mul<_Float16> {
-    static constexpr int NP = 2;
-    static constexpr float PEXP = 11;  // weights are scaled by 2^11: at most 2^15 with the slack
-    static constexpr uint32_t INF2 = 0x7c007c00, ONE = 0x3c00;
-    static __device__ __forceinline__ void split(const float* x, uint4v* p) {
-        half8_t hi, lo;
-        halves(x, hi, lo);
-        p[0] = __builtin_bit_cast(uint4v, hi);
-        p[1] = __builtin_bit_cast(uint4v, lo);
-    }
-    static __device__ __forceinline__ floatx4 mfma(uint4v a, uint4v b, floatx4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
-                                                      0, 0);
-    }
-};
-template <>
-struct Mul<__bf16> {
-    static constexpr int NP = 3;
-    static constexpr float PEXP = 0;
-    static constexpr uint32_t INF2 = 0x7f807f80, ONE = 0x3f80;
-    // cut off after 8 bits three times: exact
-    static __device__ __forceinline__ void split(const float* x, uint4v* p) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            float v[2] = {x[e], x[e + 1]};
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                const uint32_t u0 = __float_as_uint(v[0]), u1 = __float_as_uint(v[1]);
-                p[k][e / 2] = __builtin_amdgcn_perm(u1, u0, 0x07060302);
-                v[0] -= __uint_as_float(u0 & 0xffff0000u);
-                v[1] -= __uint_as_float(u1 & 0xffff0000u);
-            }
-        }
-    }
-    static __device__ __forceinline__ floatx4 mfma(uint4v a, uint4v b, floatx4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0,
-                                                       0);
-    }
-};
-template <>
-struct Mul<float> {
-    static constexpr int NP = 1;
-    static constexpr float PEXP = 0;
-    static __device__ __forceinline__ floatx4 mfma(uint4v a, uint4v b, floatx4 c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
-        return c;
-    }
-};
-
-template <class E, int HD>
-struct PagedGeom {
-    static constexpr bool F32 = sizeof(E) == 4;
-    static constexpr int KS = F32 ? 16 : 32;           // keys of a step
-    static constexpr int NT = KS / 16;                 // 16-key tiles of a step
-    static constexpr int EV = 16 / (int)sizeof(E);     // elements of 16 bytes
-    static constexpr int CK = HD / (4 * EV);           // 16-byte loads of a key's row per lane
-    static constexpr int CW = F32 || HD == 64 ? 4 : 8; // columns of V per lane and load
-    static constexpr int HH = HD / (16 * CW);          // such loads of a row
-    static constexpr int VK = KS / 4;                  // keys of V per lane
-    static constexpr int VD = CW * (int)sizeof(E) / 4; // dwords of such a load
-    static constexpr int ND = HD / 16;
-    static constexpr int NP = Mul<E>::NP;
-};
-
-// FULL: head_dim is HD (else smaller).  P16: pages hold whole 16-key tiles, so
-// that a tile's page is the same for all lanes.
-template <class E, int HD, int RT, bool FULL, bool P16>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(PagedAttn a, PagedBatch pb) {
-    using Geo = PagedGeom<E, HD>;
-    using M = Mul<E>;
-    constexpr bool F32 = Geo::F32;
-    constexpr int KS = Geo::KS, NT = Geo::NT, EV = Geo::EV, CK = Geo::CK, CW = Geo::CW, HH = Geo::HH, VK = Geo::VK;
-    constexpr int VD = Geo::VD, ND = Geo::ND, NP = Geo::NP, ROWS = 16 * RT;
-    constexpr int SUB = AP_SLICE / KS;                 // steps of a slice
-    constexpr bool QLDS = RT > 1 || HD > 128;          // Q waits in LDS
-    constexpr int WGS = paged_wgs(HD);
-    constexpr int OC = HD < 128 ? HD : 128, OS = OC + 4;   // columns of the results in LDS at a time, row stride
-    __shared__ float s_o[4][16][OS];
-    __shared__ float s_m[4][ROWS], s_l[4][ROWS];
-    __shared__ uint4v s_q[QLDS ? RT * NP * CK : 1][64];
-    const int lane = threadIdx.x & 63;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, j = lane & 15;
-    const int Hkv = a.kv.n_kv_heads, G = a.Hq / Hkv, hd = FULL ? HD : a.kv.head_dim, ps = a.pg.page_size;
-    using PlanT = Plan<PagedCount<RT>, PagedBatch>;
-    const PagedCount<RT> count{G, Hkv};
-    const PlanT plan(pb, count);
-    const int x0 = paged_begin<WGS>(plan, blockIdx.x), x1 = paged_begin<WGS>(plan, blockIdx.x + 1);
-    if (x0 >= x1) {
-        if (threadIdx.x == 0) entry_of(a.ws, blockIdx.x)->rows = 0;
-        return;
-    }
-    const float scale2 = (1.0f / sqrtf((float)hd)) * LOG2E;
-    const int64_t row_b = a.kv.row_stride * (int)sizeof(E);
-
-    struct Piece {
-        SeqView seq;
-        int h, r0, gran, g0, g1;       // kv head, first row of the block
-        const int32_t* table;
-        int64_t head_b;                // byte offset of the head
-    };
-    auto piece_at = [&](int x) {
-        const Place pl = plan.find(x);
-        Piece p;
-        p.seq = pl.seq;
-        p.gran = paged_granules(pl.seq.p0 + pl.seq.n);
-        const int nb = count.blocks(pl.seq), b = pl.at / p.gran;
-        p.h = b / nb;
-        p.r0 = ROWS * (b % nb);
-        p.g0 = pl.at % p.gran;
-        p.g1 = min(p.gran, p.g0 + (x1 - x));
-        p.table = a.pg.table + pl.base * a.pg.max_pages;
-        p.head_b = p.h * a.kv.head_stride * (int)sizeof(E);
-        return p;
-    };
-
-    // Pages.  P16: lane l has the page (-1: none) and the row within it of the
-    // wave's tile `at` + l; else of key l of a step.
-    struct Found {
-        int page, row;
-    };
-    auto look_up = [&](const Piece& p, int key) {
-        const int last = p.seq.p0 + p.seq.n - 1, k = min(key, last);
-        const int i = (int)((unsigned)k / (unsigned)ps), page = p.table[i];
-        int r = k - i * ps;
-        if (P16) r &= ~15;
-        return Found{(unsigned)page < (unsigned)a.pg.n_pages ? page : -1, r};
-    };
-    auto step_key = [&](const Piece& p, int s) { return (p.g0 + s / SUB) * AP_GRAN + w * AP_SLICE + s % SUB * KS; };
-    auto tiles_at = [&](const Piece& p, int at) {
-        const int i = at + lane, gr = min(p.g0 + (i >> 1), p.gran);
-        return look_up(p, gr * AP_GRAN + w * AP_SLICE + (i & 1) * 16);
-    };
-    // where a step's rows are: byte offsets from the head's start
-    struct Where {
-        int64_t tile[P16 ? NT : 1];    // P16: of the tiles (the same in all lanes)
-        int64_t row;                   // else: of key `lane`
-        bool good;                     // all of the step's pages are there
-        uint64_t there;                // else: which keys' are
-        bool tgood[NT];
-    };
-    Found near, far;                   // P16: pages of the tiles at tbase .., and of the 64 after them
-    int tbase = 0;
-    auto where_of = [&](const Piece& p, int s) {
-        Where wh;
-        if constexpr (P16) {
-            wh.good = true;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int i = s * NT + t - tbase;
-                const int page = __builtin_amdgcn_readlane(near.page, i), r = __builtin_amdgcn_readlane(near.row, i);
-                wh.tgood[t] = page >= 0;
-                wh.good &= page >= 0;
-                wh.tile[t] = (int64_t)max(page, 0) * (a.kv.page_stride * (int)sizeof(E)) + r * row_b;
-            }
-        } else {
-            const Found f = near;
-            wh.there = __builtin_amdgcn_ballot_w64(f.page >= 0) | ~((1ull << KS) - 1);
-            wh.good = wh.there == ~0ull;
-            wh.row = (int64_t)max(f.page, 0) * (a.kv.page_stride * (int)sizeof(E)) + f.row * row_b;
-        }
-        return wh;
-    };
-    auto from_lane = [&](int64_t v, int l) {
-        const uint32_t lo = __shfl((int)(uint32_t)v, l), hi = __shfl((int)((uint64_t)v >> 32), l);
-        return (int64_t)((uint64_t)hi << 32 | lo);
-    };
-    uint4v kr[NT][CK];
-    uint32_t vr[VK][HH][VD];
-    const uint32_t k_off = j * (uint32_t)row_b, v_off = 4 * g * (uint32_t)row_b;
-    auto load_k = [&](const Piece& p, const Where& wh) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const char* base;
-            uint32_t off = 0;
-            if constexpr (P16) {
-                base = uniform((const char*)a.kv.K + p.head_b + wh.tile[t]);
-                off = k_off;
-            } else {
-                base = (const char*)a.kv.K + p.head_b + from_lane(wh.row, 16 * t + j);
-            }
-#pragma unroll
-            for (int c = 0; c < CK; ++c) {
-                int e = 4 * EV * c + EV * g;
-                if (!FULL) e = e < hd ? e : 0;         // there Q is 0
-                kr[t][c] = *(const uint4v*)(base + off + e * (int)sizeof(E));
-            }
-        }
-    };
-    auto load_v = [&](const Piece& p, const Where& wh) {
-#pragma unroll
-        for (int i = 0; i < VK; ++i) {
-            const char* base;
-            uint32_t off = 0;
-            if constexpr (P16) {
-                base = uniform((const char*)a.kv.V + p.head_b + wh.tile[i / 4] + (i % 4) * row_b);
-                off = v_off;
-            } else {
-                base = (const char*)a.kv.V + p.head_b + from_lane(wh.row, 16 * (i / 4) + 4 * g + i % 4);
-            }
-#pragma unroll
-            for (int hh = 0; hh < HH; ++hh) {
-                int d = 16 * CW * hh + CW * j;
-                if (!FULL) d = d < hd ? d : 0;         // columns that are not written out
-                const char* at = base + off + d * (int)sizeof(E);
-                if constexpr (VD == 4) {
-                    const uint4v x = *(const uint4v*)at;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) vr[i][hh][e] = x[e];
-                } else {
-                    const uint2v x = *(const uint2v*)at;
-                    vr[i][hh][0] = x[0];
-                    vr[i][hh][1] = x[1];
-                }
-            }
-        }
-    };
-
-    uint4v qr[QLDS ? 1 : NP][QLDS ? 1 : CK];
-    float unq[RT];
-    // Q of the block's rows as the B operand, elements as K's loads have them
-    auto load_q = [&](const Piece& p) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int r = p.r0 + 16 * rt + j;
-            const bool live = r < p.seq.n * G;
-            const float* qp =
-                a.q + ((int64_t)(p.seq.t0 + (live ? r / G : 0)) * a.Hq + p.h * G + (live ? r % G : 0)) * hd;
-            float x[CK][EV], top = 0.f;
-#pragma unroll
-            for (int c = 0; c < CK; ++c) {
-                const int e0 = 4 * EV * c + EV * g;
-                const bool in = live && (FULL || e0 < hd);
-#pragma unroll
-                for (int e = 0; e < EV; e += 4) {
-                    const float4u v = *(const float4u*)(qp + (FULL || e0 < hd ? e0 : 0) + e);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        x[c][e + k] = in ? v[k] * scale2 : 0.f;
-                        top = fmaxf(top, fabsf(x[c][e + k]));
-                    }
-                }
-            }
-            unq[rt] = 1.0f;
-            if constexpr (NP == 2) {                   // to [2^13, 2^14) at the row's largest: lo keeps its bits
-                top = cols_max(top);
-                const int e2 = top > 0.f ? min(126, 14 - __builtin_amdgcn_frexp_expf(top)) : 0;
-                unq[rt] = ldexpf(1.0f, -e2);
-#pragma unroll
-                for (int c = 0; c < CK; ++c)
-#pragma unroll
-                    for (int e = 0; e < EV; ++e) x[c][e] = ldexpf(x[c][e], e2);
-            }
-#pragma unroll
-            for (int c = 0; c < CK; ++c) {
-                uint4v part[NP];
-                if constexpr (F32) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) part[0][e] = __float_as_uint(x[c][e]);
-                } else {
-                    M::split(x[c], part);
-                }
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    if constexpr (QLDS) {
-                        if ((c & 3) == w) s_q[(rt * NP + k) * CK + c][lane] = part[k];
-                    } else {
-                        qr[k][c] = part[k];
-                    }
-                }
-            }
-        }
-    };
-    auto q_of = [&](int rt, int k, int c) {
-        if constexpr (QLDS)
-            return s_q[(rt * NP + k) * CK + c][lane];
-        else
-            return qr[k][c];
-    };
-
-    Piece pc = piece_at(x0);
-    auto start_piece = [&]() {
-        tbase = 0;
-        if constexpr (P16) {
-            near = tiles_at(pc, 0);
-            far = tiles_at(pc, 64);
-        } else {
-            near = look_up(pc, step_key(pc, 0) + (lane & (KS - 1)));
-        }
-    };
-    start_piece();
-    Where wh = where_of(pc, 0);
-    load_k(pc, wh);
-    load_v(pc, wh);
-    load_q(pc);
-    if (w == 0)
-        leave_entry(a.ws, WGS, blockIdx.x, x0, pc.g0, pc.gran, plan, [&](int v) { return paged_begin<WGS>(plan, v); },
-                    JoinEntry{pc.seq.t0, min(ROWS, pc.seq.n * G - pc.r0), pc.r0, pc.h, 0, 0});
-    if (QLDS) __syncthreads();
-
-    for (int x = x0;;) {
-        const SeqView sv = pc.seq;
-        const int last = sv.p0 + sv.n - 1, h = pc.h, r0 = pc.r0, rows = min(ROWS, sv.n * G - r0);
-        const int all_see = sv.p0 + r0 / G;            // the last key that all of the block's rows see
-        const bool mixed = (r0 + rows - 1) / G != r0 / G;
-        int lim[RT];                                   // the last key that row j sees
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) lim[rt] = 16 * rt + j < rows ? sv.p0 + (r0 + 16 * rt + j) / G : -1;
-        floatx4 o[RT][ND];                             // column 16 CW hh + CW (4g + i) + c of row j: o[CW hh + c][i]
-        float m[RT], l[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -INFINITY;
-            l[rt] = 0.f;
-#pragma unroll
-            for (int n = 0; n < ND; ++n) o[rt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-        }
-        const int steps = (pc.g1 - pc.g0) * SUB;
-        for (int s = 0; s < steps; ++s) {
-            const int k0 = step_key(pc, s);
-            if (k0 > last) break;                      // only in the last granule
-            const bool more = s + 1 < steps && step_key(pc, s + 1) <= last;
-            const Where at = wh;
-            // scores
-            floatx4 sc[RT][NT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) sc[rt][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < CK; ++c)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) {
-                        const uint4v q = q_of(rt, k, c);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) sc[rt][t] = M::mfma(kr[t][c], q, sc[rt][t]);
-                    }
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) {                                // the next step's keys
-                if constexpr (P16) {
-                    if ((s + 1) * NT - tbase >= 64) {
-                        near = far;
-                        tbase += 64;
-                        far = tiles_at(pc, tbase + 64);
-                    }
-                } else {
-                    near = look_up(pc, step_key(pc, s + 1) + (lane & (KS - 1)));
-                }
-                wh = where_of(pc, s + 1);
-                load_k(pc, wh);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            // keys that not all rows see, or that are not there
-            if (k0 + KS - 1 > all_see || !at.good) {
-                auto there = [&](int key) {            // a key of the step, counted from k0
-                    const bool page = P16 ? at.tgood[NT == 1 ? 0 : key >> 4] : (at.there >> key & 1) != 0;
-                    return page && k0 + key <= last;
-                };
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = 16 * t + 4 * g + i;
-                        const bool is = there(key);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            if (!is || k0 + key > lim[rt]) sc[rt][t][i] = -INFINITY;
-                        if (!is)
-#pragma unroll
-                            for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                                for (int d = 0; d < VD; ++d) vr[4 * t + i][hh][d] = 0;
-                    }
-                // infinities and NaN in V: 0 times them is not 0, so they are taken out, and rows that
-                // see them get NaN
-                if (mixed) {
-                    bool odd = false;
-                    auto wild = [&](uint32_t u, int half) {
-                        if constexpr (F32) return (u & 0x7f800000u) == 0x7f800000u;
-                        else return ((u >> (16 * half)) & (M::INF2 & 0xffff)) == (M::INF2 & 0xffff);
-                    };
-#pragma unroll
-                    for (int i = 0; i < VK; ++i)
-#pragma unroll
-                        for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                            for (int d = 0; d < VD; ++d) odd |= wild(vr[i][hh][d], 0) || wild(vr[i][hh][d], 1);
-                    if (__builtin_amdgcn_ballot_w64(odd)) {
-                        for (int hc = 0; hc < HH * CW; ++hc) {     // a column of each lane at a time
-                            bool wl[VK];
-#pragma unroll
-                            for (int i = 0; i < VK; ++i) {
-                                wl[i] = false;
-#pragma unroll
-                                for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                                    for (int c = 0; c < CW; ++c)
-                                        if (hh * CW + c == hc)
-                                            wl[i] = wild(vr[i][hh][F32 ? c : c / 2], F32 ? 0 : c & 1);
-                            }
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) {
-                                floatx4 hit = {0.f, 0.f, 0.f, 0.f};
-                                if constexpr (F32) {
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        hit = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                            wl[i] ? 1.f : 0.f, sc[rt][0][i] != -INFINITY ? 1.f : 0.f, hit, 0, 0, 0);
-                                } else {
-                                    uint4v A, B;
-#pragma unroll
-                                    for (int d = 0; d < 4; ++d) {
-                                        A[d] = (wl[2 * d] ? M::ONE : 0) | (wl[2 * d + 1] ? M::ONE << 16 : 0);
-                                        const float s0 = sc[rt][d / 2][2 * d % 4], s1 = sc[rt][d / 2][2 * d % 4 + 1];
-                                        B[d] = (s0 != -INFINITY ? M::ONE : 0) | (s1 != -INFINITY ? M::ONE << 16 : 0);
-                                    }
-                                    hit = M::mfma(A, B, hit);
-                                }
-#pragma unroll
-                                for (int n = 0; n < ND; ++n)
-                                    if (n == hc)
-#pragma unroll
-                                        for (int i = 0; i < 4; ++i) o[rt][n][i] = hit[i] > 0.f ? NAN : o[rt][n][i];
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < VK; ++i)
-#pragma unroll
-                            for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                                for (int d = 0; d < VD; ++d) {
-                                    if constexpr (F32) {
-                                        if (wild(vr[i][hh][d], 0)) vr[i][hh][d] = 0;
-                                    } else {
-                                        if (wild(vr[i][hh][d], 0)) vr[i][hh][d] &= 0xffff0000u;
-                                        if (wild(vr[i][hh][d], 1)) vr[i][hh][d] &= 0xffffu;
-                                    }
-                                }
-                    }
-                }
-            }
-            // weights: 2^(score - m + PEXP)
-            float p[RT][VK];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float mx = sc[rt][0][0];
-#pragma unroll
-                for (int e = 1; e < 4 * NT; ++e) mx = fmaxf(mx, sc[rt][e >> 2][e & 3]);
-                mx *= unq[rt];
-                if (__builtin_amdgcn_ballot_w64(mx > m[rt] + AR_SLACK)) {
-                    const float top = cols_max(mx);
-                    if (top > m[rt] + AR_SLACK) {
-                        const float f = __builtin_amdgcn_exp2f(m[rt] - top);
-                        m[rt] = top;
-                        l[rt] *= f;
-#pragma unroll
-                        for (int n = 0; n < ND; ++n) o[rt][n] *= f;
-                    }
-                }
-                const float by = M::PEXP - (m[rt] == -INFINITY ? 0.f : m[rt]);
-#pragma unroll
-                for (int e = 0; e < 4 * NT; ++e) {
-                    p[rt][e] = __builtin_amdgcn_exp2f(fmaf(sc[rt][e >> 2][e & 3], unq[rt], by));
-                    l[rt] += p[rt][e];
-                }
-            }
-            // outputs
-            if constexpr (F32) {
-#pragma unroll
-                for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                    for (int c = 0; c < CW; ++c)
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                o[rt][hh * CW + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    __uint_as_float(vr[i][hh][c]), p[rt][i], o[rt][hh * CW + c], 0, 0, 0);
-            } else {
-                uint4v pp[RT][NP];
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) M::split(p[rt], pp[rt]);
-#pragma unroll
-                for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                    for (int d = 0; d < VD; ++d) {
-                        uint4v v0, v1;                 // columns 2d and 2d + 1 of the lane's keys
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            v0[i] = __builtin_amdgcn_perm(vr[2 * i + 1][hh][d], vr[2 * i][hh][d], 0x05040100);
-                            v1[i] = __builtin_amdgcn_perm(vr[2 * i + 1][hh][d], vr[2 * i][hh][d], 0x07060302);
-                        }
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                            for (int k = 0; k < NP; ++k) {
-                                o[rt][hh * CW + 2 * d] = M::mfma(v0, pp[rt][k], o[rt][hh * CW + 2 * d]);
-                                o[rt][hh * CW + 2 * d + 1] = M::mfma(v1, pp[rt][k], o[rt][hh * CW + 2 * d + 1]);
-                            }
-                    }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) load_v(pc, wh);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-
-        // the next piece's first loads go out, then the four waves' results are joined through LDS
-        const int xn = x + pc.g1 - pc.g0;
-        const bool more = xn < x1, whole = pc.g0 == 0 && pc.g1 == pc.gran;
-        if (more) {
-            pc = piece_at(xn);
-            start_piece();
-            wh = where_of(pc, 0);
-            load_k(pc, wh);
-            load_v(pc, wh);
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float sum = cols_sum(l[rt]);
-            if (g == 0) {
-                s_m[w][16 * rt + j] = m[rt];
-                s_l[w][16 * rt + j] = sum;
-            }
-        }
-        float* slot = slot_of(a.ws, WGS, 2 * blockIdx.x + (x == x0 ? 0 : 1), ROWS, HD);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int d0 = 0; d0 < HD; d0 += OC) {
-                if (rt + d0 > 0) __syncthreads();      // the places are written again
-#pragma unroll
-                for (int hh = d0 / (16 * CW); hh < (d0 + OC) / (16 * CW); ++hh)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int c = 0; c < CW; c += 4) {
-                            floatx4 v;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] = o[rt][hh * CW + c + e][i];
-                            *(floatx4*)&s_o[w][j][16 * CW * hh + CW * (4 * g + i) + c - d0] = v;
-                        }
-                __syncthreads();
-                for (int u = threadIdx.x; u < 16 * (OC / 4); u += 256) {
-                    const int r16 = u / (OC / 4), r = 16 * rt + r16, c = 4 * (u % (OC / 4));
-                    if (r >= rows) break;
-                    const float mt = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-                    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-                    float lt = 0.f;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        // a maximum of -infinity with a sum: scores that are NaN, kept
-                        const float f = s_m[k][r] == -INFINITY ? (s_l[k][r] == 0.f ? 0.f : 1.f)
-                                                               : __builtin_amdgcn_exp2f(s_m[k][r] - mt);
-                        if (f == 0.f) continue;
-                        lt += f * s_l[k][r];
-                        sum += f * *(const floatx4*)&s_o[k][r16][c];
-                    }
-                    if (whole) {
-                        const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-                        const int row = r0 + r;
-                        if (FULL || d0 + c < hd)
-                            *(float4u*)(a.out + ((int64_t)(sv.t0 + row / G) * a.Hq + h * G + row % G) * hd + d0 + c) =
-                                sum * inv;
-                    } else {
-                        *(floatx4*)(slot + r * HD + d0 + c) = sum;
-                        if (d0 + c == 0)               // NaN scores only: nothing else counts beside them
-                            *(float2*)(slot + ROWS * HD + 2 * r) =
-                                make_float2(mt == -INFINITY && lt != 0.f ? INFINITY : mt, lt);
-                    }
-                }
-            }
-        if (!more) break;
-        if (QLDS) {                                    // no wave reads Q any more
-            load_q(pc);
-            __syncthreads();
-        } else {
-            __syncthreads();                           // before these rows' places are written again
-            load_q(pc);
-        }
-        x = xn;
-    }
-}
-
-// ---------------------------------------------------------------------------
-static int paged_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
-
-int64_t attention_paged_bytes(int hd) { return plan_bytes(paged_wgs(hd), hd <= 128 ? 32 : 16, paged_hd(hd)); }
-
-template <class E, int HD, int RT>
-static void launch_rt(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
-    const bool full = a.kv.head_dim == HD, p16 = a.pg.page_size % 16 == 0;
-    const dim3 grid(paged_wgs(HD)), th(256);
-    if (full && p16)
-        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, true, true>), grid, th, 0, s, a, pb);
-    else if (p16)
-        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, false, true>), grid, th, 0, s, a, pb);
-    else if (full)
-        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, true, false>), grid, th, 0, s, a, pb);
-    else
-        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, false, false>), grid, th, 0, s, a, pb);
-    if (paged_granules(pb.max_seq) > AP_KEEP)          // else no block is cut
-        launch_attn_join_paged(a.out, a.ws, a.Hq, a.kv.n_kv_heads, a.kv.head_dim, HD, 16 * RT, paged_wgs(HD), s);
-}
-
-template <class E>
-static void launch_type(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
-    const int hd = paged_hd(a.kv.head_dim);
-    const bool wide = (int64_t)pb.max_new * (a.Hq / a.kv.n_kv_heads) > 16;
-    if (hd == 256)
-        launch_rt<E, 256, 1>(a, pb, s);
-    else if (hd == 128)
-        wide ? launch_rt<E, 128, 2>(a, pb, s) : launch_rt<E, 128, 1>(a, pb, s);
-    else
-        wide ? launch_rt<E, 64, 2>(a, pb, s) : launch_rt<E, 64, 1>(a, pb, s);
+void launch_attention_paged_type<float>(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
+    launch_paged_hd<float>(a, pb, s);
 }
 
 int launch_attention_paged(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
     if (a.kv.dtype == KV_F32)
-        launch_type<float>(a, pb, s);
+        launch_attention_paged_type<float>(a, pb, s);
     else if (a.kv.dtype == KV_F16)
-        launch_type<_Float16>(a, pb, s);
+        launch_attention_paged_type<_Float16>(a, pb, s);
     else
-        launch_type<__bf16>(a, pb, s);
+        launch_attention_paged_type<__bf16>(a, pb, s);
     SH_CHECK_LAUNCH();
     return 0;
 }
