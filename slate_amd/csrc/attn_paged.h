@@ -112,6 +112,14 @@ struct Mul<float> {
     }
 };
 
+// A load from global memory (a flat one, which the compiler takes where it does not see
+// that, counts as an LDS access too, and waits for Q's would wait for it).
+template <class T>
+__device__ __forceinline__ T global_load(const char* base, uint32_t off) {
+    typedef const __attribute__((address_space(1))) char* Bytes;
+    return *(const __attribute__((address_space(1))) T*)((Bytes)(uintptr_t)base + off);
+}
+
 template <class E, int HD>
 struct PagedGeom {
     static constexpr bool F32 = sizeof(E) == 4;
@@ -239,48 +247,48 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
     };
     uint4v kr[NT][CK];
     uint32_t vr[VK][HH][VD];
-    const uint32_t k_off = j * (uint32_t)row_b, v_off = 4 * g * (uint32_t)row_b;
+    // the lane's part of the addresses
+    const uint32_t k_off = (P16 ? j * (uint32_t)row_b : 0) + EV * g * (uint32_t)sizeof(E);
+    uint32_t v_off[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v_off[i] = (P16 ? (4 * g + i) * (uint32_t)row_b : 0) + CW * j * (uint32_t)sizeof(E);
     auto load_k = [&](const Piece& p, const Where& wh) {
+        const char* pool = (const char*)a.kv.K + p.head_b;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const char* base;
-            uint32_t off = 0;
-            if constexpr (P16) {
-                base = uniform((const char*)a.kv.K + p.head_b + wh.tile[t]);
-                off = k_off;
-            } else {
-                base = (const char*)a.kv.K + p.head_b + from_lane(wh.row, 16 * t + j);
-            }
+            if constexpr (P16)
+                base = uniform(pool + wh.tile[t]);
+            else
+                base = pool + from_lane(wh.row, 16 * t + j);
 #pragma unroll
             for (int c = 0; c < CK; ++c) {
-                int e = 4 * EV * c + EV * g;
-                if (!FULL) e = e < hd ? e : 0;         // there Q is 0
-                kr[t][c] = *(const uint4v*)(base + off + e * (int)sizeof(E));
+                uint32_t off = k_off + 64 * c;
+                if (!FULL && 4 * EV * c + EV * g >= hd) off = k_off - EV * g * (uint32_t)sizeof(E);    // there Q is 0
+                kr[t][c] = global_load<uint4v>(base, off);
             }
         }
     };
     auto load_v = [&](const Piece& p, const Where& wh) {
+        const char* pool = (const char*)a.kv.V + p.head_b;
 #pragma unroll
         for (int i = 0; i < VK; ++i) {
             const char* base;
-            uint32_t off = 0;
-            if constexpr (P16) {
-                base = uniform((const char*)a.kv.V + p.head_b + wh.tile[i / 4] + (i % 4) * row_b);
-                off = v_off;
-            } else {
-                base = (const char*)a.kv.V + p.head_b + from_lane(wh.row, 16 * (i / 4) + 4 * g + i % 4);
-            }
+            if constexpr (P16)
+                base = uniform(pool + wh.tile[i / 4]);
+            else
+                base = pool + from_lane(wh.row, 16 * (i / 4) + 4 * g + i % 4);
 #pragma unroll
             for (int hh = 0; hh < HH; ++hh) {
-                int d = 16 * CW * hh + CW * j;
-                if (!FULL) d = d < hd ? d : 0;         // columns that are not written out
-                const char* at = base + off + d * (int)sizeof(E);
+                uint32_t off = v_off[i % 4] + 16 * CW * hh * (uint32_t)sizeof(E);
+                // columns that are not written out
+                if (!FULL && 16 * CW * hh + CW * j >= hd) off = v_off[i % 4] - CW * j * (uint32_t)sizeof(E);
                 if constexpr (VD == 4) {
-                    const uint4v x = *(const uint4v*)at;
+                    const uint4v x = global_load<uint4v>(base, off);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) vr[i][hh][e] = x[e];
                 } else {
-                    const uint2v x = *(const uint2v*)at;
+                    const uint2v x = global_load<uint2v>(base, off);
                     vr[i][hh][0] = x[0];
                     vr[i][hh][1] = x[1];
                 }
