@@ -57,6 +57,12 @@ __device__ __forceinline__ int paged_begin(const PlanT& plan, int w) {
     return gran <= AP_KEEP ? x - in : x;
 }
 
+// Of two halves, `exp` having the exponent's bits: all ones in those of which not all
+// of these bits are set.
+__device__ __forceinline__ uint32_t finite2(uint32_t u, uint32_t exp) {
+    return ((((~u & exp) + 0x7fff7fffu) >> 15) & 0x00010001u) * 0xffffu;
+}
+
 // How a type's numbers are multiplied: NP operands stand for one f32.
 template <class E>
 struct Mul;
@@ -64,7 +70,9 @@ template <>
 struct Mul<_Float16> {
     static constexpr int NP = 2;
     static constexpr float PEXP = 11;  // weights are scaled by 2^11: at most 2^15 with the slack
-    static constexpr uint32_t INF2 = 0x7c007c00, ONE = 0x3c00;
+    static constexpr uint32_t ONE = 0x3c003c00;
+    // all ones in the halves that are finite numbers
+    static __device__ __forceinline__ uint32_t finite(uint32_t u) { return finite2(u, 0x7c007c00); }
     static __device__ __forceinline__ void split(const float* x, uint4v* p) {
         half8_t hi, lo;
         halves(x, hi, lo);
@@ -80,7 +88,8 @@ template <>
 struct Mul<__bf16> {
     static constexpr int NP = 3;
     static constexpr float PEXP = 0;
-    static constexpr uint32_t INF2 = 0x7f807f80, ONE = 0x3f80;
+    static constexpr uint32_t ONE = 0x3f803f80;
+    static __device__ __forceinline__ uint32_t finite(uint32_t u) { return finite2(u, 0x7f807f80); }
     // cut off after 8 bits three times: exact
     static __device__ __forceinline__ void split(const float* x, uint4v* p) {
 #pragma unroll
@@ -104,6 +113,10 @@ template <>
 struct Mul<float> {
     static constexpr int NP = 1;
     static constexpr float PEXP = 0;
+    static constexpr uint32_t ONE = 0x3f800000;
+    static __device__ __forceinline__ uint32_t finite(uint32_t u) {
+        return 0u - (((~u & 0x7f800000u) + 0x7fffffffu) >> 31);
+    }
     static __device__ __forceinline__ floatx4 mfma(uint4v a, uint4v b, floatx4 c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -150,10 +163,13 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
     constexpr int SUB = AP_SLICE / KS;                 // steps of a slice
     constexpr bool QLDS = RT > 1 || RW > 1 || HD > 128;        // Q waits in LDS
     constexpr int WGS = paged_wgs(HD);
-    constexpr int OC = RW > 1 ? 64 : HD < 128 ? HD : 128, OS = OC + 4; // columns of the results in LDS at a time, stride
-    __shared__ float s_o[4][16][OS];
+    constexpr int OS = HD + 4;                         // row stride of a wave's results in LDS (floats)
+    // Q while a range is worked on, then the waves' results
+    constexpr int Q_BYTES = QLDS ? RW * RT * NP * CK * 64 * 16 : 0, O_BYTES = 4 * GROUP * OS * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
     __shared__ float s_m[4][GROUP], s_l[4][GROUP];
-    __shared__ uint4v s_q[RW][QLDS ? RT * NP * CK : 1][64];
+    float(*const s_o)[GROUP][OS] = (float(*)[GROUP][OS])smem;
+    uint4v(*const s_q)[RT * NP * CK][64] = (uint4v(*)[RT * NP * CK][64])smem;
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, j = lane & 15, kw = w % KW, rg = w / KW;
@@ -383,7 +399,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
         const int last = sv.p0 + sv.n - 1, h = pc.h, r0 = pc.r0, rows = min(ROWS, sv.n * G - r0);
         const int rw = r0 + GROUP * rg;                // the group's first row
         const int all_see = sv.p0 + rw / G;            // the last key that all of its rows see
-        const bool mixed = (min(rw + GROUP, r0 + rows) - 1) / G != rw / G;
+        const int own = min(GROUP, r0 + rows - rw);    // its rows: it may have none
+        const bool mixed = (rw + own - 1) / G != rw / G;
         int lim[RT];                                   // the last key that row j sees
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -399,7 +416,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
 #pragma unroll
             for (int n = 0; n < ND; ++n) o[rt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
-        const int steps = (pc.g1 - pc.g0) * SUB * RW;
+        const int steps = own > 0 ? (pc.g1 - pc.g0) * SUB * RW : 0;
         for (int s = 0; s < steps; ++s) {
             const int k0 = step_key(pc, s);
             if (k0 > last) break;                      // only in the last granule
@@ -460,68 +477,61 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
                 // infinities and NaN in V: 0 times them is not 0, so they are taken out, and rows that
                 // see them get NaN
                 if (mixed) {
-                    bool odd = false;
-                    auto wild = [&](uint32_t u, int half) {
-                        if constexpr (F32) return (u & 0x7f800000u) == 0x7f800000u;
-                        else return ((u >> (16 * half)) & (M::INF2 & 0xffff)) == (M::INF2 & 0xffff);
-                    };
+                    uint32_t odd = 0;
 #pragma unroll
                     for (int i = 0; i < VK; ++i)
 #pragma unroll
                         for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
-                            for (int d = 0; d < VD; ++d) odd |= wild(vr[i][hh][d], 0) || wild(vr[i][hh][d], 1);
-                    if (__builtin_amdgcn_ballot_w64(odd)) {
-                        for (int hc = 0; hc < HH * CW; ++hc) {     // a column of each lane at a time
-                            bool wl[VK];
+                            for (int d = 0; d < VD; ++d) odd |= ~M::finite(vr[i][hh][d]);
+                    if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+                        uint32_t sees[RT][4];          // 1 where row j sees the lane's key, as P's operand
 #pragma unroll
-                            for (int i = 0; i < VK; ++i) {
-                                wl[i] = false;
+                        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                                for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                                    for (int c = 0; c < CW; ++c)
-                                        if (hh * CW + c == hc)
-                                            wl[i] = wild(vr[i][hh][F32 ? c : c / 2], F32 ? 0 : c & 1);
+                            for (int e = 0; e < 4; ++e) {
+                                if constexpr (F32)
+                                    sees[rt][e] = sc[rt][0][e] != -INFINITY ? M::ONE : 0;
+                                else
+                                    sees[rt][e] = (sc[rt][e / 2][2 * e % 4] != -INFINITY ? M::ONE & 0xffff : 0) |
+                                                  (sc[rt][e / 2][2 * e % 4 + 1] != -INFINITY ? M::ONE & 0xffff0000u : 0);
                             }
 #pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) {
-                                floatx4 hit = {0.f, 0.f, 0.f, 0.f};
-                                if constexpr (F32) {
+                        for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        hit = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                            wl[i] ? 1.f : 0.f, sc[rt][0][i] != -INFINITY ? 1.f : 0.f, hit, 0, 0, 0);
-                                } else {
-                                    uint4v A, B;
+                            for (int d = 0; d < VD; ++d) {
+                                uint32_t wild[VK];
 #pragma unroll
-                                    for (int d = 0; d < 4; ++d) {
-                                        A[d] = (wl[2 * d] ? M::ONE : 0) | (wl[2 * d + 1] ? M::ONE << 16 : 0);
-                                        const float s0 = sc[rt][d / 2][2 * d % 4], s1 = sc[rt][d / 2][2 * d % 4 + 1];
-                                        B[d] = (s0 != -INFINITY ? M::ONE : 0) | (s1 != -INFINITY ? M::ONE << 16 : 0);
-                                    }
-                                    hit = M::mfma(A, B, hit);
+                                for (int i = 0; i < VK; ++i) {
+                                    const uint32_t fine = M::finite(vr[i][hh][d]);
+                                    wild[i] = ~fine & M::ONE;
+                                    vr[i][hh][d] &= fine;
                                 }
 #pragma unroll
-                                for (int n = 0; n < ND; ++n)
-                                    if (n == hc)
+                                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                                    for (int c = 0; c < (F32 ? 1 : 2); ++c) {
+                                        floatx4 hit = {0.f, 0.f, 0.f, 0.f};
+                                        if constexpr (F32) {
+#pragma unroll
+                                            for (int i = 0; i < 4; ++i)
+                                                hit = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                                    __uint_as_float(wild[i]), __uint_as_float(sees[rt][i]), hit, 0, 0, 0);
+                                        } else {
+                                            uint4v A;
+#pragma unroll
+                                            for (int i = 0; i < 4; ++i)
+                                                A[i] = __builtin_amdgcn_perm(wild[2 * i + 1], wild[2 * i],
+                                                                             c ? 0x07060302 : 0x05040100);
+                                            hit = M::mfma(A, uint4v{sees[rt][0], sees[rt][1], sees[rt][2], sees[rt][3]},
+                                                          hit);
+                                        }
+                                        const int n = hh * CW + (F32 ? d : 2 * d + c);
 #pragma unroll
                                         for (int i = 0; i < 4; ++i) o[rt][n][i] = hit[i] > 0.f ? NAN : o[rt][n][i];
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < VK; ++i)
-#pragma unroll
-                            for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                                for (int d = 0; d < VD; ++d) {
-                                    if constexpr (F32) {
-                                        if (wild(vr[i][hh][d], 0)) vr[i][hh][d] = 0;
-                                    } else {
-                                        if (wild(vr[i][hh][d], 0)) vr[i][hh][d] &= 0xffff0000u;
-                                        if (wild(vr[i][hh][d], 1)) vr[i][hh][d] &= 0xffffu;
+                                        __builtin_amdgcn_sched_barrier(0);     // few registers at a time
                                     }
-                                }
+                            }
                     }
                 }
             }
@@ -608,67 +618,53 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
                 s_l[w][16 * rt + j] = sum;
             }
         }
-        float* slot = slot_of(a.ws, WGS, 2 * blockIdx.x + (x == x0 ? 0 : 1), ROWS, HD);
+        if (QLDS) __syncthreads();                     // no wave reads Q any more
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int d0 = 0; d0 < HD; d0 += OC) {
-                if (rt + d0 > 0) __syncthreads();      // the places are written again
+            for (int hh = 0; hh < HH; ++hh)
 #pragma unroll
-                for (int hh = 0; hh < HH; ++hh)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int c = 0; c < CW; c += 4) {
+                        floatx4 v;
 #pragma unroll
-                        for (int c = 0; c < CW; c += 4) {
-                            const int col = 16 * CW * hh + CW * (4 * g + i) + c - d0;
-                            if (OC < HD && (col < 0 || col >= OC)) continue;
-                            floatx4 v;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] = o[rt][hh * CW + c + e][i];
-                            *(floatx4*)&s_o[w][j][col] = v;
-                        }
-                __syncthreads();
-                for (int u = threadIdx.x; u < 16 * RW * (OC / 4); u += 256) {
-                    const int gr = u / (16 * (OC / 4)), r16 = u / (OC / 4) % 16, c = 4 * (u % (OC / 4));
-                    const int rl = 16 * rt + r16, r = GROUP * gr + rl;
-                    if (r >= rows) continue;
-                    const int w0 = gr * KW;
-                    float mt = s_m[w0][rl];
-#pragma unroll
-                    for (int k = 1; k < KW; ++k) mt = fmaxf(mt, s_m[w0 + k][rl]);
-                    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-                    float lt = 0.f;
-#pragma unroll
-                    for (int k = w0; k < w0 + KW; ++k) {
-                        // a maximum of -infinity with a sum: scores that are NaN, kept
-                        const float f = s_m[k][rl] == -INFINITY ? (s_l[k][rl] == 0.f ? 0.f : 1.f)
-                                                                : __builtin_amdgcn_exp2f(s_m[k][rl] - mt);
-                        if (f == 0.f) continue;
-                        lt += f * s_l[k][rl];
-                        sum += f * *(const floatx4*)&s_o[k][r16][c];
+                        for (int e = 0; e < 4; ++e) v[e] = o[rt][hh * CW + c + e][i];
+                        *(floatx4*)&s_o[w][16 * rt + j][16 * CW * hh + CW * (4 * g + i) + c] = v;
                     }
-                    if (whole) {
-                        const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-                        const int row = r0 + r;
-                        if (FULL || d0 + c < hd)
-                            *(float4u*)(a.out + ((int64_t)(sv.t0 + row / G) * a.Hq + h * G + row % G) * hd + d0 + c) =
-                                sum * inv;
-                    } else {
-                        *(floatx4*)(slot + r * HD + d0 + c) = sum;
-                        if (d0 + c == 0)               // NaN scores only: nothing else counts beside them
-                            *(float2*)(slot + ROWS * HD + 2 * r) =
-                                make_float2(mt == -INFINITY && lt != 0.f ? INFINITY : mt, lt);
-                    }
-                }
+        __syncthreads();
+        float* slot = slot_of(a.ws, WGS, 2 * blockIdx.x + (x == x0 ? 0 : 1), ROWS, HD);
+        for (int u = threadIdx.x; u < rows * (HD / 4); u += 256) {
+            const int r = u / (HD / 4), c = 4 * (u % (HD / 4)), w0 = r / GROUP * KW, rl = r % GROUP;
+            float mt = s_m[w0][rl];
+#pragma unroll
+            for (int k = 1; k < KW; ++k) mt = fmaxf(mt, s_m[w0 + k][rl]);
+            floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+            float lt = 0.f;
+#pragma unroll
+            for (int k = w0; k < w0 + KW; ++k) {
+                // a maximum of -infinity with a sum: scores that are NaN, kept
+                const float f = s_m[k][rl] == -INFINITY ? (s_l[k][rl] == 0.f ? 0.f : 1.f)
+                                                        : __builtin_amdgcn_exp2f(s_m[k][rl] - mt);
+                if (f == 0.f) continue;
+                lt += f * s_l[k][rl];
+                sum += f * *(const floatx4*)&s_o[k][rl][c];
             }
-        if (!more) break;
-        if (QLDS) {                                    // no wave reads Q any more
-            load_q(pc);
-            __syncthreads();
-        } else {
-            __syncthreads();                           // before these rows' places are written again
-            load_q(pc);
+            if (whole) {
+                const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+                const int row = r0 + r;
+                if (FULL || c < hd)
+                    *(float4u*)(a.out + ((int64_t)(sv.t0 + row / G) * a.Hq + h * G + row % G) * hd + c) = sum * inv;
+            } else {
+                *(floatx4*)(slot + r * HD + c) = sum;
+                if (c == 0)                            // NaN scores only: nothing else counts beside them
+                    *(float2*)(slot + ROWS * HD + 2 * r) = make_float2(mt == -INFINITY && lt != 0.f ? INFINITY : mt, lt);
+            }
         }
+        if (!more) break;
+        __syncthreads();                               // before these rows' places are written again
+        load_q(pc);
+        if (QLDS) __syncthreads();
         x = xn;
     }
 }
