@@ -46,15 +46,23 @@ struct PagedCount {
     }
 };
 
-// Where workgroup w's range begins: N w / P, or the start of the block there
-// if it is short.
+// Where workgroup w's range begins (the place there is for x < plan.total): N w / P,
+// or the start of the block there if it is short.
+struct PagedBegin {
+    int x;
+    Place place;
+};
 template <int WGS, class PlanT>
-__device__ __forceinline__ int paged_begin(const PlanT& plan, int w) {
-    const int x = plan.begin(w, WGS);
-    if (x >= plan.total) return plan.total;
-    const Place pl = plan.find(x);
-    const int gran = paged_granules(pl.seq.p0 + pl.seq.n), in = pl.at % gran;
-    return gran <= AP_KEEP ? x - in : x;
+__device__ __forceinline__ PagedBegin paged_begin(const PlanT& plan, int w) {
+    PagedBegin b{plan.begin(w, WGS), {}};
+    if (b.x >= plan.total) return PagedBegin{plan.total, {}};
+    b.place = plan.find(b.x);
+    const int gran = paged_granules(b.place.seq.p0 + b.place.seq.n), in = b.place.at % gran;
+    if (gran <= AP_KEEP) {
+        b.x -= in;
+        b.place.at -= in;
+    }
+    return b;
 }
 
 // Of two halves, `exp` having the exponent's bits: all ones in those of which not all
@@ -150,15 +158,17 @@ struct PagedGeom {
 
 // RW groups of 4 / RW waves: a group has 16 RT rows and all keys of the range, so
 // that a block's K and V come once from memory and RW times from the L2.
-// FULL: head_dim is HD (else smaller).  P16: pages hold whole 16-key tiles, so
-// that a tile's page is the same for all lanes.
-template <class E, int HD, int RT, int RW, bool FULL, bool P16>
+// FULL: head_dim is HD (else smaller).  P: pages hold whole tiles of 16 keys, so that a
+// tile's page is the same for all lanes; or whole fours, the keys of a lane in S^T; or
+// any number of rows (1).
+template <class E, int HD, int RT, int RW, bool FULL, int P>
 __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(PagedAttn a, PagedBatch pb) {
     using Geo = PagedGeom<E, HD>;
     using M = Mul<E>;
     constexpr bool F32 = Geo::F32;
     constexpr int KS = Geo::KS, NT = Geo::NT, EV = Geo::EV, CK = Geo::CK, CW = Geo::CW, HH = Geo::HH, VK = Geo::VK;
     constexpr int VD = Geo::VD, ND = Geo::ND, NP = Geo::NP;
+    constexpr bool P16 = P == 16;
     constexpr int KW = 4 / RW, GROUP = 16 * RT, ROWS = RW * GROUP;
     constexpr int SUB = AP_SLICE / KS;                 // steps of a slice
     constexpr bool QLDS = RT > 1 || RW > 1 || HD > 128;        // Q waits in LDS
@@ -177,8 +187,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
     using PlanT = Plan<PagedCount<ROWS>, PagedBatch>;
     const PagedCount<ROWS> count{G, Hkv};
     const PlanT plan(pb, count);
-    const int x0 = paged_begin<WGS>(plan, blockIdx.x), x1 = paged_begin<WGS>(plan, blockIdx.x + 1);
-    if (x0 >= x1) {
+    const PagedBegin begin = paged_begin<WGS>(plan, blockIdx.x);
+    const int x0 = begin.x;
+    if (x0 >= plan.total) {
         if (threadIdx.x == 0) entry_of(a.ws, blockIdx.x)->rows = 0;
         return;
     }
@@ -191,8 +202,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
         const int32_t* table;
         int64_t head_b;                // byte offset of the head
     };
-    auto piece_at = [&](int x) {
-        const Place pl = plan.find(x);
+    auto piece_of = [&](const Place& pl) {
         Piece p;
         p.seq = pl.seq;
         p.gran = paged_granules(pl.seq.p0 + pl.seq.n);
@@ -200,14 +210,14 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
         p.h = b / nb;
         p.r0 = ROWS * (b % nb);
         p.g0 = pl.at % p.gran;
-        p.g1 = min(p.gran, p.g0 + (x1 - x));
+        p.g1 = p.gran;                                 // if the range goes so far
         p.table = a.pg.table + pl.base * a.pg.max_pages;
         p.head_b = p.h * a.kv.head_stride * (int)sizeof(E);
         return p;
     };
 
-    // Pages.  P16: lane l has the page (-1: none) and the row within it of the
-    // wave's tile `at` + l; else of key l of a step.
+    // Pages.  P16: lane l has the page and the row within it of the wave's tile `at` +
+    // l; else of the P keys from P l on of a step.
     struct Found {
         int page, row;
     };
@@ -215,9 +225,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
         const int last = p.seq.p0 + p.seq.n - 1, k = min(key, last);
         const int i = (int)((unsigned)k / (unsigned)ps), page = p.table[i];
         int r = k - i * ps;
-        if (P16) r &= ~15;
-        return Found{(unsigned)page < (unsigned)a.pg.n_pages ? page : -1, r};
+        r &= ~(P - 1);
+        return Found{page, r};                         // (the page is looked at when it is used)
     };
+    auto is_page = [&](int page) { return (unsigned)page < (unsigned)a.pg.n_pages; };
     // a wave's slices: every KW-th of a granule
     auto slice_key = [&](const Piece& p, int i) {
         return min(p.g0 + i / RW, p.gran) * AP_GRAN + (kw + KW * (i % RW)) * AP_SLICE;
@@ -227,15 +238,16 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
         const int i = at + lane;
         return look_up(p, slice_key(p, i >> 1) + (i & 1) * 16);
     };
+    auto keys_at = [&](const Piece& p, int s) { return look_up(p, step_key(p, s) + P * (lane & (KS / P - 1))); };
     // where a step's rows are: byte offsets from the head's start
     struct Where {
         int64_t tile[P16 ? NT : 1];    // P16: of the tiles (the same in all lanes)
-        int64_t row;                   // else: of key `lane`
+        int64_t row;                   // else: of the lane's P keys
         bool good;                     // all of the step's pages are there
-        uint64_t there;                // else: which keys' are
+        uint64_t there;                // else: which lanes' are
         bool tgood[NT];
     };
-    Found near, far;                   // P16: pages of the tiles at tbase .., and of the 64 after them
+    Found near;                        // P16: pages of the 64 tiles at tbase; else of the next step's keys
     int tbase = 0;
     auto where_of = [&](const Piece& p, int s) {
         Where wh;
@@ -245,15 +257,15 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
             for (int t = 0; t < NT; ++t) {
                 const int i = s * NT + t - tbase;
                 const int page = __builtin_amdgcn_readlane(near.page, i), r = __builtin_amdgcn_readlane(near.row, i);
-                wh.tgood[t] = page >= 0;
-                wh.good &= page >= 0;
-                wh.tile[t] = (int64_t)max(page, 0) * (a.kv.page_stride * (int)sizeof(E)) + r * row_b;
+                wh.tgood[t] = is_page(page);
+                wh.good &= wh.tgood[t];
+                wh.tile[t] = (int64_t)(wh.tgood[t] ? page : 0) * (a.kv.page_stride * (int)sizeof(E)) + r * row_b;
             }
         } else {
             const Found f = near;
-            wh.there = __builtin_amdgcn_ballot_w64(f.page >= 0) | ~((1ull << KS) - 1);
+            wh.there = __builtin_amdgcn_ballot_w64(is_page(f.page)) | ~((1ull << KS / P) - 1);
             wh.good = wh.there == ~0ull;
-            wh.row = (int64_t)max(f.page, 0) * (a.kv.page_stride * (int)sizeof(E)) + f.row * row_b;
+            wh.row = (int64_t)(is_page(f.page) ? f.page : 0) * (a.kv.page_stride * (int)sizeof(E)) + f.row * row_b;
         }
         return wh;
     };
@@ -264,10 +276,16 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
     uint4v kr[NT][CK];
     uint32_t vr[VK][HH][VD];
     // the lane's part of the addresses
-    const uint32_t k_off = (P16 ? j * (uint32_t)row_b : 0) + EV * g * (uint32_t)sizeof(E);
-    uint32_t v_off[4];
+    const uint32_t k_off = j % P * (uint32_t)row_b + EV * g * (uint32_t)sizeof(E);
+    const uint32_t k_last = j % P * (uint32_t)row_b + (hd - EV) * (uint32_t)sizeof(E);
+    uint32_t v_off[4], v_last[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v_off[i] = (P16 ? (4 * g + i) * (uint32_t)row_b : 0) + CW * j * (uint32_t)sizeof(E);
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t row = (4 * g + i) % P * (uint32_t)row_b;
+        v_off[i] = row + CW * j * (uint32_t)sizeof(E);
+        v_last[i] = row + (hd - CW) * (uint32_t)sizeof(E);
+    }
+    uint32_t real = ~0u;                               // 0: loads that nothing waits for, all lanes the same bytes
     auto load_k = [&](const Piece& p, const Where& wh) {
         const char* pool = (const char*)a.kv.K + p.head_b;
 #pragma unroll
@@ -276,29 +294,29 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
             if constexpr (P16)
                 base = uniform(pool + wh.tile[t]);
             else
-                base = pool + from_lane(wh.row, 16 * t + j);
+                base = pool + from_lane(wh.row, (16 * t + j) / P);
 #pragma unroll
             for (int c = 0; c < CK; ++c) {
-                uint32_t off = k_off + 64 * c;
-                if (!FULL && 4 * EV * c + EV * g >= hd) off = k_off - EV * g * (uint32_t)sizeof(E);    // there Q is 0
+                uint32_t off = (k_off & real) + 64 * c;
+                if (!FULL) off = min(off, k_last);     // past the row Q is 0
                 kr[t][c] = global_load<uint4v>(base, off);
             }
         }
     };
     auto load_v = [&](const Piece& p, const Where& wh) {
         const char* pool = (const char*)a.kv.V + p.head_b;
+        const char* base = nullptr;
 #pragma unroll
         for (int i = 0; i < VK; ++i) {
-            const char* base;
-            if constexpr (P16)
-                base = uniform(pool + wh.tile[i / 4]);
-            else
-                base = pool + from_lane(wh.row, 16 * (i / 4) + 4 * g + i % 4);
+            if constexpr (P16) {
+                if (i % 4 == 0) base = uniform(pool + wh.tile[i / 4]);
+            } else {
+                if (i % P == 0) base = pool + from_lane(wh.row, (16 * (i / 4) + 4 * g + i % 4) / P);
+            }
 #pragma unroll
             for (int hh = 0; hh < HH; ++hh) {
-                uint32_t off = v_off[i % 4] + 16 * CW * hh * (uint32_t)sizeof(E);
-                // columns that are not written out
-                if (!FULL && 16 * CW * hh + CW * j >= hd) off = v_off[i % 4] - CW * j * (uint32_t)sizeof(E);
+                uint32_t off = (v_off[i % 4] & real) + 16 * CW * hh * (uint32_t)sizeof(E);
+                if (!FULL) off = min(off, v_last[i % 4]);      // columns that are not written out
                 if constexpr (VD == 4) {
                     const uint4v x = global_load<uint4v>(base, off);
 #pragma unroll
@@ -374,23 +392,30 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
             return qr[k][c];
     };
 
-    Piece pc = piece_at(x0);
+    Piece pc = piece_of(begin.place);
     auto start_piece = [&]() {
         tbase = 0;
         if constexpr (P16) {
             near = tiles_at(pc, 0);
-            far = tiles_at(pc, 64);
         } else {
-            near = look_up(pc, step_key(pc, 0) + (lane & (KS - 1)));
+            near = keys_at(pc, 0);
         }
+        const Where wh = where_of(pc, 0);
+        if constexpr (!P16) near = keys_at(pc, 1);
+        return wh;
     };
-    start_piece();
-    Where wh = where_of(pc, 0);
+    Where wh = start_piece();
     load_k(pc, wh);
     load_v(pc, wh);
+    const int x1 = paged_begin<WGS>(plan, blockIdx.x + 1).x;
+    if (x0 >= x1) {                                    // the block is another workgroup's
+        if (threadIdx.x == 0) entry_of(a.ws, blockIdx.x)->rows = 0;
+        return;
+    }
+    pc.g1 = min(pc.gran, pc.g0 + (x1 - x0));
     load_q(pc);
     if (w == 0)
-        leave_entry(a.ws, WGS, blockIdx.x, x0, pc.g0, pc.gran, plan, [&](int v) { return paged_begin<WGS>(plan, v); },
+        leave_entry(a.ws, WGS, blockIdx.x, x0, pc.g0, pc.gran, plan, [&](int v) { return paged_begin<WGS>(plan, v).x; },
                     JoinEntry{pc.seq.t0, min(ROWS, pc.seq.n * G - pc.r0), pc.r0, pc.h, 0, 0});
     if (QLDS) __syncthreads();
 
@@ -416,11 +441,13 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
 #pragma unroll
             for (int n = 0; n < ND; ++n) o[rt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
-        const int steps = own > 0 ? (pc.g1 - pc.g0) * SUB * RW : 0;
+        const int xn = x + pc.g1 - pc.g0;
+        const bool more = xn < x1, whole = pc.g0 == 0 && pc.g1 == pc.gran;
+        // steps that have keys (in the last granule a wave may have none); one at least, for the loads behind it
+        int steps = own > 0 ? (pc.g1 - pc.g0) * SUB * RW : 1;
+        while (steps > 1 && step_key(pc, steps - 1) > last) --steps;
         for (int s = 0; s < steps; ++s) {
             const int k0 = step_key(pc, s);
-            if (k0 > last) break;                      // only in the last granule
-            const bool more = s + 1 < steps && step_key(pc, s + 1) <= last;
             const Where at = wh;
             // scores
             floatx4 sc[RT][NT];
@@ -439,24 +466,32 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
                         for (int t = 0; t < NT; ++t) sc[rt][t] = M::mfma(kr[t][c], q, sc[rt][t]);
                     }
             __builtin_amdgcn_sched_barrier(0);
-            if (more) {                                // the next step's keys
+            // the next step's keys, the next piece's or, at the end, some bytes: no load hangs on a
+            // branch, so that the compiler can count how many may be under way at a wait
+            if (s + 1 < steps) {
                 if constexpr (P16) {
                     if ((s + 1) * NT - tbase >= 64) {
-                        near = far;
                         tbase += 64;
-                        far = tiles_at(pc, tbase + 64);
+                        near = tiles_at(pc, tbase);
+                        SH_WAIT_VMCNT(0);              // here, every 32 steps, rather than where its lanes are read
                     }
-                } else {
-                    near = look_up(pc, step_key(pc, s + 1) + (lane & (KS - 1)));
                 }
                 wh = where_of(pc, s + 1);
-                load_k(pc, wh);
+                if constexpr (!P16) near = keys_at(pc, s + 2);
+            } else if (more) {
+                pc = piece_of(plan.find(xn));
+                pc.g1 = min(pc.gran, pc.g0 + (x1 - xn));
+                wh = start_piece();
+            } else {
+                real = 0;
+                if constexpr (!P16) wh.row = 0;
             }
+            load_k(pc, wh);
             __builtin_amdgcn_sched_barrier(0);
             // keys that not all rows see, or that are not there
             if (k0 + KS - 1 > all_see || !at.good) {
                 auto there = [&](int key) {            // a key of the step, counted from k0
-                    const bool page = P16 ? at.tgood[NT == 1 ? 0 : key >> 4] : (at.there >> key & 1) != 0;
+                    const bool page = P16 ? at.tgood[NT == 1 ? 0 : key >> 4] : (at.there >> key / P & 1) != 0;
                     return page && k0 + key <= last;
                 };
 #pragma unroll
@@ -596,20 +631,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (more) load_v(pc, wh);
+            load_v(pc, wh);
             __builtin_amdgcn_sched_barrier(0);
         }
 
-        // the next piece's first loads go out, then the four waves' results are joined through LDS
-        const int xn = x + pc.g1 - pc.g0;
-        const bool more = xn < x1, whole = pc.g0 == 0 && pc.g1 == pc.gran;
-        if (more) {
-            pc = piece_at(xn);
-            start_piece();
-            wh = where_of(pc, 0);
-            load_k(pc, wh);
-            load_v(pc, wh);
-        }
+        // the waves' results are joined through LDS
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const float sum = cols_sum(l[rt]);
@@ -682,12 +708,14 @@ void launch_attention_paged_type<__bf16>(const PagedAttn& a, const PagedBatch& p
 template <class E, int HD, int RT, int RW>
 static void launch_paged_rows(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
     const dim3 grid(paged_wgs(HD)), th(256);
-    if (a.pg.page_size % 16 != 0)
-        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, false, false>), grid, th, 0, s, a, pb);
+    if (a.pg.page_size % 4 != 0)
+        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, false, 1>), grid, th, 0, s, a, pb);
+    else if (a.pg.page_size % 16 != 0)
+        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, false, 4>), grid, th, 0, s, a, pb);
     else if (a.kv.head_dim != HD)
-        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, false, true>), grid, th, 0, s, a, pb);
+        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, false, 16>), grid, th, 0, s, a, pb);
     else
-        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, true, true>), grid, th, 0, s, a, pb);
+        hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, true, 16>), grid, th, 0, s, a, pb);
     if (paged_granules(pb.max_seq) > AP_KEEP)          // else no block is cut
         launch_attn_join_paged(a.out, a.ws, a.Hq, a.kv.n_kv_heads, a.kv.head_dim, HD, 16 * RT * RW, paged_wgs(HD), s);
 }
