@@ -398,7 +398,8 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     __shared__ float s_top[VF_ROWS], s_z[VF_ROWS];
     __shared__ int s_best[VF_ROWS], s_parent[VF_ROWS], s_tok[VF_ROWS];
     __shared__ double s_part[VF_TH / 64], s_mass[VF_TH];
-    __shared__ int s_node, s_acc, s_turned;
+    __shared__ int s_node, s_acc, s_turned, s_n_out;
+    int* const s_out = (int*)s_z;                      // the node's tokens that were turned down, once s_z was read
     const int b = blockIdx.x, lane = threadIdx.x & 63, V = a.V, nch = chunks_of(V);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Space sp = space_of(a);
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     __syncthreads();
     if (w == 0) {
         // drafts in order, 64 at a time: a row's children lie behind it
-        int node = 0, acc = 0, turned = -1;
+        int node = 0, acc = 0, turned = -1, n_out = 0;
         double rest = 1;
         for (int i0 = 0; i0 < n; i0 += 64) {
             const int i = i0 + lane, up = i < n && i > 0 ? s_parent[i] : -1;
@@ -472,10 +473,15 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
                     node = c;
                     rest = 1;
                     turned = -1;
+                    n_out = 0;
                     left = __builtin_amdgcn_ballot_w64(up == node) & ~((2ull << l) - 1);
                 } else {
                     rest -= p;
                     turned = c;
+                    if (p > 0) {                       // (a token outside the vocabulary or a second time: no p)
+                        if (lane == 0) s_out[n_out] = s_tok[c];
+                        ++n_out;
+                    }
                     left &= left - 1;
                 }
             }
@@ -484,6 +490,7 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
             s_node = node;
             s_acc = acc;
             s_turned = turned;
+            s_n_out = n_out;
             a.n_accepted[b] = acc;
         }
     }
@@ -508,37 +515,35 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     double* own = nch <= VF_TH ? s_mass : sp.mass + (int64_t)b * nch;
     int pick = -1;
     // the second pass, where nothing was left, is from p itself
-    for (int without = !a.q && turned >= 0; without >= 0 && pick < 0; --without) {
-        auto taken = [&](int j) { return s_parent[j] == node && s_tok[j] >= 0 && s_tok[j] < V; };
+    for (int without = !a.q && s_n_out > 0; without >= 0 && pick < 0; --without) {
+        const int n_out = without ? s_n_out : 0;
         auto values = [&](int at, double* m) {
             float x[4];
             load4(z, at, V, -INFINITY, x);
-            if (without)
-                for (int j = node + 1; j <= turned; ++j)
+            for (int k = 0; k < n_out; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (taken(j) && s_tok[j] == at + i) x[i] = -INFINITY;
+                for (int i = 0; i < 4; ++i)
+                    if (s_out[k] == at + i) x[i] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i) m[i] = weight(x[i], top, heat.by);
         };
         for (int c = threadIdx.x; c < nch; c += VF_TH) own[c] = part[c].sum * weight(part[c].top, top, heat.by);
-        __syncthreads();
-        if (without) {
-            for (int j = node + 1 + w; j <= turned; j += VF_TH / 64) {
-                if (!taken(j)) continue;
-                const int c = s_tok[j] / VF_CHUNK;     // of two tokens in a chunk either writes the same
+        if (n_out > 0) {
+            __syncthreads();
+            for (int j = w; j < n_out; j += VF_TH / 64) {
+                const int c = s_out[j] / VF_CHUNK;     // of two tokens in a chunk either writes the same
                 float x[16];
                 load16(z, c, V, -INFINITY, x);
-                for (int k = node + 1; k <= turned; ++k)
+                for (int k = 0; k < n_out; ++k)
+                    if (s_out[k] / VF_CHUNK == c)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (taken(k) && s_tok[k] == place(c, i)) x[i] = -INFINITY;
-                double s = weights_of(x, top, heat.by);
-                s = wave_sum_f64(s);
+                        for (int i = 0; i < 16; ++i)
+                            if (s_out[k] == place(c, i)) x[i] = -INFINITY;
+                const double s = wave_sum_f64(weights_of(x, top, heat.by));
                 if (lane == 0) own[c] = s;
             }
-            __syncthreads();
         }
+        __syncthreads();
         pick = pick_token<VF_TH>(nch, u_next, [&](int c) { return own[c]; }, values, s_part);
         __syncthreads();
     }
