@@ -60,13 +60,9 @@ class Plan {
 
     __device__ __forceinline__ Plan(const Batch& pb, const Count& count) : pb_(pb), count_(count) {
         end = pb.B;
-        cut(0);
-        first_ = load(0);
+        first_ = cut_and_load(0);
         total = __builtin_amdgcn_readlane(first_.upto, 63);
-        for (int b0 = 64; b0 < end; b0 += 64) {
-            cut(b0);
-            total += __builtin_amdgcn_readlane(load(b0).upto, 63);
-        }
+        for (int b0 = 64; b0 < end; b0 += 64) total += __builtin_amdgcn_readlane(cut_and_load(b0).upto, 63);
     }
     // The plan's first 64 sequences can wait in LDS instead of in registers.
     struct Lane {
@@ -108,21 +104,30 @@ class Plan {
     }
 
   private:
-    __device__ __forceinline__ void cut(int b0) {
+    // Sequences b0 .. b0 + 63, all their descriptors in one round of loads.
+    struct Read {
+        SeqView seq;
+        int64_t base;
+        bool falls;                    // of tok_off behind the sequence: it ends the plan
+    };
+    __device__ __forceinline__ Read read(int b0) const {
         const int b = b0 + (int)(threadIdx.x & 63);
-        const uint64_t falls = __builtin_amdgcn_ballot_w64(b < end && pb_.tok_off[b + 1] < pb_.tok_off[b]);
-        if (falls) end = b0 + __builtin_ctzll(falls);
+        Read r{};
+        if (b < pb_.B) r = Read{seq_view(pb_, b), seq_base(pb_, b), pb_.tok_off[b + 1] < pb_.tok_off[b]};
+        return r;
     }
-    __device__ __forceinline__ Lane load(int b0) const {
-        const int b = b0 + (int)(threadIdx.x & 63);
-        Lane s{};
-        if (b < end) {
-            s.seq = seq_view(pb_, b);
-            s.base = seq_base(pb_, b);
-            s.own = count_(s.seq);
-        }
+    __device__ __forceinline__ Lane lane_of(int b0, const Read& r) const {
+        Lane s{r.seq, r.base, 0, 0};
+        if (b0 + (int)(threadIdx.x & 63) < end) s.own = count_(r.seq);
         s.upto = wave_scan(s.own);
         return s;
+    }
+    __device__ __forceinline__ Lane load(int b0) const { return lane_of(b0, read(b0)); }
+    __device__ __forceinline__ Lane cut_and_load(int b0) {
+        const Read r = read(b0);
+        const uint64_t falls = __builtin_amdgcn_ballot_w64(r.falls);
+        if (falls) end = min(end, b0 + __builtin_ctzll(falls));
+        return lane_of(b0, r);
     }
     const Batch& pb_;
     const Count count_;
