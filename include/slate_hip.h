@@ -380,13 +380,15 @@ int   slate_hip_kv_store_paged(const slate_hip_paged_kv_t* kv, const slate_hip_p
  * outside 0 .. n_slots-1, more than max_pages * page_size rows) is left out; rows
  * of out that no sequence owns stay as they were.  Keys in pages outside 0 ..
  * n_pages-1 count as not seen, and a token that sees none gets zeros.  What the
- * cache holds in rows that a token does not see never matters, not even
- * infinities and NaN; one in a row that it sees makes its output not finite.
- * Queries must be finite and below 2^100 in size, bf16 and f32 K and V too.  Sums are
- * f32.  f32 caches are multiplied in f32, for bf16 ones queries and weights are split
- * into 24 bits, for f16 ones into 22.
+ * cache holds in rows that a token does not see never matters, not even infinities
+ * and NaN; one in V of a row that it sees makes that column of its output not
+ * finite, a NaN in K all of it.
+ * Queries must be finite and below 2^100 in size, and so must bf16 and f32 K and V.  Sums
+ * are f32.  f32 caches are multiplied in f32; over bf16 ones queries and weights have 24
+ * bits; over f16 ones 22, and a weight is resolved to 2^-35 of the largest.
  * Made for few tokens a sequence (decode steps, drafts): K and V are read once for
- * every 16 query rows of a kv head, or 32 where there are more.  T * n_q_heads <=
+ * every 16 query rows of a kv head where max_new brings no more, else for every 32 or 64
+ * (head_dim above 128: 32).  T * n_q_heads <=
  * 2^31 - 128, and n_kv_heads * (T * n_q_heads / n_kv_heads / 16 + B) * max_pages *
  * page_size / 128 stays below 2^31.  ws as for attention_ragged_q8, of
  * slate_hip_attention_paged_bytes. */
@@ -418,7 +420,7 @@ int64_t slate_hip_attention_paged_bytes(int n_q_heads, int n_kv_heads, int head_
  * Where none stands the next token is the lowest i with p(i) > 0 and a sum of p up to i above
  * u_next[b] times the whole sum (the last with p > 0 where no sum is).  u (device
  * float[T], at the drafts) and u_next (float[B]) are uniform in [0, 1).  Tokens
- * outside 0 .. V-1 never stand.  q is not negative.
+ * outside 0 .. V-1 never stand.  q is not negative.  All T rows of logits are read.
  * Outputs (device): n_accepted[b] (-1 for a sequence that is left out: without rows, with
  * more than 1024 drafts, outside 0 .. T, or behind a fall of tok_off); out_tok[T]: in a sequence's rows the accepted tokens, the next
  * one (-1: no p), then -1; out_row[T] (or NULL): the rows that were accepted,

@@ -76,7 +76,7 @@ class Weights {
     // has: none above 2^512 and one above 2^-512, so that what counts as 2^-900
     // below shows in no sum (infinities, NaN, temperatures without an end: no).
     __device__ __forceinline__ bool takes(float top) const {
-        return most_ < 1e38f && !__builtin_amdgcn_ballot_w64(top > most_) && __builtin_amdgcn_ballot_w64(top > -most_);
+        return most_ < 1e38f && most_ > 1e-30f && !__builtin_amdgcn_ballot_w64(top > most_) && __builtin_amdgcn_ballot_w64(top > -most_);
     }
     __device__ __forceinline__ double operator()(float x) const {
         constexpr double WHOLE = 6755399441055744.0;   // 1.5 2^52: a sum with it is a whole number in its low bits

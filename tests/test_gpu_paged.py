@@ -16,6 +16,7 @@ Tolerances, from the arithmetic of the kernels:
   until that holds for every sequence.
 """
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -213,6 +214,28 @@ def test_pages_many_tokens(hip, B, n):
     assert check_extend(d, h, list(range(B))[::-1], [0] * B, [n - b % 7 for b in range(B)]) == 0
 
 
+def test_pages_without_a_limit_on_tokens(hip):
+    """T_cap as large as it can be: the call takes what the tokens need."""
+    d, h = DevicePages(3, 400, 900, 16), pr.Pages(3, 400, 900, 16)
+    d.reset()
+    assert check_extend(d, h, [2, 0], [0, 0], [5000, 37], 2 ** 31 - 1) == 0
+    assert check_extend(d, h, [2, 1], [5000, 0], [0, 0], 2 ** 31 - 1) == 0
+
+
+def test_pages_of_a_slot_in_one(hip):
+    """One page that is as long as a slot can be: counts of rows next to 2^31."""
+    most = 2 ** 31 - 1024
+    d = DevicePages(2, 1, 1, most)
+    d.load(np.full((2, 1), -1), np.zeros(2), [0])
+    assert d.extend([1], [most - 3], [4], 9, 4)[0] == -2
+    st, got = d.extend([1], [most - 3], [3], 9, 3)
+    assert st == 0 and list(got[3][:3]) == [most - 3, most - 2, most - 1]
+    table, held, free, n = d.state()
+    assert table[1, 0] == 0 and list(held) == [0, 1] and n == 0
+    assert d.trim([1], [2 ** 31 - 1]) == 0 and d.state()[3] == 0
+    assert d.trim([1], [0]) == 0 and d.state()[3] == 1
+
+
 # -- a cache ------------------------------------------------------------------------
 class Cache:
     """Pools of n_pages pages in shuffled order behind a table; rows that no sequence has cached hold NaN and
@@ -344,6 +367,22 @@ def test_store(hip, dtype, layout, Hkv, hd, page, T):
         both = np.isnan(got) & np.isnan(want)
         assert np.all(both | (got.view(np.uint16 if dtype == F16 else np.uint32) ==
                               want.view(np.uint16 if dtype == F16 else np.uint32)))
+
+
+def test_store_more_rows_than_workgroups(hip):
+    T, hd = 70001, 8
+    rng = np.random.default_rng(4)
+    d = DevicePages(1, 1, 40, 2048)
+    pools = [dev(np.zeros(40 * 2048 * hd, np.uint16)) for _ in range(2)]
+    kv = slate_amd.PagedKv(pools[0].ptr, pools[1].ptr, BF16, 1, hd, 2048 * hd, 0, hd)
+    x = [rng.normal(0, 1, (T, hd)).astype(np.float32) for _ in range(2)]
+    row = rng.permutation(40 * 2048)[:T].astype(np.int32)
+    bufs = [dev(x[0]), dev(x[1]), dev(row)]
+    ok(lib().slate_hip_kv_store_paged(C.byref(kv), d.ref, bufs[0].p, bufs[1].p, hd, bufs[2].p, T))
+    for pool, v in zip(pools, x):
+        want = np.zeros((40 * 2048, hd), np.uint16)
+        want[row] = to_type(v, BF16)
+        assert np.array_equal(pool.to_array(np.uint16, want.shape), want)
 
 
 # -- attention --------------------------------------------------------------------------
@@ -599,6 +638,28 @@ def test_attention_workspace_content(hip):
         r.check()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_attention_is_the_same_every_time(hip, dtype):
+    """The order of sums goes by the lengths alone; and several threads call it at once."""
+    c = Cache([(5000, 5), (40, 1), (0, 3), (777, 2)], 2, 128, 16, dtype, 0, 21)
+    r = Attend(c, 8)
+    r.call()
+    r.check()
+    first = r.result()
+    others = [Attend(c, 8) for _ in range(3)]
+
+    def work(o):
+        for _ in range(8):
+            o.call()
+    threads = [threading.Thread(target=work, args=(o,)) for o in others]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for o in others:
+        assert np.array_equal(o.result().view(np.uint32), first.view(np.uint32))
+
+
 # -- verification -----------------------------------------------------------------------
 class Drafts:
     """A batch of drafts on host and device; near() says how far the reference keeps from its borders."""
@@ -703,6 +764,35 @@ def test_verify_many_sequences(hip, B, kind):
 @pytest.mark.parametrize("kind", ["probs", "plain", "tree"])
 def test_verify_one_long_draft(hip, kind):
     Drafts([300, 2], 50, kind, 6).call().check()
+
+
+def test_verify_most_drafts(hip):
+    """1024 drafts are taken, one more is not."""
+    d = Drafts([1025, 2, 1026, 3], 12, "plain", 14, scale=0.3, temps=[3, 1, 1, 1],
+               edit=lambda d, rng: d.u.__imul__(np.float32(0.02)))
+    d.want[2] = None
+    d.call().check()
+    assert len(d.want[0][0]) > 70                      # over more than a wave's lanes
+    d = Drafts([1025, 1], 12, "tree", 14, scale=0.3, temps=[3, 1])
+    d.call().check()
+
+
+def test_verify_at_the_border(hip):
+    """u q equal to p turns a draft down: two tokens of 1/2 each, q 1/2 and 1 (numbers without rounding)."""
+    V, B = 2, 4
+    z = dev(np.zeros((2 * B, V), np.float32))
+    tok = dev(np.tile([0, 1], B), np.int32)
+    q = dev(np.tile(np.array([[0.5, 0.5], [0.0, 1.0]], np.float32), (B, 1)))
+    u = np.zeros(2 * B, np.float32)
+    u[1::2] = [0.5, np.nextafter(np.float32(0.5), np.float32(0)), 0.25, 0.0]
+    r = dev(np.full(B, 0.9, np.float32))
+    ud, off = dev(u), dev(np.arange(0, 2 * B + 1, 2), np.int32)
+    for probs in (q.p, None):
+        outs = [DeviceBuffer(4 * B), DeviceBuffer(8 * B)]
+        ok(lib().slate_hip_verify_drafts(outs[0].p, outs[1].p, None, z.p, V, tok.p, None, probs, V, None, ud.p, r.p, off.p,
+                                         B, 2 * B, V, None, 0))
+        assert list(outs[0].to_array(np.int32, B)) == [0, 1, 1, 1]
+        assert list(outs[1].to_array(np.int32, (B, 2))[0]) == [0, -1]      # what is left is the other token
 
 
 @pytest.mark.parametrize("kind", ["probs", "plain", "tree"])
