@@ -556,6 +556,20 @@ def test_attention_v_of_any_size(hip, dtype, scale, n):
     r.check()
 
 
+@pytest.mark.parametrize("seed", range(3))
+@pytest.mark.parametrize("scale", [1e-7, 1e-6, 1e-5, 1e-4])
+@pytest.mark.parametrize("seq", [(12, 1), (330, 5), (1700, 1), (700, 16)])
+def test_attention_v_below_normal(hip, seq, scale, seed):
+    """V in f16 around and below its normal numbers: as good as any, each sequence by itself."""
+    c = Cache([seq], 2, 128, 16, F16, 0, seed)
+    c.values["V"][0] = to_type((of_type(c.values["V"][0], F16) * scale).astype(np.float32), F16)
+    c.pools["V"][c.where(0, np.arange(sum(seq)))] = c.values["V"][0]
+    c.v.upload(c.pools["V"])
+    r = Attend(c, 4)
+    r.call()
+    r.check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("scale", [2.0 ** -12, 30.0])
 def test_attention_scores_of_any_size(hip, dtype, scale):
