@@ -30,7 +30,11 @@ namespace slate_hip {
 __host__ __device__ constexpr int paged_wgs(int hd) { return hd > 128 ? 256 : 512; }
 constexpr int AP_SLICE = 32;           // keys of a wave within a granule
 constexpr int AP_GRAN = 4 * AP_SLICE;  // keys of a granule
-constexpr int AP_KEEP = 4;             // blocks of up to this many granules are not cut
+// Up to this many granules a sequence no block of a call is cut, which spares the joining
+// kernel; longer calls cut where the ranges end, also their short blocks.  Decode, bf16, 8
+// kv heads of 128, us cut / not cut: one sequence of 333 keys 10.4 / 9.1, one of 1000 10.9 /
+// 10.7, 16 of up to 512 14.3 / 16.2, 32 19.7 / 17.4, 64 27.8 / 24.1, 256 91.0 / 87.4.
+constexpr int AP_SHORT = 8;
 
 typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
@@ -46,19 +50,22 @@ struct PagedCount {
     }
 };
 
+// Whether a call's blocks may be cut.
+__host__ __device__ constexpr bool paged_cuts(int max_seq) { return paged_granules(max_seq) > AP_SHORT; }
+
 // Where workgroup w's range begins (the place there is for x < plan.total): N w / P,
-// or the start of the block there if it is short.
+// or the start of the block there where none is cut.
 struct PagedBegin {
     int x;
     Place place;
 };
 template <int WGS, class PlanT>
-__device__ __forceinline__ PagedBegin paged_begin(const PlanT& plan, int w) {
+__device__ __forceinline__ PagedBegin paged_begin(const PlanT& plan, int w, bool cuts) {
     PagedBegin b{plan.begin(w, WGS), {}};
     if (b.x >= plan.total) return PagedBegin{plan.total, {}};
     b.place = plan.find(b.x);
-    const int gran = paged_granules(b.place.seq.p0 + b.place.seq.n), in = b.place.at % gran;
-    if (gran <= AP_KEEP) {
+    if (!cuts) {
+        const int in = b.place.at % paged_granules(b.place.seq.p0 + b.place.seq.n);
         b.x -= in;
         b.place.at -= in;
     }
@@ -192,7 +199,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
     using PlanT = Plan<PagedCount<ROWS>, PagedBatch>;
     const PagedCount<ROWS> count{G, Hkv};
     const PlanT plan(pb, count);
-    const PagedBegin begin = paged_begin<WGS>(plan, blockIdx.x);
+    const bool cuts = paged_cuts(pb.max_seq);
+    const PagedBegin begin = paged_begin<WGS>(plan, blockIdx.x, cuts);
     const int x0 = begin.x;
     if (x0 >= plan.total) {
         if (threadIdx.x == 0) entry_of(a.ws, blockIdx.x)->rows = 0;
@@ -412,7 +420,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
     Where wh = start_piece();
     load_k(pc, wh);
     load_v(pc, wh);
-    const int x1 = paged_begin<WGS>(plan, blockIdx.x + 1).x;
+    const int x1 = paged_begin<WGS>(plan, blockIdx.x + 1, cuts).x;
     if (x0 >= x1) {                                    // the block is another workgroup's
         if (threadIdx.x == 0) entry_of(a.ws, blockIdx.x)->rows = 0;
         return;
@@ -420,7 +428,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
     pc.g1 = min(pc.gran, pc.g0 + (x1 - x0));
     load_q(pc);
     if (w == 0)
-        leave_entry(a.ws, WGS, blockIdx.x, x0, pc.g0, pc.gran, plan, [&](int v) { return paged_begin<WGS>(plan, v).x; },
+        leave_entry(a.ws, WGS, blockIdx.x, x0, pc.g0, pc.gran, plan,
+                    [&](int v) { return paged_begin<WGS>(plan, v, cuts).x; },
                     JoinEntry{pc.seq.t0, min(ROWS, pc.seq.n * G - pc.r0), pc.r0, pc.h, 0, 0});
     if (QLDS) __syncthreads();
 
@@ -744,7 +753,7 @@ static void launch_paged_rows(const PagedAttn& a, const PagedBatch& pb, hipStrea
         hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, false, 16>), grid, th, 0, s, a, pb);
     else
         hipLaunchKernelGGL((attn_paged_kernel<E, HD, RT, RW, true, 16>), grid, th, 0, s, a, pb);
-    if (paged_granules(pb.max_seq) > AP_KEEP)          // else no block is cut
+    if (paged_cuts(pb.max_seq))
         launch_attn_join_paged(a.out, a.ws, a.Hq, a.kv.n_kv_heads, a.kv.head_dim, HD, 16 * RT * RW, paged_wgs(HD), s);
 }
 
