@@ -130,16 +130,22 @@ __global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ 
             m = mt;
             l *= f;
             o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+            // PAGED: eight parts summed before they are added, so that up to 512 of one size do not
+            // round the same way one by one
+            float l8 = PAGED ? 0.f : l;
+            float4 o8 = PAGED ? make_float4(0.f, 0.f, 0.f, 0.f) : o;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float fk = __builtin_amdgcn_exp2f(ml[k].x - mt);
                 if (fk == 0.f) continue;
-                l += fk * ml[k].y;
-                o.x += fk * v[k].x;
-                o.y += fk * v[k].y;
-                o.z += fk * v[k].z;
-                o.w += fk * v[k].w;
+                l8 += fk * ml[k].y;
+                o8.x += fk * v[k].x;
+                o8.y += fk * v[k].y;
+                o8.z += fk * v[k].z;
+                o8.w += fk * v[k].w;
             }
+            l = PAGED ? l + l8 : l8;
+            o = PAGED ? make_float4(o.x + o8.x, o.y + o8.y, o.z + o8.z, o.w + o8.w) : o8;
         }
         if (PAGED && c >= hd) return;
         const float inv = PAGED && l == 0.f ? 0.f : 1.0f / l;

@@ -571,6 +571,26 @@ def test_attention_v_below_normal(hip, seq, scale, seed):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("v", [1.0, 2.0 ** -20])
+@pytest.mark.parametrize("score", [8.0, 12.3, 13.6, 15.1])
+def test_attention_many_small_weights(hip, dtype, v, score):
+    """One key far above 16000 that weigh alike: their weights' roundings all go the same way."""
+    c = Cache([(16000, 1)], 1, 128, 16, dtype, 0, 4)
+    r = Attend(c, 1)
+    q = r.q[0, 0].astype(np.float64)
+    K, V = np.zeros((16001, 1, 128)), np.full((16001, 1, 128), v)
+    K[5, 0] = score * 128 ** 0.5 * q / (q @ q)
+    V[5, 0] = -3 * v
+    for name, x in (("K", K), ("V", V)):
+        c.values[name][0] = to_type(x.astype(np.float32), dtype)
+        c.pools[name][c.where(0, np.arange(16001))] = c.values[name][0]
+    c.k.upload(c.pools["K"])
+    c.v.upload(c.pools["V"])
+    r.call()
+    r.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("scale", [2.0 ** -12, 30.0])
 def test_attention_scores_of_any_size(hip, dtype, scale):
     """Scores near 0 (all weights alike) and in the hundreds (one key takes all)."""
