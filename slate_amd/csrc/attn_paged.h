@@ -19,6 +19,16 @@
 // f16: Q (scaled by a power of two) and the weights (times 2^11) as two halves, 22
 // bits; bf16: as three, 24 bits; f32: f32 MFMAs.  Sums are f32.  A row's running
 // maximum moves only when a score passes it by 2^4.
+//
+// With 8 kv heads of 128 (a 4 GiB copy runs at 4.77 TB/s):
+//  - one token of 64 users, 4 query heads, f16, up to 16384 keys: 439 us, 5.95 TB/s;
+//  - of 16 users, bf16, up to 4096 keys: 41 us, the joining kernel 4.7 of it and about 3
+//    until the first keys are there (plan, table), the rest at 5.9 TB/s;
+//  - 3 to 5 tokens of 16 users, f32, up to 8192 keys: 133 us, 4.8 TB/s; the f32 MFMAs are
+//    busy for 61 % of that time;
+//  - 4 to 8 tokens of 8 users, 8 query heads, bf16, up to 16384 keys: 100 us, 3.65 TB/s;
+//    matrix unit 35 %, vector unit 37 %, waves wait in 27 % of their cycles, two a SIMD (64
+//    rows a wave, one a SIMD: 120 us).
 #pragma once
 #include "attn_plan.h"
 #include "attn_rows.h"
@@ -748,6 +758,8 @@ void launch_attention_paged_type<_Float16>(const PagedAttn& a, const PagedBatch&
 template <>
 void launch_attention_paged_type<__bf16>(const PagedAttn& a, const PagedBatch& pb, hipStream_t s);
 
+// Pages of whole tiles of 16 rows are looked up by the tile, others by four rows or, of odd
+// sizes, by the row (decode of 16, bf16, pages of 16 rows: 41, 46 and 54 us).
 template <class E, int HD, int RT, int RW>
 static void launch_paged_rows(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
     const dim3 grid(paged_wgs(HD)), th(256);
@@ -763,19 +775,30 @@ static void launch_paged_rows(const PagedAttn& a, const PagedBatch& pb, hipStrea
         launch_attn_join_paged(a.out, a.ws, a.Hq, a.kv.n_kv_heads, a.kv.head_dim, HD, 16 * RT * RW, paged_wgs(HD), s);
 }
 
+// Rows of a block, by the query rows that a kv head's sequences bring (of the longest, 8 kv
+// heads, us a call; 16 / 32 / 64 rows in a block):
+//  - 4 rows (one token of 4 heads, 16 sequences, bf16 of 128): 41 / 45 / -;
+//  - 20 rows (5 tokens of 4 heads, 16 sequences, bf16 of 128): 93 / 84 / 87, of 64: - / 48 / 52;
+//  - 64 rows (8 tokens of 8 heads, 8 sequences of up to 16384 keys, of 128): bf16 138 / 120 /
+//    101, f32 - / 187 / 194; prompt chunks of 600 tokens: bf16 - / 390 / 276, f32 - / 776 / 766.
+// 64 rows share K and V between two groups of waves, which f32's products are too long to
+// gain by (16 sequences of 5 tokens of 8 heads: 193 / 211).  head_dim 256 has registers for
+// 16 rows a wave; two groups of waves, 32 rows, take 76 us where 16 rows take 86 (64 rows,
+// bf16), and 1040 where they take 1397 (chunks).
 template <class E>
 static void launch_paged_hd(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
+    constexpr int MOST = sizeof(E) == 4 ? 1 : 2;       // groups of waves
     const int64_t rows = (int64_t)pb.max_new * (a.Hq / a.kv.n_kv_heads);
     if (a.kv.head_dim > 128)
         rows <= 16 ? launch_paged_rows<E, 256, 1, 1>(a, pb, s) : launch_paged_rows<E, 256, 1, 2>(a, pb, s);
     else if (a.kv.head_dim > 64)
         rows <= 16   ? launch_paged_rows<E, 128, 1, 1>(a, pb, s)
         : rows <= 32 ? launch_paged_rows<E, 128, 2, 1>(a, pb, s)
-                     : launch_paged_rows<E, 128, 2, 2>(a, pb, s);
+                     : launch_paged_rows<E, 128, 2, MOST>(a, pb, s);
     else
         rows <= 16   ? launch_paged_rows<E, 64, 1, 1>(a, pb, s)
         : rows <= 32 ? launch_paged_rows<E, 64, 2, 1>(a, pb, s)
-                     : launch_paged_rows<E, 64, 2, 2>(a, pb, s);
+                     : launch_paged_rows<E, 64, 2, MOST>(a, pb, s);
 }
 
 }  // namespace slate_hip
