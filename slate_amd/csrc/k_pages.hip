@@ -6,7 +6,9 @@
 namespace slate_hip {
 
 constexpr int PGS_MAX_TH = 1024;       // threads of the one workgroup: a sequence each
-constexpr int PGS_FEW = 256;           // up to as many sequences in a workgroup of as many threads
+// Up to as many sequences in a workgroup of as many threads (64 sequences: extend 3.5 us and
+// trim 2.4, with 1024 threads 4.3 and 2.9).
+constexpr int PGS_FEW = 256;
 constexpr int PGS_HASH = 2048;
 // Tokens whose rows the workgroup that takes the pages finds itself; more are left to
 // workgroups of their own where T_cap has room for more (64 sequences: 768 tokens 5.5 us
@@ -234,7 +236,7 @@ __global__ __launch_bounds__(TH) void pages_trim_kernel(Pages pg, const int32_t*
 // ---------------------------------------------------------------------------
 // Rows rounded to the pools' type: 8 elements a thread, so that heads and rows
 // of any stride are written 16 (f32: 32) bytes at a time.  Memory bound: 5.9 TB/s for
-// 5592 tokens of 8 heads of 128 (12 us; f32 read, f16 written), 2.3 us for 16 tokens.
+// 5876 tokens of 8 heads of 128 (12 us; f32 read, f16 written), 2.4 us for 16 tokens.
 constexpr int ST_WGS = 65536;
 template <class E>
 struct Eight {

@@ -19,9 +19,9 @@ namespace slate_hip {
 
 constexpr int VF_CHUNK = 1024;         // logits of a wave: 16 a lane
 constexpr int VF_TH = 512;             // threads that walk a sequence
-// Workgroups of the sums: five waves a SIMD.  256 rows of 128256 logits take 34.4 us (3.8
-// TB/s; 27.5 with no exponentials), 35.8 with four, 38 with six, 47 with eight, which
-// leave the compiler fewer registers.
+// Workgroups of the sums: five waves a SIMD.  254 rows of 128256 logits take 31 to 34 us
+// (130 MB, 4 TB/s; 27.5 with no exponentials); where they took 34.4, four waves took 35.8,
+// six 38 and eight 47, which leave the compiler fewer registers.
 constexpr int VF_SUM_WGS = 1280;
 constexpr int VF_ROWS = PK_MAX_DRAFT + 1;
 
@@ -392,7 +392,9 @@ __device__ int pick_token(int nch, float u, const Mass& mass, const Values& valu
 }
 
 // One workgroup per sequence: its rows' sums joined, its drafts' chances, the walk,
-// and the next token where no draft's probability has to be taken off.
+// and the next token where no draft's probability has to be taken off.  Latency: 4.4 us
+// for one sequence, 8.4 for 64 of four drafts, 10.5 for 16 trees of eight, whose
+// tokens turned down have a chunk each summed again.
 __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
     __shared__ double s_sum[VF_ROWS], s_p[VF_ROWS], s_u[VF_ROWS];
     __shared__ float s_top[VF_ROWS], s_z[VF_ROWS];
@@ -554,6 +556,7 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
 // of a sequence the token.  The masses pass between workgroups of other XCDs, so they
 // and the count of workgroups are written and read past the L2 (relaxed atomics of the
 // device's scope; a workgroup's count follows its masses by the wait between them).
+// 8 us for one sequence (latency), 13 for 64 (66 MB, 5 TB/s).
 constexpr int VL_TH = 256;
 __global__ __launch_bounds__(VL_TH) void verify_less_kernel(VerifyArgs a) {
     __shared__ double s_part[VL_TH / 64];
