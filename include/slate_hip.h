@@ -388,10 +388,9 @@ int   slate_hip_kv_store_paged(const slate_hip_paged_kv_t* kv, const slate_hip_p
  * bits; over f16 ones 22, and a weight is resolved to 2^-35 of the largest.
  * Made for few tokens a sequence (decode steps, drafts): K and V are read once for
  * every 16 query rows of a kv head where max_new brings no more, else for every 32 or 64
- * (head_dim above 128: 32).  T * n_q_heads <=
- * 2^31 - 128, and n_kv_heads * (T * n_q_heads / n_kv_heads / 16 + B) * max_pages *
- * page_size / 128 stays below 2^31.  ws as for attention_ragged_q8, of
- * slate_hip_attention_paged_bytes. */
+ * (f32, and head_dim above 128: 32).  T * n_q_heads <= 2^31 - 128, and n_kv_heads * (T *
+ * n_q_heads / n_kv_heads / 16 + B) * max_pages * page_size / 128 stays below 2^31.  ws as
+ * for attention_ragged_q8, of slate_hip_attention_paged_bytes. */
 int   slate_hip_attention_paged(float* out, const float* q, const slate_hip_paged_kv_t* kv,
                                 const slate_hip_pages_t* pages, const int32_t* slot, const int32_t* tok_off,
                                 const int32_t* pos0, int B, int T, int max_new, int n_q_heads, void* ws,
@@ -422,9 +421,10 @@ int64_t slate_hip_attention_paged_bytes(int n_q_heads, int n_kv_heads, int head_
  * float[T], at the drafts) and u_next (float[B]) are uniform in [0, 1).  Tokens
  * outside 0 .. V-1 never stand.  q is not negative.  All T rows of logits are read.
  * Outputs (device): n_accepted[b] (-1 for a sequence that is left out: without rows, with
- * more than 1024 drafts, outside 0 .. T, or behind a fall of tok_off); out_tok[T]: in a sequence's rows the accepted tokens, the next
- * one (-1: no p), then -1; out_row[T] (or NULL): the rows that were accepted,
- * counted within the sequence, then -1.  Rows that no sequence owns stay as they were.
+ * more than 1024 drafts, outside 0 .. T, or behind a fall of tok_off); out_tok[T]: in a
+ * sequence's rows the accepted tokens, the next one (-1: no p), then -1; out_row[T] (or
+ * NULL): the rows that were accepted, counted within the sequence, then -1.  Rows that no
+ * sequence owns stay as they were.
  * Probabilities, sums and comparisons are in 64 bits, exponentials good to 2^-42.  V is at
  * most 2^31 - 1024.
  * ws: device scratch of slate_hip_verify_drafts_bytes, as for attention_ragged_q8. */

@@ -590,6 +590,19 @@ def test_attention_many_small_weights(hip, dtype, v, score):
     r.check()
 
 
+@pytest.mark.parametrize("spare", [0, 1])
+@pytest.mark.parametrize("dtype,Hkv,hd,G,n,B", [(BF16, 8, 64, 1, 1, 70), (F16, 2, 128, 4, 1, 3), (F32, 1, 64, 8, 5, 9),
+                                                (BF16, 1, 256, 4, 9, 5), (F16, 16, 64, 2, 1, 50)])
+def test_attention_slots_of_1024_rows(hip, dtype, Hkv, hd, G, n, B, spare):
+    """Slots of 1024 rows and of a page more, full and nearly empty ones, more blocks than workgroups and fewer."""
+    rng = np.random.default_rng(B)
+    seqs = [(1024 - n, n)] + [(int(rng.choice([0, 1, 127, 128, 900, 1024 - n])), n) for _ in range(B - 1)]
+    r = Attend(Cache(seqs, Hkv, hd, 16, dtype, 0, 3, spare=spare), G)
+    assert r.c.d.shape[1] == 64 + spare
+    r.call()
+    r.check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("scale", [2.0 ** -12, 30.0])
 def test_attention_scores_of_any_size(hip, dtype, scale):
