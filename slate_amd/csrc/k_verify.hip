@@ -76,7 +76,8 @@ class Weights {
     // has: none above 2^512 and one above 2^-512, so that what counts as 2^-900
     // below shows in no sum (infinities, NaN, temperatures without an end: no).
     __device__ __forceinline__ bool takes(float top) const {
-        return most_ < 1e38f && most_ > 1e-30f && !__builtin_amdgcn_ballot_w64(top > most_) && __builtin_amdgcn_ballot_w64(top > -most_);
+        return most_ < 1e38f && most_ > 1e-30f && !__builtin_amdgcn_ballot_w64(top > most_) &&
+               __builtin_amdgcn_ballot_w64(top > -most_);
     }
     __device__ __forceinline__ double operator()(float x) const {
         constexpr double WHOLE = 6755399441055744.0;   // 1.5 2^52: a sum with it is a whole number in its low bits
@@ -427,7 +428,8 @@ __global__ __launch_bounds__(VF_TH) void verify_walk_kernel(VerifyArgs a) {
         s_parent[i] = up;
         const bool in = up >= 0 && x >= 0 && x < V;
         s_z[i] = in ? a.logits[(int64_t)(t0 + up) * a.ld + x] : -INFINITY;
-        s_u[i] = in ? a.u[t0 + i] * (a.q ? (double)a.q[(int64_t)(t0 + i) * a.q_ld + x] : 1.0) : INFINITY;   // infinite: never
+        const double q = in && a.q ? (double)a.q[(int64_t)(t0 + i) * a.q_ld + x] : 1.0;
+        s_u[i] = in ? a.u[t0 + i] * q : INFINITY;      // infinite: never
     }
     for (int i = VF_TH / 64 - 1 - w; i < n; i += VF_TH / 64) {
         const Part p = row_part(sp.part + (int64_t)(t0 + i) * nch, nch, heat);

@@ -163,7 +163,8 @@ int slate_hip_verify_drafts(int32_t* n_accepted, int32_t* out_tok, int32_t* out_
                             const float* temperature, const float* u, const float* u_next, const int32_t* tok_off,
                             int B, int T, int V, void* ws, size_t ws_bytes) {
     SH_REQUIRE(n_accepted && out_tok && logits && token && u && u_next && tok_off, "verify_drafts: null pointer");
-    SH_REQUIRE(B >= 1 && B <= PK_MAX_SEQ && T >= 1 && V >= 1 && V <= PK_MAX_KEYS, "verify_drafts: bad sizes (B=%d, T=%d, V=%d)", B, T, V);
+    SH_REQUIRE(B >= 1 && B <= PK_MAX_SEQ && T >= 1 && V >= 1 && V <= PK_MAX_KEYS,
+               "verify_drafts: bad sizes (B=%d, T=%d, V=%d)", B, T, V);
     SH_REQUIRE(ld >= V && (!draft_probs || draft_ld >= V), "verify_drafts: rows of %d, ld=%lld, draft_ld=%lld", V,
                (long long)ld, (long long)draft_ld);
     SH_REQUIRE(!draft_probs || !parent, "verify_drafts: draft_probs are for chains (parent NULL)");
