@@ -449,7 +449,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
         const int rw = r0 + GROUP * rg;                // the group's first row
         const int all_see = sv.p0 + rw / G;            // the last key that all of its rows see
         const int own = min(GROUP, r0 + rows - rw);    // its rows: it may have none
-        const bool mixed = (rw + own - 1) / G != rw / G;
+        const int most = sv.p0 + (rw + own - 1) / G;   // the last key that any of them sees
+        const bool mixed = most != all_see;
         int lim[RT];                                   // the last key that row j sees
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -512,11 +513,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
             }
             load_k(pc, wh);
             __builtin_amdgcn_sched_barrier(0);
-            // keys that not all rows see, or that are not there
+            // keys that not all rows see; V of those that none sees or that are not there is taken out
             if (k0 + KS - 1 > all_see || !at.good) {
                 auto there = [&](int key) {            // a key of the step, counted from k0
                     const bool page = P16 ? at.tgood[NT == 1 ? 0 : key >> 4] : (at.there >> key / P & 1) != 0;
-                    return page && k0 + key <= last;
+                    return page && k0 + key <= most;
                 };
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
