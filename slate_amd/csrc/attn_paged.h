@@ -723,10 +723,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attn_paged_kernel(Paged
             float lt = 0.f;
 #pragma unroll
             for (int k = w0; k < w0 + KW; ++k) {
-                // a maximum of -infinity with a sum: scores that are NaN, kept
+                // a maximum of -infinity with a sum: scores that are NaN, kept; and 0 times NaN or infinity is NaN, so
+                // that these are seen whatever weight their part has
                 const float f = s_m[k][rl] == -INFINITY ? (s_l[k][rl] == 0.f ? 0.f : 1.f)
                                                         : __builtin_amdgcn_exp2f(s_m[k][rl] - mt);
-                if (f == 0.f) continue;
                 lt += f * s_l[k][rl];
                 sum += f * *(const floatx4*)&s_o[k][rl][c];
             }

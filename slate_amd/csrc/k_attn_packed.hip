@@ -136,8 +136,8 @@ __global__ __launch_bounds__(JOIN_TH) void attn_join_kernel(float* __restrict__ 
             float4 o8 = PAGED ? make_float4(0.f, 0.f, 0.f, 0.f) : o;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float fk = __builtin_amdgcn_exp2f(ml[k].x - mt);
-                if (fk == 0.f) continue;
+                if (ml[k].x == -INFINITY) continue;    // no part, or one that saw no key
+                const float fk = __builtin_amdgcn_exp2f(ml[k].x - mt);     // (0 too: times NaN or infinity it is NaN)
                 l8 += fk * ml[k].y;
                 o8.x += fk * v[k].x;
                 o8.y += fk * v[k].y;

@@ -5,10 +5,22 @@ Tolerances as in test_gpu_paged.py; what a value must not change is equal bit fo
 import numpy as np
 import pytest
 
-from tests.test_gpu_paged import BF16, F16, F32, Attend, Cache, to_type
+from tests import test_gpu_packed as packed
+from tests.test_gpu_paged import BF16, F16, F32, Attend, Cache, of_type, to_type
 
 pytestmark = pytest.mark.gpu
 WILD = (np.nan, np.inf, -np.inf)
+
+
+def put(c, name, b, x):
+    """Sequence b's K or V rows x [rows, Hkv, hd] on the host; upload() sends them."""
+    c.values[name][b] = to_type(np.asarray(x, np.float32), c.dtype)
+    c.pools[name][c.where(b, np.arange(len(x)))] = c.values[name][b]
+
+
+def upload(c):
+    c.k.upload(c.pools["K"])
+    c.v.upload(c.pools["V"])
 
 
 def with_value(c, name, b, row, col, value):
@@ -40,3 +52,60 @@ def test_a_draft_does_not_reach_the_tokens_before_it(hip, hd, G, p, dtype):
             assert not np.isfinite(got[at:n, :, 5]).any()
             assert np.array_equal(np.delete(got[at:n], 5, 2), np.delete(clean[at:n], 5, 2))
     c.v.upload(c.pools["V"])
+
+
+def hot(c, r, b, row, score):
+    """K's row of kv head 0 gets about this score from every query of the batch, the others stay around 0."""
+    rng = np.random.default_rng(3)
+    base = rng.normal(0, 1, c.hd)
+    r.q = (base + 0.1 * rng.normal(0, 1, r.q.shape)).astype(np.float32)
+    r.qd.upload(r.q)
+    K = of_type(c.values["K"][b], c.dtype)
+    K[row, 0] = score * c.hd ** 0.5 * base / (base @ base)
+    put(c, "K", b, K)
+    upload(c)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("p,top,low", [(700, 5, 40), (700, 690, 70), (20000, 5, 15000), (20000, 19990, 70)])
+@pytest.mark.parametrize("n,G", [(1, 4), (3, 8), (8, 8)])
+def test_a_value_reaches_every_token_that_sees_it(hip, n, G, p, top, low, dtype):
+    """A key that takes all of the weight does not hide a NaN or an infinity in another part of the cache."""
+    c = Cache([(p, n)], 1, 64, 16, dtype, 0, 8)
+    r = Attend(c, G)
+    hot(c, r, 0, top, 300.0)
+    r.call()
+    clean = r.result()[:n]
+    assert np.isfinite(clean).all()
+    for what in WILD:
+        c.v.upload(with_value(c, "V", 0, low, 7, what))
+        r.call()
+        got = r.result()[:n]
+        assert not np.isfinite(got[:, :, 7]).any(), what
+        assert np.array_equal(np.delete(got, 7, 2), np.delete(clean, 7, 2)), what
+    c.v.upload(c.pools["V"])
+    c.k.upload(with_value(c, "K", 0, low, 7, np.nan))
+    r.call()
+    assert np.isnan(r.result()[:n]).all()
+
+
+@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("top,low", [(5, 15000), (19990, 70)])
+def test_a_tree_sees_a_value_beside_a_key_that_takes_all(hip, top, low, n):
+    """The same over the slots of f32 rows, whose ranges are joined by the same kernel."""
+    p, hd, G = 20000, 64, 2
+    rng = np.random.default_rng(5)
+    bt = packed.Batch([(p, n), (50, 2)], 1, hd, p + 100, rng)
+    pools = packed.fill_f32(bt, 3)
+    base = rng.normal(0, 1, hd)
+    at = bt.row(0, 0, top)
+    pools["K"][at:at + hd] = 300.0 * hd ** 0.5 * base / (base @ base)
+    at = bt.row(0, 0, low)
+    pools["V"][at:at + hd] = np.nan
+    r = packed.Run(bt, G, False, 3, packed.random_parents(bt, rng, "random"), pools=pools)
+    r.q = (base + 0.1 * rng.normal(0, 1, r.q.shape)).astype(np.float32)
+    r.qd.upload(r.q)
+    r.call()
+    out = r.result()
+    assert np.isnan(out[:n]).all()
+    assert np.isfinite(out[n:]).all()
