@@ -710,15 +710,17 @@ __global__ __launch_bounds__(AM_TH, 2) void attn_many_kernel(PackedAttn a, Packe
                 const float* at = area + ((k - 1) * tiles + tile) * AR_TILE * OS + j * OS;
                 const float2 ml = *(const float2*)(at + HD);
                 const float mt = fmaxf(R.m, ml.x);
-                const float f0 = R.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(R.m - mt);
-                const float f1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mt);
+                // (a part that saw no key is left out; any other, if its factor is 0, still has its NaN and infinities)
+                const bool none0 = R.m == -INFINITY, none1 = ml.x == -INFINITY;
+                const float f0 = none0 ? 0.f : __builtin_amdgcn_exp2f(R.m - mt);
+                const float f1 = none1 ? 0.f : __builtin_amdgcn_exp2f(ml.x - mt);
                 R.m = mt;
                 l = l * f0 + ml.y * f1;
 #pragma unroll
                 for (int n = 0; n < ND; ++n) {
                     const floatx4 other = *(const floatx4*)(at + 16 * n + 4 * g);
-                    R.o[n] = (f0 == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : R.o[n] * f0) +
-                             (f1 == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : other * f1);
+                    R.o[n] = (none0 ? floatx4{0.f, 0.f, 0.f, 0.f} : R.o[n] * f0) +
+                             (none1 ? floatx4{0.f, 0.f, 0.f, 0.f} : other * f1);
                 }
             }
         }

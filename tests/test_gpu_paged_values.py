@@ -90,9 +90,9 @@ def test_a_value_reaches_every_token_that_sees_it(hip, n, G, p, top, low, dtype)
 
 
 @pytest.mark.parametrize("n", [3, 40])
-@pytest.mark.parametrize("top,low", [(5, 15000), (19990, 70)])
+@pytest.mark.parametrize("top,low", [(5, 15000), (19990, 70), (70, 100), (100, 70)])
 def test_a_tree_sees_a_value_beside_a_key_that_takes_all(hip, top, low, n):
-    """The same over the slots of f32 rows, whose ranges are joined by the same kernel."""
+    """The same over the slots of f32 rows, whose parts are joined in the kernel and whose ranges by the same one."""
     p, hd, G = 20000, 64, 2
     rng = np.random.default_rng(5)
     bt = packed.Batch([(p, n), (50, 2)], 1, hd, p + 100, rng)
