@@ -362,7 +362,9 @@ int   slate_hip_pages_extend(const slate_hip_pages_t* pages, const int32_t* slot
 /* Give back the pages behind the first length[b] rows (device int32[B]; 0: all)
  * of slot[b]: of requests that end, of drafts that did not stand.  The pages
  * that pages_extend just took come back in the order in which they lay there.
- * status as above (-1 also where the stack would hold more than n_pages). */
+ * status as above (-1 also where the stack would hold more than n_pages, or where
+ * an entry that would go back names no page).  A page goes back for every slot that
+ * names it: of slots that share pages all but one are cleared by the caller. */
 int   slate_hip_pages_trim(const slate_hip_pages_t* pages, const int32_t* slot, const int32_t* length, int B,
                            int32_t* status);
 /* New K and V rows into their pages: k, v [T, n_kv_heads * head_dim] f32 (16-byte

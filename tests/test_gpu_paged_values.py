@@ -5,8 +5,9 @@ Tolerances as in test_gpu_paged.py; what a value must not change is equal bit fo
 import numpy as np
 import pytest
 
+from tests import paged_ref as pr
 from tests import test_gpu_packed as packed
-from tests.test_gpu_paged import BF16, F16, F32, Attend, Cache, of_type, to_type
+from tests.test_gpu_paged import BF16, F16, F32, Attend, Cache, DevicePages, of_type, same_pages, to_type
 
 pytestmark = pytest.mark.gpu
 WILD = (np.nan, np.inf, -np.inf)
@@ -109,3 +110,39 @@ def test_a_tree_sees_a_value_beside_a_key_that_takes_all(hip, top, low, n):
     out = r.result()
     assert np.isnan(out[:n]).all()
     assert np.isfinite(out[n:]).all()
+
+
+# -- pages ------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [-1, 25, -2 ** 31, 2 ** 31 - 1])
+@pytest.mark.parametrize("at", [(0, 2), (3, 0), (5, 9)])
+def test_trim_refuses_what_is_no_page(hip, at, bad):
+    """An entry among those that would go back names no page: refused, and nothing is given back."""
+    d, h = DevicePages(6, 10, 25, 4), pr.Pages(6, 10, 25, 4)
+    d.reset()
+    assert d.extend([3, 0, 5], [0, 0, 0], [9, 12, 40], 99)[0] == 0
+    assert h.extend([3, 0, 5], [0, 0, 0], [9, 12, 40], 99)[0] == 0
+    table, held, free, n = d.state()
+    broken = table.copy()
+    broken[at] = bad
+    d.load(broken, held, free[:n])
+    before = d.state()
+    assert d.trim([1, 5, 3, 0], [0, 0, 0, 0]) == -1
+    for a, b in zip(before, d.state()):
+        assert np.array_equal(a, b)
+    keep = [40 if s == at[0] else 4 for s in (5, 3, 0)]        # the entry stays where it is: as before
+    assert d.trim([5, 3, 0], keep) == 0 == h.trim([5, 3, 0], keep)
+    h.table[at] = bad
+    same_pages(d, h)
+
+
+@pytest.mark.parametrize("B,n", [(1, 100000), (3, 40001), (300, 333)])
+def test_trim_of_many_pages(hip, B, n):
+    """More pages than the workgroup takes in a round."""
+    d, h = DevicePages(B, n // 16 + 1, 9000, 16), pr.Pages(B, n // 16 + 1, 9000, 16)
+    d.reset()
+    slot = list(range(B))[::-1]
+    for p, k in ((0, [n - b % 7 for b in range(B)]), (16, [b % 40 for b in range(B)])):
+        assert d.extend(slot, [p] * B, k, 1 << 20)[0] == 0 == h.extend(slot, [p] * B, k, 1 << 20)[0]
+        keep = [b % 3 * 16 + b % 2 for b in range(B)]
+        assert d.trim(slot, keep) == 0 == h.trim(slot, keep)
+        same_pages(d, h)
