@@ -1,13 +1,15 @@
 """The cache in pages and the verification of drafts at values, scores and sizes far from the ordinary ones.
 
-Tolerances as in test_gpu_paged.py; what a value must not change is equal bit for bit.
+Tolerances as in test_gpu_paged.py: outputs are held in the 2-norm to 2^-18, here each group of columns by itself (a
+score is off by about 2^-22 and a weight by as much, so what a weight adds to an output is too; 2^-18 leaves 16 times
+that); what a value must not change is equal bit for bit.
 """
 import numpy as np
 import pytest
 
 from tests import paged_ref as pr
 from tests import test_gpu_packed as packed
-from tests.test_gpu_paged import BF16, F16, F32, Attend, Cache, DevicePages, of_type, same_pages, to_type
+from tests.test_gpu_paged import BF16, F16, F32, NORM_TOL, Attend, Cache, DevicePages, of_type, same_pages, to_type
 
 pytestmark = pytest.mark.gpu
 WILD = (np.nan, np.inf, -np.inf)
@@ -110,6 +112,56 @@ def test_a_tree_sees_a_value_beside_a_key_that_takes_all(hip, top, low, n):
     out = r.result()
     assert np.isnan(out[:n]).all()
     assert np.isfinite(out[n:]).all()
+
+
+# -- f16 below its normal numbers -----------------------------------------------------
+def columns_good(r, b, columns):
+    c, (p, n) = r.c, r.c.seqs[b]
+    tk = np.arange(c.off[b], c.off[b + 1])
+    for h in range(c.Hkv):
+        q = r.q[tk][:, h * r.G:(h + 1) * r.G].astype(np.float64)
+        want, _, _ = pr.attend(q, c.rows(b, "K", h), c.rows(b, "V", h), p, c.hd)
+        got = r.result()[tk][:, h * r.G:(h + 1) * r.G]
+        err = np.linalg.norm((got - want)[..., columns]) / np.linalg.norm(want[..., columns])
+        assert err <= NORM_TOL, (h, err)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -16, 2.0 ** -19, 2.0 ** -21])
+@pytest.mark.parametrize("hd,G,seq", [(64, 4, (12, 1)), (128, 4, (900, 1)), (128, 4, (900, 5)), (128, 8, (3000, 8)),
+                                      (256, 4, (330, 6)), (80, 3, (500, 2))])
+def test_small_columns_of_f16(hip, hd, G, seq, scale):
+    """Columns of V around and below the smallest normal number, beside ordinary ones, are as good as those."""
+    c = Cache([seq, (40, 1)], 2, hd, 16, F16, 0, 11)
+    small = np.zeros(hd, bool)
+    small[8:16] = small[hd - 3] = small[33] = True
+    for b in range(2):
+        x = of_type(c.values["V"][b], F16)
+        x[..., small] *= scale
+        put(c, "V", b, x)
+    upload(c)
+    r = Attend(c, G)
+    r.call()
+    r.check()
+    for b in range(2):
+        columns_good(r, b, small)
+        columns_good(r, b, ~small)
+
+
+@pytest.mark.parametrize("value", [1.0, 6.2e-5, -60000.0])
+@pytest.mark.parametrize("p,n,G", [(50, 5, 4), (1000, 3, 8), (20, 2, 40)])
+def test_a_draft_does_not_change_small_values_before_it(hip, p, n, G, value):
+    """V below the normal numbers, a later draft's above: the tokens before it stay as they were, bit for bit."""
+    c = Cache([(p, n)], 1, 128, 16, F16, 0, 12)
+    put(c, "V", 0, of_type(c.values["V"][0], F16) * 2.0 ** -21)
+    upload(c)
+    r = Attend(c, G)
+    r.call()
+    clean = r.result()
+    c.v.upload(with_value(c, "V", 0, p + n - 1, 5, value))
+    r.call()
+    got = r.result()
+    assert np.array_equal(got[:n - 1], clean[:n - 1])
+    assert np.array_equal(np.delete(got[n - 1], 5, 1), np.delete(clean[n - 1], 5, 1))
 
 
 # -- pages ------------------------------------------------------------------------------
