@@ -385,10 +385,12 @@ int   slate_hip_kv_store_paged(const slate_hip_paged_kv_t* kv, const slate_hip_p
  * cache holds in rows that a token does not see never matters, not even infinities
  * and NaN; one in V of a row that it sees makes that column of its output not
  * finite, a NaN in K all of it.
- * Queries must be finite and below 2^100 in size, and so must bf16 and f32 K and V.  Sums
- * are f32 (outputs below 2^-100 in size lose bits).  f32 caches are multiplied in f32;
- * over bf16 ones queries and weights have 24 bits; over f16 ones 22, and a weight is
- * resolved to 2^-35 of the largest.
+ * Queries must be finite and below 2^100 in size, and so must bf16 and f32 K and V (V below
+ * 2^90 where slots have more than 2^23 rows); over those the sum of the |q_i k_i| of a token
+ * and a row that it sees must be below 2^126.  Sums are f32 (outputs below 2^-100 in size
+ * lose bits).  f32 caches are multiplied in f32; over bf16 ones queries and weights have 24
+ * bits; over f16 ones 22, where a weight is resolved to 2^-35 of the largest and an element
+ * of a query to 2^-37 of its row's largest.
  * Made for few tokens a sequence (decode steps, drafts): K and V are read once for
  * every 16 query rows of a kv head where max_new brings no more, else for every 32 or 64
  * (f32, and head_dim above 128: 32).  T * n_q_heads <= 2^31 - 128, and n_kv_heads * (T *

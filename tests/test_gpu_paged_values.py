@@ -164,6 +164,56 @@ def test_a_draft_does_not_change_small_values_before_it(hip, p, n, G, value):
     assert np.array_equal(np.delete(got[n - 1], 5, 1), np.delete(clean[n - 1], 5, 1))
 
 
+@pytest.mark.parametrize("size,some", [(2.0 ** 16, False), (2.0 ** 20, False), (2.0 ** 22, False), (2.0 ** 16, True)])
+@pytest.mark.parametrize("hd,G,seq", [(128, 4, (900, 1)), (128, 4, (900, 5)), (64, 8, (3000, 8)), (256, 4, (330, 6))])
+def test_small_keys_of_f16(hip, hd, G, seq, size, some):
+    """K below the normal numbers under large queries: scores as good as any.  `some`: in two of three columns; the
+    other queries, `size` smaller, are off by at most 2^-38 of the row's largest (4 size), 2^-20 of themselves."""
+    c = Cache([seq], 2, hd, 16, F16, 0, 13)
+    small = np.ones(hd, bool)
+    if some:
+        small[::3] = False
+    K = of_type(c.values["K"][0], F16)
+    K[..., small] /= size
+    put(c, "K", 0, K)
+    upload(c)
+    r = Attend(c, G)
+    r.q[..., small] *= np.float32(size)
+    r.qd.upload(r.q)
+    r.call()
+    r.check()
+
+
+# -- scores of any size ---------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("p,n,G", [(300, 1, 4), (300, 5, 8), (5000, 3, 4)])
+def test_scores_next_to_the_largest(hip, p, n, G, dtype):
+    """Sums of |q k| just below 2^126: the key with the largest score is all that counts, so an output is its V."""
+    hd = 64
+    c = Cache([(p, n)], 1, hd, 16, dtype, 0, 14)
+    r = Attend(c, G)
+    for seed in range(20):
+        rng = np.random.default_rng(seed)
+        K = rng.normal(0, 1, (p + n, 1, hd)) * 2.0 ** 60
+        put(c, "K", 0, K)
+        K = c.rows(0, "K", 0)
+        q = rng.normal(0, 1, (n, G, hd))
+        most = (np.abs(q) @ np.abs(K).T).max()
+        r.q[:n] = (q * (0.99 * 2.0 ** 126 / most)).astype(np.float32)
+        s = r.q[:n].astype(np.float64) @ K.T
+        for i in range(n):
+            s[i, :, p + i + 1:] = -np.inf
+        two = np.sort(s, 2)[..., -2:]
+        if ((two[..., 1] - two[..., 0]) > 2.0 ** -16 * 2.0 ** 126).all():      # hd 2^-24 of 2^126 is 2^-18 of it
+            break
+    else:
+        raise AssertionError("no inputs away from ties")
+    upload(c)
+    r.qd.upload(r.q)
+    r.call()
+    assert np.array_equal(r.result()[:n], c.rows(0, "V", 0)[s.argmax(2)].astype(np.float32))
+
+
 # -- pages ------------------------------------------------------------------------------
 @pytest.mark.parametrize("bad", [-1, 25, -2 ** 31, 2 ** 31 - 1])
 @pytest.mark.parametrize("at", [(0, 2), (3, 0), (5, 9)])
