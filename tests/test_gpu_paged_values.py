@@ -9,7 +9,8 @@ import pytest
 
 from tests import paged_ref as pr
 from tests import test_gpu_packed as packed
-from tests.test_gpu_paged import BF16, F16, F32, NORM_TOL, Attend, Cache, DevicePages, of_type, same_pages, to_type
+from tests.test_gpu_paged import (BF16, F16, F32, NORM_TOL, Attend, Cache, DevicePages, Drafts, of_type,
+                                  same_pages, to_type)
 
 pytestmark = pytest.mark.gpu
 WILD = (np.nan, np.inf, -np.inf)
@@ -248,3 +249,32 @@ def test_trim_of_many_pages(hip, B, n):
         keep = [b % 3 * 16 + b % 2 for b in range(B)]
         assert d.trim(slot, keep) == 0 == h.trim(slot, keep)
         same_pages(d, h)
+
+
+# -- large vocabularies --------------------------------------------------------------------
+@pytest.mark.parametrize("kind,V,chunks", [("probs", 560000, 256), ("plain", 1060000, 512), ("tree", 1060000, 512)])
+def test_verify_more_chunks_than_threads(hip, kind, V, chunks):
+    """Vocabularies whose chunks of 1024 are summed in several rounds: the next token in the first, a middle and the
+    last round, at both ends of u_next, and behind chunks that have no weight."""
+    end = np.float32(1.0 - 2.0 ** -24)
+
+    def edit(d, rng):
+        for b, place in enumerate((9, chunks * 1024 + 5, V - 2)):
+            t = int(d.off[b])
+            d.z[t, place:place + 2] = d.z[t].max() + np.float32(6.0)
+            d.r[b] = 0.4
+        t = int(d.off[3])
+        d.z[t, V - 3 * 1024:] = -np.inf
+        d.r[3] = end
+        t = int(d.off[4])
+        d.z[t, :chunks * 1024 + 700] = -np.inf
+        d.r[4] = 0.0
+        if kind == "probs":
+            d.token[t + 1] = 0                         # a banned one: p has gone to the others
+        d.u[d.off[:5] + 1] = end                       # drafts are turned down
+    d = Drafts([2, 2, 2, 3, 2, 1], V, kind, 15, edit=edit, temps=[1.0] * 6)
+    assert [w[1] // (chunks * 1024) for w in d.want[:5]][:3] == [0, 1, (V - 2) // (chunks * 1024)]
+    assert d.want[4][1] >= chunks * 1024 + 700 and d.want[3][1] < V - 3 * 1024
+    assert all(len(w[0]) == 0 for w in d.want[:5])
+    d.call().check()
+    d.call(own_ws=True).check()
