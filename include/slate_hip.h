@@ -370,7 +370,7 @@ int   slate_hip_pages_trim(const slate_hip_pages_t* pages, const int32_t* slot, 
 /* New K and V rows into their pages: k, v [T, n_kv_heads * head_dim] f32 (16-byte
  * aligned), rows ld floats apart (ld % 4 == 0), rounded to the pools' type to
  * nearest, ties to even.  A row whose tok_row is outside 0 .. n_pages * page_size - 1
- * is stored nowhere; of two rows with the same tok_row either may stay. */
+ * is stored nowhere; where two rows have the same tok_row each element is either's. */
 int   slate_hip_kv_store_paged(const slate_hip_paged_kv_t* kv, const slate_hip_pages_t* pages, const float* k,
                                const float* v, int64_t ld, const int32_t* tok_row, int T);
 /* Causal GQA attention of new tokens over the pages: q, out [T, n_q_heads *

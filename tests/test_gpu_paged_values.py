@@ -4,12 +4,15 @@ Tolerances as in test_gpu_paged.py: outputs are held in the 2-norm to 2^-18, her
 score is off by about 2^-22 and a weight by as much, so what a weight adds to an output is too; 2^-18 leaves 16 times
 that); what a value must not change is equal bit for bit.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 
+import slate_amd
 from tests import paged_ref as pr
 from tests import test_gpu_packed as packed
-from tests.test_gpu_paged import (BF16, F16, F32, NORM_TOL, Attend, Cache, DevicePages, Drafts, of_type,
+from tests.test_gpu_paged import (BF16, F16, F32, NORM_TOL, Attend, Cache, DevicePages, Drafts, dev, lib, of_type, ok,
                                   same_pages, to_type)
 
 pytestmark = pytest.mark.gpu
@@ -249,6 +252,22 @@ def test_trim_of_many_pages(hip, B, n):
         keep = [b % 3 * 16 + b % 2 for b in range(B)]
         assert d.trim(slot, keep) == 0 == h.trim(slot, keep)
         same_pages(d, h)
+
+
+def test_rows_stored_to_the_same_place(hip):
+    """Tokens with one cache row: each of its elements is one of theirs, and nothing else changes."""
+    T, Hkv, hd, ps = 40, 3, 64, 4
+    d = DevicePages(1, 2, 2, ps)
+    pools = [dev(np.zeros(2 * Hkv * ps * hd, np.float32)) for _ in range(2)]
+    kv = slate_amd.PagedKv(pools[0].ptr, pools[1].ptr, F32, Hkv, hd, Hkv * ps * hd, ps * hd, hd)
+    x = [np.random.default_rng(k).normal(0, 1, (T, Hkv, hd)).astype(np.float32) for k in range(2)]
+    rows, src = dev(np.full(T, 5), np.int32), [dev(v) for v in x]
+    ok(lib().slate_hip_kv_store_paged(C.byref(kv), d.ref, src[0].p, src[1].p, Hkv * hd, rows.p, T))
+    for pool, v in zip(pools, x):
+        got = pool.to_array(np.float32, (2, Hkv, ps, hd))
+        assert (got[1, :, 1] == v).any(0).all()
+        got[1, :, 1] = 0
+        assert not got.any()
 
 
 # -- large vocabularies --------------------------------------------------------------------
