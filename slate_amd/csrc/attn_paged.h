@@ -26,7 +26,7 @@
 //    until the first keys are there (plan, table), the rest at 5.9 TB/s;
 //  - 3 to 5 tokens of 16 users, f32, up to 8192 keys: 133 us, 4.8 TB/s; the f32 MFMAs are
 //    busy for 61 % of that time;
-//  - 4 to 8 tokens of 8 users, 8 query heads, bf16, up to 16384 keys: 100 us, 3.65 TB/s;
+//  - 4 to 8 tokens of 8 users, 8 query heads, bf16, up to 16384 keys: 97 us, 3.75 TB/s;
 //    matrix unit 35 %, vector unit 37 %, waves wait in 27 % of their cycles, two a SIMD (64
 //    rows a wave, one a SIMD: 120 us).
 #pragma once
@@ -40,9 +40,10 @@ namespace slate_hip {
 __host__ __device__ constexpr int paged_wgs(int hd) { return hd > 128 ? 256 : 512; }
 constexpr int AP_SLICE = 32;           // keys of a wave within a granule
 constexpr int AP_GRAN = 4 * AP_SLICE;  // keys of a granule
-// Up to this many granules a sequence no block of a call is cut, which spares the joining
-// kernel; longer calls cut where the ranges end, also their short blocks.  Decode, bf16, 8
-// kv heads of 128, us cut / not cut: one sequence of 333 keys 10.4 / 9.1, one of 1000 10.9 /
+// Where slots have room for no more than this many granules no block is cut, which spares
+// the joining kernel; calls over larger slots cut where the ranges end, also blocks of short
+// sequences (the host knows what a slot can hold, not the lengths).  Decode, bf16, 8 kv heads
+// of 128, us cut / not cut: one sequence of 333 keys 10.4 / 9.1, one of 1000 10.9 /
 // 10.7, 16 of up to 512 14.3 / 16.2, 32 19.7 / 17.4, 64 27.8 / 24.1, 256 91.0 / 87.4.
 constexpr int AP_SHORT = 8;
 
@@ -790,7 +791,9 @@ template <>
 void launch_attention_paged_type<__bf16>(const PagedAttn& a, const PagedBatch& pb, hipStream_t s);
 
 // Pages of whole tiles of 16 rows are looked up by the tile, others by four rows or, of odd
-// sizes, by the row (decode of 16, bf16, pages of 16 rows: 41, 46 and 54 us).
+// sizes, by the row (decode of 16, bf16, pages of 16 rows: 41, 46 and 54 us; the addresses
+// take registers, and the 16-bit kernels of head_dim 128 keep 36 to 152 bytes a lane in
+// scratch memory there).
 template <class E, int HD, int RT, int RW>
 static void launch_paged_rows(const PagedAttn& a, const PagedBatch& pb, hipStream_t s) {
     const dim3 grid(paged_wgs(HD)), th(256);
@@ -806,8 +809,9 @@ static void launch_paged_rows(const PagedAttn& a, const PagedBatch& pb, hipStrea
         launch_attn_join_paged(a.out, a.ws, a.Hq, a.kv.n_kv_heads, a.kv.head_dim, HD, 16 * RT * RW, paged_wgs(HD), s);
 }
 
-// Rows of a block, by the query rows that a kv head's sequences bring (of the longest, 8 kv
-// heads, us a call; 16 / 32 / 64 rows in a block):
+// Rows of a block, by the query rows that a kv head's sequences may bring (max_new decides
+// for the whole call: beside a prompt chunk decode rows lie in its large blocks).  8 kv heads,
+// us a call; 16 / 32 / 64 rows in a block:
 //  - 4 rows (one token of 4 heads, 16 sequences, bf16 of 128): 41 / 45 / -;
 //  - 20 rows (5 tokens of 4 heads, 16 sequences, bf16 of 128): 93 / 84 / 87, of 64: - / 48 / 52;
 //  - 64 rows (8 tokens of 8 heads, 8 sequences of up to 16384 keys, of 128): bf16 138 / 120 /

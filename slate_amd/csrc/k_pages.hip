@@ -11,8 +11,9 @@ constexpr int PGS_MAX_TH = 1024;       // threads of the one workgroup: a sequen
 constexpr int PGS_FEW = 256;
 constexpr int PGS_HASH = 2048;
 // Tokens whose rows the workgroup that takes the pages finds itself; more are left to
-// workgroups of their own where T_cap has room for more (64 sequences: 768 tokens 5.5 us
-// in one kernel and 6.7 in two, 1536 tokens 7.5 and 7.3).
+// workgroups of their own where T_cap has room for more (us a call, in one kernel and in
+// two: 64 sequences, 1024 tokens 5.7 and 7.7, 1536 6.7 and 7.7, 2048 7.7 and 7.6; 4
+// sequences, 2048 tokens 5.6 and 6.5).
 constexpr int PGS_OWN_TOKENS = 2048;
 
 // Sums over the workgroup, each thread bringing a count below 2^31: the
